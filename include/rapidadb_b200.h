@@ -87,6 +87,37 @@ int rdb_distance(int metric, int dtype, const void* q, int64_t nq, const void* x
 /* Squared L2 norm of each row of x [n, d] (fp32 accumulation). */
 int rdb_row_sqnorms(int dtype, const void* x, int64_t n, int d, float* out, void* stream);
 
+/* Softmax cross entropy of nq queries against every row of a base, and its
+ * gradients (no reference counterpart: the reference trains nothing but its
+ * k-means stub).  With s_bn = scale * <q_b, x_n>:
+ *   loss_b = log sum_n exp(s_bn) - s_b,t(b),  0 where targets[b] == ignore_index
+ *   dq = G x, dx = G^T q,  G_bn = g_b scale (softmax(s_b)_n - [n = t(b)])
+ * The [nq, n] logits are never kept.  q [nq, d], x [n, d] in `dtype`, row
+ * strides multiples of 16 bytes and 16-byte aligned bases; targets [nq] int64;
+ * scale > 0.  A target that is neither ignore_index nor in [0, n) makes that
+ * query's loss, and the gradients it enters, NaN; what an ignored query row
+ * holds (NaN included) reaches nothing.
+ *   reduction  RDB_REDUCE_NONE: loss [nq]; _MEAN (over the queries that are
+ *              not ignored; NaN when all are) / _SUM: loss [1].
+ *   stats      [3, nq] fp32, saved for the backward pass: row 0 the largest
+ *              logit m, row 1 log2 sum 2^(s' - m), both of s' = s log2 e;
+ *              log sum exp = ln 2 (row 0 + row 1); row 2 the query's loss.
+ *   grad       of the loss: [nq] or [1] as the loss, fp32.
+ *   dq / dx    gradients in `dtype` (NULL: not wanted); sums over queries and
+ *              rows run in fp32 in a fixed order. */
+#define RDB_REDUCE_NONE 0
+#define RDB_REDUCE_MEAN 1
+#define RDB_REDUCE_SUM 2
+size_t rdb_softmax_xent_workspace(int dtype, int64_t nq, int64_t n, int d, int reduction);
+int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
+                     const int64_t* targets, float scale, int64_t ignore_index, int reduction, float* loss,
+                     float* stats, void* ws, size_t ws_bytes, void* stream);
+size_t rdb_softmax_xent_backward_workspace(int dtype, int64_t nq, int64_t n, int d, int need_dq, int need_dx);
+int rdb_softmax_xent_backward(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n,
+                              int64_t ldx, int d, const int64_t* targets, float scale, int64_t ignore_index,
+                              int reduction, const float* grad, const float* stats, void* dq, int64_t lddq, void* dx,
+                              int64_t lddx, void* ws, size_t ws_bytes, void* stream);
+
 /* Per-row metric value from squared norms: |x|^2 (L2), sqrt|x|^2 or
  * sqrt(|x|^2 + 1e-8) (cosine, d > 128 / d <= 128), 0 (dot).  out may alias sq. */
 int rdb_vec_values(int metric, int d, const float* sq, int64_t n, float* out, void* stream);
@@ -146,6 +177,16 @@ int rdb_sq8_encode(int dtype, const void* x, int64_t n, int64_t ldx, int d, int8
                    void* stream);
 int rdb_sq8_row_values(int metric, const int8_t* codes, const float* scales, int64_t n, int64_t ldc, int d,
                        float* out, void* stream);
+/* Scores of int8 codes (no reference counterpart; the int8 form of
+ * dot_product_cuda, csrc/kernels/distance.cu:566-610):
+ *   out[b, n] = (qs[b] * xs[n]) * sum_t qc[b, t] * xc[n, t]
+ * qc [nq, d] and xc [n, d] int8 codes with one fp32 scale per row (as
+ * rdb_sq8_encode writes them; any int8 value is accepted), row strides
+ * multiples of 16 bytes and bases 16-byte aligned; d <= 131071 keeps the
+ * integer sum exact in 32 bits.  out [nq, n] in out_dtype (RDB_F32 / F16 /
+ * BF16; rounded once from fp32), row stride ldo elements. */
+int rdb_sq8_dot(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
+                int64_t n, int64_t ldx, int d, int out_dtype, void* out, int64_t ldo, void* stream);
 size_t rdb_flat_search_sq8_workspace(int metric, int64_t nq, int64_t n, int d, int k, int flags);
 int rdb_flat_search_sq8(int metric, const float* q, int64_t nq, int64_t ldq, const int8_t* codes, const float* scales,
                         int64_t n, int64_t ldx, const float* xv, int d, int k, const int64_t* ids, int64_t id_offset,

@@ -40,6 +40,37 @@ PYBIND11_MODULE(_C, m) {
     m.def("dot_product", [](const at::Tensor& q, const at::Tensor& x) { return distance(Metric::DOT_PRODUCT, q, x); },
           "Dot product matrix [Q, N]", py::arg("queries"), py::arg("database"), py::call_guard<py::gil_scoped_release>());
 
+    // ---- int8 scores: the quantiser of a user's own rows and the product of codes
+    m.def("sq8_encode", &sq8_encode, "int8 codes [n, dim] and scales [n] of float rows", py::arg("vectors"),
+          py::call_guard<py::gil_scoped_release>());
+    m.def("sq8_dot_product", &sq8_dot_product,
+          "Dot product matrix [Q, N] of int8 codes with a scale per query and per row", py::arg("query_codes"),
+          py::arg("query_scales"), py::arg("codes"), py::arg("scales"), py::arg("dtype") = at::kFloat,
+          py::call_guard<py::gil_scoped_release>());
+    // ---- training: rapidadb_b200.losses wraps these for autograd
+    m.def("softmax_cross_entropy", &softmax_cross_entropy,
+          "softmax cross entropy of queries against every database row: (loss, stats)", py::arg("queries"),
+          py::arg("database"), py::arg("targets"), py::arg("scale") = 1.0, py::arg("ignore_index") = -100,
+          py::arg("reduction") = RDB_REDUCE_MEAN, py::call_guard<py::gil_scoped_release>());
+    m.def(
+        "softmax_cross_entropy_backward",
+        [](const at::Tensor& grad, const at::Tensor& q, const at::Tensor& x, const at::Tensor& t, const at::Tensor& stats,
+           double scale, int64_t ignore_index, int reduction, bool need_queries, bool need_database) {
+            Result r;
+            {
+                py::gil_scoped_release nogil;
+                r = softmax_cross_entropy_backward(grad, q, x, t, stats, scale, ignore_index, reduction, need_queries,
+                                                   need_database);
+            }
+            // None for a gradient that was not asked for
+            return py::make_tuple(need_queries ? py::cast(std::get<0>(r)) : py::none(),
+                                  need_database ? py::cast(std::get<1>(r)) : py::none());
+        },
+        "gradients (queries, database) of softmax_cross_entropy", py::arg("grad"), py::arg("queries"),
+        py::arg("database"), py::arg("targets"), py::arg("stats"), py::arg("scale") = 1.0,
+        py::arg("ignore_index") = -100, py::arg("reduction") = RDB_REDUCE_MEAN, py::arg("need_queries") = true,
+        py::arg("need_database") = true);
+
     // ---- top-k (torch_extension.cpp:47-63)
     m.def("topk", [](const at::Tensor& d, int64_t k, bool largest) { return topk(d, k, largest); },
           "Sorted top-k per row", py::arg("distances"), py::arg("k"), py::arg("largest") = true, py::call_guard<py::gil_scoped_release>());

@@ -46,9 +46,10 @@ void sq8_encode_into(const at::Tensor& vectors, at::Tensor codes, at::Tensor sca
     at::Tensor v = vectors;
     if (!(v.scalar_type() == at::kFloat || v.scalar_type() == at::kHalf || v.scalar_type() == at::kBFloat16))
         v = v.to(at::kFloat);
-    if (v.stride(1) != 1) v = v.contiguous();
+    if (v.stride(1) != 1 || (n > 1 && v.stride(0) < v.size(1))) v = v.contiguous();
+    const int64_t ldv = n > 1 ? v.stride(0) : v.size(1);  // a single row may carry any stride
     TORCH_CHECK(codes.is_contiguous() || codes.stride(1) == 1, "codes rows must be dense");
-    check_status(rdb_sq8_encode(dtype_code(v.scalar_type()), v.data_ptr(), n, v.stride(0), static_cast<int>(v.size(1)),
+    check_status(rdb_sq8_encode(dtype_code(v.scalar_type()), v.data_ptr(), n, ldv, static_cast<int>(v.size(1)),
                                 codes.data_ptr<int8_t>(), codes.stride(0), scales.data_ptr<float>(), stream_ptr()),
                  "sq8 encode");
 }

@@ -42,6 +42,20 @@ Result topk_merge(const at::Tensor& vals, const at::Tensor& ids, int64_t k, bool
 at::Tensor select_threshold(const at::Tensor& scores, int64_t k, bool largest,
                             const c10::optional<at::Tensor>& out = c10::nullopt);
 
+// ------------------------------------------------- int8 scores and training --
+// SQ8 codes [n, d] and scales [n] of float rows (rdb_sq8_encode)
+Result sq8_encode(const at::Tensor& vectors);
+// [nq, n] scores of int8 codes, one scale per query and per row (rdb_sq8_dot)
+at::Tensor sq8_dot_product(const at::Tensor& query_codes, const at::Tensor& query_scales, const at::Tensor& codes,
+                           const at::Tensor& scales, at::ScalarType dtype);
+// softmax cross entropy of queries against every database row: (loss, stats),
+// and (dq, dx) (rdb_softmax_xent, rdb_softmax_xent_backward)
+Result softmax_cross_entropy(const at::Tensor& queries, const at::Tensor& database, const at::Tensor& targets,
+                             double scale, int64_t ignore_index, int reduction);
+Result softmax_cross_entropy_backward(const at::Tensor& grad, const at::Tensor& queries, const at::Tensor& database,
+                                      const at::Tensor& targets, const at::Tensor& stats, double scale,
+                                      int64_t ignore_index, int reduction, bool need_queries, bool need_database);
+
 // -------------------------------------------------------------- FlatIndex --
 // csrc/include/rapidadb/index/flat_index.h:12-53, csrc/index/flat_index.cpp
 class FlatIndex {

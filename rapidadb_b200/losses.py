@@ -1,0 +1,65 @@
+"""Training losses over a base of embeddings.
+
+``softmax_cross_entropy(queries, database, targets)`` is the retrieval loss of
+a query encoder (and, where they are trained, of the stored rows): every row of
+the database is a class, the logits are ``scale * queries @ database.T``, and
+``targets[b]`` is the row that query b should retrieve.  The [batch, n] logits
+are never kept: the forward pass streams the rows through the tensor cores with
+a running softmax, the backward pass recomputes them piece by piece (kernels in
+csrc/xent.cu).  The reference has no training beyond its k-means declaration
+(csrc/include/rapidadb/clustering/kmeans.h:9-24).
+"""
+from __future__ import annotations
+
+import torch
+
+from rapidadb_b200._lib import C
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+class _SoftmaxCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, queries, database, targets, scale, ignore_index, reduction):
+        loss, stats = C().softmax_cross_entropy(queries, database, targets, scale, ignore_index, reduction)
+        ctx.save_for_backward(queries, database, targets, stats)
+        ctx.call = (scale, ignore_index, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        queries, database, targets, stats = ctx.saved_tensors
+        dq, dx = C().softmax_cross_entropy_backward(grad, queries, database, targets, stats, *ctx.call,
+                                                    need_queries=ctx.needs_input_grad[0],
+                                                    need_database=ctx.needs_input_grad[1])
+        return dq, dx, None, None, None, None
+
+
+def softmax_cross_entropy(queries: torch.Tensor, database: torch.Tensor, targets: torch.Tensor,
+                          scale: float = 1.0, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of ``queries`` against every row of ``database``.
+
+    ``loss[b] = logsumexp_n(scale * <q_b, x_n>) - scale * <q_b, x_targets[b]>``
+
+    Args:
+        queries:      [batch, dim] CUDA tensor, float32 / float16 / bfloat16.
+        database:     [n, dim], same device and dtype, n >= 1 (e.g. the rows of
+                      an index, or a batch of positives for in-batch negatives).
+        targets:      [batch] int64 or int32 row numbers.  A query whose target
+                      is ``ignore_index`` has loss 0 and no gradient, whatever
+                      it holds; any other target outside [0, n) gives NaN.
+        scale:        inverse temperature, positive and finite.  (A learnable
+                      one: pass ``queries * temperature`` and ``scale=1``.)
+        reduction:    "mean" over the queries that are not ignored (NaN when
+                      all are), "sum" or "none" ([batch] losses).
+
+    The loss is float32; gradients have their tensor's dtype.  Gradients are
+    computed only for the inputs that require them, in a fixed order of sums
+    (the same inputs give the same bits), and once: there is no second
+    derivative.
+    """
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
+    return _SoftmaxCrossEntropy.apply(queries, database, targets, float(scale), int(ignore_index),
+                                      _REDUCTIONS[reduction])

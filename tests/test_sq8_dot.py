@@ -1,0 +1,251 @@
+"""Int8 scores: quantising a user's rows (_C.sq8_encode) and the product of
+codes with a scale per query and per row (_C.sq8_dot_product), against the
+oracle's codes and plain 64-bit arithmetic.
+
+The integer sum is exact, so an output is off by the roundings that follow it:
+sum -> fp32, qs * xs, and their product (2^-24 each), and one to the output
+type (half an eps of it)."""
+import numpy as np
+import pytest
+import torch
+
+import oracle
+
+U32 = 2.0 ** -24
+
+
+def _C():
+    import rapidadb._C as mod
+
+    return mod
+
+
+def codes_of(rng, n, d, lo=-128):
+    return torch.from_numpy(rng.integers(lo, 128, (n, d), dtype=np.int8)), \
+        torch.from_numpy(rng.uniform(1e-3, 2e-2, n).astype(np.float32))
+
+
+def check(out, qc, qs, xc, xs, dtype):
+    acc = qc.double() @ xc.double().T
+    ref = acc * qs.double()[:, None] * xs.double()[None, :]
+    # three fp32 roundings and the output's; fp16 may go below its normal range
+    tol = ref.abs() * (3.01 * U32 + torch.finfo(dtype).eps / 2 * (dtype != torch.float32)) + \
+        (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    assert out.dtype == dtype and out.shape == ref.shape
+    bad = (out.cpu().double() - ref).abs() > tol
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} outside, first {bad.nonzero()[0].tolist()}"
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals_without_gpu():
+    C = _C()
+    with pytest.raises(RuntimeError, match="vectors must be a CUDA tensor"):
+        C.sq8_encode(torch.randn(3, 4))
+    c, s = torch.zeros(3, 16, dtype=torch.int8), torch.ones(3)
+    with pytest.raises(RuntimeError, match="query_codes must be a CUDA tensor"):
+        C.sq8_dot_product(c, s, c, s)
+
+
+def test_abi_refusals_without_gpu():
+    """Every bad argument is rejected before any device work."""
+    import ctypes
+    import os
+
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(__file__), "..", "rapidadb_b200", "librdb_kernels.so"))
+    lib.rdb_last_error.restype = ctypes.c_char_p
+    i64, vp = ctypes.c_int64, ctypes.c_void_p
+    f = lib.rdb_sq8_dot
+    f.argtypes = [vp, vp, i64, i64, vp, vp, i64, i64, ctypes.c_int, ctypes.c_int, vp, i64, vp]
+    ok = dict(qc=1 << 20, qs=1 << 21, nq=2, ldq=16, xc=1 << 22, xs=1 << 23, n=4, ldx=16, d=16, t=0, out=1 << 24, ldo=4)
+    for kw, msg in [(dict(t=3), b"dtype"), (dict(d=0), b"shape"), (dict(ldq=8), b"shape"), (dict(ldo=3), b"shape"),
+                    (dict(d=131072, ldq=131072, ldx=131072), b"131071"), (dict(qc=None), b"NULL"),
+                    (dict(ldx=24), b"multiples of 16"), (dict(xc=(1 << 22) + 4), b"aligned"),
+                    (dict(n=1 << 31, ldo=1 << 31), b"2^31")]:
+        a = {**ok, **kw}
+        rc = f(a["qc"], a["qs"], a["nq"], a["ldq"], a["xc"], a["xs"], a["n"], a["ldx"], a["d"], a["t"], a["out"],
+               a["ldo"], None)
+        assert rc == 1 and msg in lib.rdb_last_error(), (kw, lib.rdb_last_error())
+    assert f(None, None, 0, 16, None, None, 4, 16, 16, 0, None, 4, None) == 0  # nothing to do
+
+
+@pytest.mark.gpu
+def test_refusals(device):
+    C = _C()
+    c, s = torch.zeros(3, 16, dtype=torch.int8, device=device), torch.ones(3, device=device)
+    for args, msg in [((c, s, c[:, :8], s), "dimension mismatch"), ((c, s[:2], c, s), "query_scales must be 1D"),
+                      ((c, s, c, s[:2]), "scales must be 1D"), ((c.int(), s, c, s), "codes must be int8"),
+                      ((c, s.double(), c, s), "scales must be float32"), ((c[0], s, c, s), "must be 2D"),
+                      ((c, s, c.cpu(), s), "CUDA"), ((c, s, c, s.cpu()), "same CUDA device"),
+                      ((c, s, c, s, torch.float64), "dtype must be"), ((c[:, :0], s, c[:, :0], s), "at least one")]:
+        with pytest.raises(RuntimeError, match=msg):
+            C.sq8_dot_product(*args)
+    with pytest.raises(RuntimeError, match="must be 2D"):
+        C.sq8_encode(s)
+    with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+        C.sq8_encode(s.double().reshape(1, 3))
+
+
+# -------------------------------------------------------------------- encode
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(1, 1), (5, 7), (33, 64), (9, 100), (70, 768), (3, 1025), (2, 5000)])
+def test_encode_equals_definition(device, n, d, dtype):
+    rng = np.random.default_rng(n * 1000 + d)
+    x = torch.from_numpy(rng.standard_normal((n, d), dtype=np.float32)).to(dtype)
+    x[0] = 0  # a zero row
+    if n > 2:
+        x[1] = 1e-41 if dtype == torch.float32 else 0.5  # subnormal rows; a constant row
+        x[2, 0] = 60000.0
+    codes, scales = _C().sq8_encode(x.to(device))
+    rc, rs = oracle.sq8_encode(x.float().numpy())
+    assert codes.dtype == torch.int8 and scales.dtype == torch.float32
+    assert np.array_equal(codes.cpu().numpy(), rc[:, :d]) and np.array_equal(scales.cpu().numpy(), rs)
+
+
+@pytest.mark.gpu
+def test_encode_strided_rows(device):
+    """Columns of a wider matrix, a transposed matrix, and an odd base offset."""
+    x = torch.randn(40, 301, device=device)
+    for v in (x[:, 3:103], x.t()[:100, :40], x[:, 1::3], x[::2, :64], x[:0]):
+        codes, scales = _C().sq8_encode(v)
+        rc, rs = oracle.sq8_encode(np.ascontiguousarray(v.cpu().numpy())) if len(v) else (np.zeros((0, 301)), np.zeros(0))
+        assert np.array_equal(codes.cpu().numpy(), rc[:, :v.shape[1]]) and np.array_equal(scales.cpu().numpy(), rs)
+
+
+# ------------------------------------------------------------------- product
+SIZES = [(1, 1, 1), (1, 1000, 768), (2, 37, 16), (3, 255, 100), (8, 129, 64), (9, 256, 128), (16, 300, 200),
+         (17, 513, 33), (32, 1000, 768), (33, 256, 129), (64, 31, 1024), (65, 700, 48), (127, 257, 512), (128, 1, 256),
+         (129, 520, 96), (255, 300, 130), (256, 256, 256), (257, 511, 640), (300, 2049, 144), (600, 90, 1000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nq,n,d", SIZES)
+def test_dot_product(device, nq, n, d, dtype):
+    rng = np.random.default_rng(nq * 7919 + n * 31 + d)
+    qc, qs = codes_of(rng, nq, d)
+    xc, xs = codes_of(rng, n, d)
+    out = _C().sq8_dot_product(qc.to(device), qs.to(device), xc.to(device), xs.to(device), dtype)
+    check(out, qc, qs, xc, xs, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 5, 40, 300])
+def test_extreme_codes_and_long_rows(device, nq):
+    """All codes at -128 / 127 and the largest allowed dimension: the integer
+    sum reaches 131071 * 2^14 < 2^31 and stays exact."""
+    n, d = 70, 131071
+    qc, xc = torch.full((nq, d), -128, dtype=torch.int8), torch.full((n, d), -128, dtype=torch.int8)
+    xc[1] = 127
+    xc[2, ::2] = 127
+    qs, xs = torch.rand(nq) + 0.5, torch.rand(n) + 0.5
+    out = _C().sq8_dot_product(qc.to(device), qs.to(device), xc.to(device), xs.to(device))
+    check(out, qc, qs, xc, xs, torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 6, 50, 290])
+def test_special_scales(device, nq):
+    """Zero, infinite and NaN scales act on their own query or row only."""
+    rng = np.random.default_rng(nq)
+    qc, qs = codes_of(rng, nq, 96, lo=1)
+    xc, xs = codes_of(rng, 300, 96, lo=1)
+    qs[nq // 2], xs[3], xs[7], xs[299] = 0.0, float("inf"), float("nan"), 0.0
+    out = _C().sq8_dot_product(qc.to(device), qs.to(device), xc.to(device), xs.to(device)).cpu()
+    ref = (qs.double()[:, None] * xs.double()[None, :]) * (qc.double() @ xc.double().T)
+    assert torch.equal(out.isnan(), ref.isnan()) and torch.equal(out.isinf(), ref.isinf())
+    assert (out[:, 299] == 0).all()
+    fin = ref.isfinite()
+    assert ((out.double() - ref).abs()[fin] <= 3.01 * U32 * ref.abs()[fin]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 4, 20, 270])
+def test_strided_operands(device, nq):
+    """Index rows (padded stride with other bytes behind the dimension), a
+    wider matrix's columns, odd bases and reversed orders."""
+    rng = np.random.default_rng(5)
+    d = 100
+    wide = torch.from_numpy(rng.integers(-127, 128, (600, 176), dtype=np.int8)).to(device)
+    qw = torch.from_numpy(rng.integers(-127, 128, (nq, 112), dtype=np.int8)).to(device)
+    s = torch.rand(1200, device=device) + 0.1
+    views = [wide[:, :d], wide[:, 16:16 + d], wide[:, 5:5 + d], wide[::2, :d], wide.t()[:d, :].t()[:, :d],
+             wide[:, :d].expand(600, d), wide[:1, :d].expand(7, d)]
+    for x in views:
+        for q in (qw[:, :d], qw[:, 7:7 + d]):
+            xs = s[:2 * x.shape[0]:2]  # strided scales
+            out = _C().sq8_dot_product(q, s[:nq], x, xs)
+            check(out, q.cpu(), s[:nq].cpu(), x.cpu(), xs.cpu(), torch.float32)
+
+
+@pytest.mark.gpu
+def test_empty_and_single(device):
+    C = _C()
+    c, s = torch.ones(3, 20, dtype=torch.int8, device=device), torch.ones(3, device=device)
+    assert C.sq8_dot_product(c[:0], s[:0], c, s).shape == (0, 3)
+    assert C.sq8_dot_product(c, s, c[:0], s[:0]).shape == (3, 0)
+    assert C.sq8_encode(torch.zeros(0, 8, device=device))[0].shape == (0, 8)
+    assert C.sq8_dot_product(c[:1, :1], s[:1], c[:1, :1], s[:1]).item() == 1.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 24, 300])
+def test_graph_stream_and_two_captures(device, nq):
+    """Side streams, a captured and replayed product with new inputs, and two
+    captured products replayed together."""
+    C = _C()
+    rng = np.random.default_rng(3)
+    qc, qs = codes_of(rng, nq, 128)
+    xc, xs = codes_of(rng, 500, 128)
+    qd, qsd, xd, xsd = (t.to(device) for t in (qc, qs, xc, xs))
+    want = C.sq8_dot_product(qd, qsd, xd, xsd)
+    st, st2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        a = C.sq8_dot_product(qd, qsd, xd, xsd)
+    with torch.cuda.stream(st2):
+        b = C.sq8_dot_product(qd, qsd, xd, xsd)
+    torch.cuda.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(C.sq8_dot_product(qd, qsd, xd, xsd))
+        graphs.append(g)
+    qc2, _ = codes_of(rng, nq, 128)
+    qd.copy_(qc2)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        graphs[0].replay()
+    with torch.cuda.stream(st2):
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        check(o, qc2, qs, xc, xs, torch.float32)
+
+
+@pytest.mark.gpu
+def test_scores_of_an_int8_index(device):
+    """The codes of a Flat INT8 index scored with quantised queries: close to
+    the index's exact scores, by the quantisation of the query alone."""
+    from rapidadb import IndexConfig, Metric, RapidaDB
+    from rapidadb_b200.config import Precision
+
+    C = _C()
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(2000, 100, generator=g).to(device)
+    q = torch.randn(9, 100, generator=g).to(device)
+    db = RapidaDB(config=IndexConfig(dim=100, metric=Metric.DOT_PRODUCT, precision=Precision.INT8))
+    db.add(x)
+    idx = db._index
+    codes, scales = idx.sq8_codes(), idx.sq8_scales()
+    qc, qs = C.sq8_encode(q)
+    s = C.sq8_dot_product(qc, qs, codes, scales)
+    check(s, qc.cpu(), qs.cpu(), codes.cpu(), scales.cpu(), torch.float32)
+    # a query coordinate moves by at most qs / 2
+    exact = q.double() @ (codes.double() * scales.double()[:, None]).T
+    slack = 0.501 * qs.double()[:, None] * (codes.double().abs() * scales.double()[:, None]).sum(1)[None, :]
+    assert ((s.double() - exact).abs() <= slack + 1e-4).all()
+    v, i = C.topk(s, 10, True)
+    assert torch.equal(v, s.gather(1, i)) and (v[:, :-1] >= v[:, 1:]).all()
