@@ -5,10 +5,18 @@
 // sum is an exact int32 (|code| <= 128 and d <= kMaxDim, so it stays below
 // 2^31); one fp32 product of the two scales and one with the sum follow, and
 // fp16 / bf16 outputs are rounded once from that fp32 value.
+//
+// Few queries: the codes of the rows are what has to be read, so a CUDA-core
+// kernel (dp4a) streams them once past query codes held in shared memory.
+// Otherwise the tcgen05 tile loop (kind::i8) with the rows as the tile's M: a
+// thread of the epilogue owns one row, so a warp's store of one query's scores
+// is 32 consecutive elements and needs no staging.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "common.cuh"
+#include <algorithm>
+
+#include "tile_tc.cuh"
 
 namespace rdb {
 namespace {
@@ -25,33 +33,185 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// one warp per (query, row)
+__device__ __forceinline__ float score(float qs, float xs, int acc) {
+    return __fmul_rn(__fmul_rn(qs, xs), static_cast<float>(acc));
+}
+
+// ------------------------------------------------------------ few queries --
+
+constexpr int GV_THREADS = 256;
+constexpr int GV_LANES = 8;               // lanes per row: 128 bytes of a row per load
+constexpr int GV_SMEM = 48 * 1024;        // query codes
+
+// NQ queries at most (rounded up to a power of two).  Four rows per warp.
+template <typename T, int NQ>
+__global__ void __launch_bounds__(GV_THREADS)
+    sq8_few_kernel(const int8_t* __restrict__ qc, const float* __restrict__ qs, int nq, int64_t ldq,
+                   const int8_t* __restrict__ xc, const float* __restrict__ xs, int64_t n, int64_t ldx, int d,
+                   T* __restrict__ out, int64_t ldo) {
+    extern __shared__ __align__(16) int8_t sq[];  // [NQ][dp], zero behind d and behind nq
+    const int dp = (d + 15) / 16 * 16, chunks = dp / 16;
+    for (int i = threadIdx.x; i < NQ * dp; i += GV_THREADS) {
+        const int b = i / dp, t = i - b * dp;
+        sq[i] = (b < nq && t < d) ? qc[b * ldq + t] : static_cast<int8_t>(0);
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, sub = lane & (GV_LANES - 1);
+    const int rows_per_block = GV_THREADS / GV_LANES;
+    const int full = d / 16;  // 16-byte chunks that lie inside the row
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows_per_block; r0 < n;
+         r0 += static_cast<int64_t>(gridDim.x) * rows_per_block) {
+        const int64_t r = r0 + threadIdx.x / GV_LANES;
+        const bool in = r < n;
+        const int8_t* x = xc + (in ? r : 0) * ldx;
+        int acc[NQ];
+#pragma unroll
+        for (int b = 0; b < NQ; ++b) acc[b] = 0;
+#pragma unroll 4
+        for (int c = sub; c < chunks; c += GV_LANES) {
+            int4 v;
+            if (c < full) {
+                v = __ldg(reinterpret_cast<const int4*>(x) + c);
+            } else {
+                // the row's last bytes: nothing behind them is read
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+                for (int t = c * 16; t < d; ++t)
+                    w[(t & 15) >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(x[t])) << (8 * (t & 3));
+                v = make_int4(w[0], w[1], w[2], w[3]);
+            }
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) {
+                const int4 q = *reinterpret_cast<const int4*>(sq + b * dp + c * 16);
+                acc[b] = __dp4a(v.x, q.x, acc[b]);
+                acc[b] = __dp4a(v.y, q.y, acc[b]);
+                acc[b] = __dp4a(v.z, q.z, acc[b]);
+                acc[b] = __dp4a(v.w, q.w, acc[b]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NQ; ++b)
+#pragma unroll
+            for (int o = GV_LANES / 2; o > 0; o >>= 1) acc[b] += __shfl_xor_sync(0xffffffffu, acc[b], o);
+        if (in) {
+            const float s = xs[r];
+#pragma unroll
+            for (int b = 0; b < NQ; ++b)
+                if (b < nq && (b & (GV_LANES - 1)) == sub) out[b * ldo + r] = from_f<T>(score(qs[b], s, acc[b]));
+        }
+    }
+}
+
+template <typename T, int NQ>
+int launch_few(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
+               int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
+    const int rows = GV_THREADS / GV_LANES;
+    const int64_t blocks = std::min<int64_t>((n + rows - 1) / rows, 8LL * num_sms());
+    const size_t smem = static_cast<size_t>(NQ) * ((d + 15) / 16 * 16);
+    sq8_few_kernel<T, NQ><<<(unsigned)blocks, GV_THREADS, smem, s>>>(qc, qs, (int)nq, ldq, xc, xs, n, ldx, d,
+                                                                     static_cast<T*>(out), ldo);
+    RDB_LAUNCH_CHECK();
+    return RDB_OK;
+}
+
+// ----------------------------------------------------------- tensor cores --
+
+struct DotArgs {
+    const float *qs, *xs;
+    int64_t nq, n, ldo;
+    int nqt, nxt;  // tiles of 256 queries, of 256 rows
+    int nk;
+    void* out;
+};
+
 template <typename T>
-__global__ void sq8_dot_kernel(const int8_t* __restrict__ qc, const float* __restrict__ qs, int64_t nq, int64_t ldq,
-                               const int8_t* __restrict__ xc, const float* __restrict__ xs, int64_t n, int64_t ldx,
-                               int d, T* __restrict__ out, int64_t ldo) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t b = w / n, r = w % n;
-    if (b >= nq) return;
-    const int8_t *q = qc + b * ldq, *x = xc + r * ldx;
-    int acc = 0;
-    const int d4 = d & ~3;
-    for (int t = 4 * lane; t < d4; t += 128)
-        acc = __dp4a(*reinterpret_cast<const int*>(q + t), *reinterpret_cast<const int*>(x + t), acc);
-    if (lane < (d & 3)) acc += static_cast<int>(q[d4 + lane]) * static_cast<int>(x[d4 + lane]);
-    acc = __reduce_add_sync(0xffffffffu, acc);
-    if (lane == 0) out[b * ldo + r] = from_f<T>(__fmul_rn(__fmul_rn(qs[b], xs[r]), static_cast<float>(acc)));
+struct DotPolicy {
+    static constexpr bool kInt8 = true;
+    // rows are walked in groups of 8 tiles: the tiles in flight form a block of
+    // both operands that L2 holds
+    static constexpr int kGroup = 8;
+    const CUtensorMap *mx, *mq;
+    const DotArgs& a;
+
+    using Job = TileJob;
+    struct Iter {
+        const DotPolicy& p;
+        int64_t i;
+        int step;
+        __device__ Iter(const DotPolicy& pol, int pair, int npairs) : p(pol), i(pair), step(npairs) {}
+        __device__ __forceinline__ bool next(Job& j) {
+            const DotArgs& a = p.a;
+            if (i >= static_cast<int64_t>(a.nqt) * a.nxt) return false;
+            const int64_t per = static_cast<int64_t>(kGroup) * a.nqt;
+            const int g = static_cast<int>(i / per), in = static_cast<int>(i % per);
+            const int gs = min(kGroup, a.nxt - g * kGroup);
+            j.ma = p.mx;
+            j.mb = p.mq;
+            j.m0 = (g * kGroup + in % gs) * TT_M;
+            j.n0 = in / gs * TT_N;
+            j.nn = static_cast<int>(min(static_cast<int64_t>(TT_N), (a.nq - j.n0 + 31) / 32 * 32));
+            j.k0 = 0;
+            j.nk = a.nk;
+            j.nseg = 1;
+            j.a_mn = j.b_mn = false;
+            i += step;
+            return true;
+        }
+    };
+    struct Epi {
+        float xs;
+    };
+
+    __device__ __forceinline__ void begin(Epi& e, const Job& j, int row, int) const {
+        const int64_t r = static_cast<int64_t>(j.m0) + row;
+        e.xs = r < a.n ? a.xs[r] : 0.f;
+    }
+
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
+        const int64_t x = static_cast<int64_t>(j.m0) + row, b0 = j.n0 + col;
+        if (x >= a.n) return;
+        T* o = static_cast<T*>(a.out) + b0 * a.ldo + x;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (b0 + i < a.nq) o[i * a.ldo] = from_f<T>(score(__ldg(a.qs + b0 + i), e.xs, static_cast<int>(r[i])));
+    }
+
+    __device__ __forceinline__ void end(Epi&, const Job&, int, int) const {}
+};
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
+    sq8_tile_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mq,
+                    const __grid_constant__ DotArgs a, const TileStatus st) {
+    extern __shared__ uint8_t smem_raw[];
+    const DotPolicy<T> p{&mx, &mq, a};
+    tile_loop(smem_raw, p, false, st);
+}
+
+template <typename T>
+int launch_tile(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
+                int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
+    static bool attr[64] = {false};
+    RDB_TRY(tile_smem_attr(sq8_tile_kernel<T>, attr));
+    CUtensorMap mx, mq;
+    RDB_TRY(make_map_3d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, d, n, 1, ldx, 0, 128));
+    RDB_TRY(make_map_3d(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, d, nq, 1, ldq, 0, 128));
+    DotArgs a{qs, xs, nq, n, ldo, (int)((nq + TT_N - 1) / TT_N), (int)((n + TT_M - 1) / TT_M), (d + 127) / 128, out};
+    const int64_t tiles = (int64_t)a.nqt * a.nxt;
+    sq8_tile_kernel<T><<<2 * (unsigned)std::min<int64_t>(tile_pairs(), tiles), TT_THREADS, TT_SMEM, s>>>(
+        mx, mq, a, tile_status());
+    RDB_LAUNCH_CHECK();
+    return RDB_OK;
 }
 
 template <typename T>
 int launch_dot(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
                int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
-    const int64_t blocks = (nq * n + 7) / 8;
-    RDB_CHECK_ARG(blocks < (1LL << 31), "too many scores for one launch");
-    sq8_dot_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(qc, qs, nq, ldq, xc, xs, n, ldx, d, static_cast<T*>(out), ldo);
-    RDB_LAUNCH_CHECK();
-    return RDB_OK;
+    const int64_t dp = (d + 15) / 16 * 16;
+    if (nq <= 1 && dp <= GV_SMEM) return launch_few<T, 1>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
+    if (nq <= 2 && 2 * dp <= GV_SMEM) return launch_few<T, 2>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
+    if (nq <= 4 && 4 * dp <= GV_SMEM) return launch_few<T, 4>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
+    if (nq <= 8 && 8 * dp <= GV_SMEM) return launch_few<T, 8>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
+    return launch_tile<T>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
 }
 
 }  // namespace

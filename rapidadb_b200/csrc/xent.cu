@@ -1,20 +1,33 @@
 // Softmax cross entropy of queries against every stored row, with gradients.
 //
-//   s_bn   = scale <q_b, x_n>                  (never written to memory)
+//   s_bn   = scale <q_b, x_n>                  (the [nq, n] matrix is never kept)
 //   loss_b = log sum_n exp(s_bn) - s_b,t(b)    (0 where t(b) == ignore_index)
 //   G_bn   = g_b scale (exp(s_bn) / sum_n exp(s_bn) - [n = t(b)])
 //   dq = G x,  dx = G^T q
 //
-// The sum is taken in base 2 around a running maximum: with c = scale log2 e,
+// Every product runs on the tcgen05 tile loop of tile_tc.cuh.
+//
+// Forward: one pass over the rows.  The sum is taken in base 2 around a running
+// maximum in the epilogue of each 256 x 256 tile, c = scale log2 e,
 //   m = max_n c <q, x_n>,   z = sum_n 2^(c <q, x_n> - m),
-// held in fp32; log sum exp = ln 2 (m + log2 z).  The target's own term stays out
-// of the running sum: with r = the sum of the other terms relative to the
-// target's, loss = log1p(r), so a query that finds its row keeps a loss near 0,
-// and its p - 1 = expm1(-loss), to full precision.
+// held in fp32, one (m, z) per query, row split and epilogue half, joined by
+// xent_join_kernel.  The target's own term stays out of the running sum: with
+// r = the sum of the other terms relative to the target's, loss = log1p(r), so
+// a query that finds its row keeps a loss near 0, and its p - 1 = expm1(-loss),
+// to full precision.
+//
+// Backward: the rows in pieces of C.  Per piece one launch recomputes the
+// logits and writes G / (g_b scale) = p - [n = t] as a [nq, C] workspace in the
+// operands' type (about 64 MB, so that it stays in L2), one launch multiplies
+// it both ways: dx rows directly (K = nq), dq into fp32 partial sums (K = C,
+// split over several tiles when there are few queries), joined at the end.
+// No atomics: every sum has a fixed order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "common.cuh"
+#include <algorithm>
+
+#include "tile_tc.cuh"
 
 namespace rdb {
 namespace {
@@ -22,6 +35,12 @@ namespace {
 constexpr int NT = 256, NW = NT / 32;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr double kLog2e = 1.4426950408889634;
+// G is held as 2^14 (p - [n = t]): the largest value is 2^14, and an fp16
+// probability keeps its 11 bits down to 2^-28 (2^-14 without the factor).  A
+// power of two: exact for every type.
+constexpr float kGScale = 16384.f, kGLog2 = 14.f;
+
+inline int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -40,147 +59,563 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// two floats in the 16-bit type, a in the low half
 template <typename T>
-__device__ __forceinline__ float warp_dot(const T* a, const T* b, int d, int lane) {
+__device__ __forceinline__ uint32_t pack16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// v = hi + mid + lo, each bf16: what the first two leave is exact in fp32
+__device__ __forceinline__ void split3(float v, float (&o)[3]) {
+    o[0] = __bfloat162float(__float2bfloat16_rn(v));
+    const float r = v - o[0];
+    o[1] = __bfloat162float(__float2bfloat16_rn(r));
+    o[2] = r - o[1];
+}
+
+// ---------------------------------------------------------------- forward --
+
+struct FwdArgs {
+    int64_t nq, n;       // queries, rows of this piece
+    int64_t row0;        // first row of the piece in the base
+    int nqb, ntiles, nsplit, slot0;
+    int nkb, nseg;
+    float c;
+    const int64_t* targets;
+    float2* part;        // [2 * slots][nq] (max <q, x>, z) of each split and half
+    float* tdot;         // [nq] <q, x_t>
+};
+
+struct FwdPolicy {
+    static constexpr bool kInt8 = false;
+    const CUtensorMap *mq, *mx;
+    const FwdArgs& a;
+
+    struct Job : TileJob {
+        int split;
+        bool first, last;
+    };
+    struct Iter {
+        const FwdPolicy& p;
+        int unit, step, t, hi, lo;
+        __device__ Iter(const FwdPolicy& pol, int pair, int npairs) : p(pol), unit(pair - npairs), step(npairs), t(0), hi(0), lo(0) {}
+        __device__ __forceinline__ bool next(Job& j) {
+            if (t == hi) {
+                unit += step;
+                if (unit >= p.a.nqb * p.a.nsplit) return false;
+                const int64_t sp = unit / p.a.nqb;
+                lo = t = static_cast<int>(sp * p.a.ntiles / p.a.nsplit);
+                hi = static_cast<int>((sp + 1) * p.a.ntiles / p.a.nsplit);
+            }
+            j.ma = p.mq;
+            j.mb = p.mx;
+            j.m0 = unit % p.a.nqb * TT_M;
+            j.n0 = t * TT_N;
+            j.nn = TT_N;
+            j.k0 = 0;
+            j.nk = p.a.nkb;
+            j.nseg = p.a.nseg;
+            j.a_mn = j.b_mn = false;
+            j.split = unit / p.a.nqb;
+            j.first = t == lo;
+            j.last = t == hi - 1;
+            ++t;
+            return true;
+        }
+    };
+    struct Epi {
+        float m, mb, z;  // running maximum of <q, x>, c times it, sum
+        int64_t tgt;     // target as a row of the piece (any value: not there)
+    };
+
+    __device__ __forceinline__ void begin(Epi& e, const Job& j, int row, int) const {
+        if (!j.first) return;
+        e.m = -INFINITY;
+        e.mb = e.z = 0.f;
+        const int64_t b = j.m0 + row;
+        e.tgt = b < a.nq ? a.targets[b] - a.row0 : -1;
+    }
+
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        const int64_t c0 = static_cast<int64_t>(j.n0) + col;
+        if (c0 + 32 > a.n) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (c0 + i >= a.n) v[i] = -INFINITY;
+        }
+        const int64_t rel = e.tgt - c0;
+        if (rel >= 0 && rel < 32 && e.tgt < a.n) {
+            // the target's own term is kept apart
+            a.tdot[j.m0 + row] = pick32(v, static_cast<int>(rel));
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                v[i] = i == static_cast<int>(rel) ? -INFINITY : v[i];
+        }
+        float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
+#pragma unroll
+        for (int i = 4; i < 32; i += 4) {
+            m0 = fmaxf(m0, fmaxf(v[i], v[i + 1]));
+            m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
+        }
+        m0 = fmaxf(m0, m1);
+        if (m0 > e.m) {
+            e.z *= ex2((e.m - m0) * a.c);  // 0 before the first finite value
+            e.m = m0;
+            e.mb = m0 * a.c;
+        }
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            s0 += ex2(fmaf(v[i], a.c, -e.mb));
+            s1 += ex2(fmaf(v[i + 1], a.c, -e.mb));
+            s2 += ex2(fmaf(v[i + 2], a.c, -e.mb));
+            s3 += ex2(fmaf(v[i + 3], a.c, -e.mb));
+        }
+        e.z += (s0 + s1) + (s2 + s3);
+    }
+
+    __device__ __forceinline__ void end(Epi& e, const Job& j, int row, int half) const {
+        const int64_t b = j.m0 + row;
+        if (j.last && b < a.nq)
+            a.part[(2 * static_cast<int64_t>(a.slot0 + j.split) + half) * a.nq + b] = make_float2(e.m, e.z);
+    }
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
+    xent_scan_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mx,
+                     const __grid_constant__ FwdArgs a, const bool bf16, const TileStatus st) {
+    extern __shared__ uint8_t smem_raw[];
+    const FwdPolicy p{&mq, &mx, a};
+    tile_loop(smem_raw, p, bf16, st);
+}
+
+// Joins the parts of 32 queries per block; stats and loss of each query.  An
+// ignored query has loss 0; one whose target is no row is NaN throughout.
+__global__ void __launch_bounds__(NT)
+    xent_join_kernel(const float2* part, int slots, const float* tdot, const int64_t* targets, int64_t ignore,
+                     int64_t n, float c, int64_t nq, float* stats, float* loss) {
+    __shared__ float2 sh[NW][32];
+    const int qi = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * 32 + qi;
+    float M = -INFINITY, Z = 0.f;
+    auto add = [&](float m, float z) {
+        const float nm = fmaxf(M, m);
+        Z = Z * (M > -INFINITY ? ex2((M - nm) * c) : (Z == Z ? 0.f : Z)) +
+            z * (m > -INFINITY ? ex2((m - nm) * c) : (z == z ? 0.f : z));
+        M = nm;
+    };
+    if (b < nq)
+        for (int s = g; s < slots; s += NW) {
+            const float2 v = part[static_cast<int64_t>(s) * nq + b];
+            add(v.x, v.y);
+        }
+    sh[g][qi] = make_float2(M, Z);
+    __syncthreads();
+    if (g != 0 || b >= nq) return;
+    for (int k = 1; k < NW; ++k) add(sh[k][qi].x, sh[k][qi].y);
+    const int64_t t = targets[b];
+    const bool ignored = t == ignore, has = t >= 0 && t < n;
+    const float nan = __int_as_float(0x7fc00000);
+    // Z sums 2^(c v - c M); u: the target's exponent relative to that
+    const float Mc = M > -INFINITY ? M * c : 0.f;
+    const float td = has ? tdot[b] : -INFINITY;
+    const float u = fmaf(td, c, -Mc);
+    float m = Mc, lz, l;
+    if (u >= 0.f || (has && !(M > -INFINITY))) {
+        // the target is the largest (or the only) term
+        m = td * c;
+        const float rest = M > -INFINITY ? Z * ex2(-u) : 0.f * Z;
+        l = isfinite(td) ? log1pf(rest) : nan;
+        lz = log2f(rest + ex2(fmaf(td, c, -m)));
+    } else {
+        lz = log2f(Z + (has ? ex2(u) : 0.f));
+        l = kLn2 * (lz - u);
+    }
+    if (ignored) l = 0.f;
+    else if (!has) l = lz = nan;
+    stats[b] = m;
+    stats[nq + b] = lz;
+    stats[2 * nq + b] = l;
+    if (loss) loss[b] = l;
+}
+
+// mean or sum of the losses of the queries that are not ignored
+__global__ void __launch_bounds__(1024)
+    xent_reduce_kernel(const float* loss_q, const int64_t* targets, int64_t ignore, int64_t nq, int mean, float* loss) {
+    __shared__ float ss[32];
+    __shared__ int sc[32];
     float s = 0.f;
-    for (int t = lane; t < d; t += 32) s = fmaf(to_f(a[t]), to_f(b[t]), s);
+    int cnt = 0;
+    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x)
+        if (targets[i] != ignore) s += loss_q[i], ++cnt;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-}
-
-// 2^(a - m) with an empty or all -inf running maximum standing for "no terms"
-__device__ __forceinline__ float exp2_from(float a, float m) { return exp2f(a - (m == -INFINITY ? 0.f : m)); }
-
-// (M, Z): running maximum and sum over the rows but the target, tv the target's
-// value -> st = (largest value m, log2 sum 2^(s - m), loss) of the query.  An
-// ignored query has loss 0; one whose target is not a row is NaN throughout.
-__device__ __forceinline__ void finish_row(float M, float Z, float tv, bool has, bool ignored, float (&st)[3]) {
-    const float m = fmaxf(M, tv), mr = m == -INFINITY ? 0.f : m;
-    const float rest = Z * exp2_from(M, m);
-    st[0] = m;
-    st[1] = log2f(rest + exp2f(tv - mr));
-    if (ignored) {
-        st[2] = 0.f;
-    } else if (!has) {
-        st[1] = st[2] = __int_as_float(0x7fc00000);
-    } else {
-        st[2] = tv >= M ? log1pf(rest) : kLn2 * (st[1] + (m - tv));
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(NT) xent_forward_kernel(const T* q, int64_t ldq, const T* x, int64_t n, int64_t ldx,
-                                                          int d, const int64_t* targets, float c, int64_t ignore,
-                                                          float* loss, float* stats, int64_t nq) {
-    __shared__ float sm[NW], sz[NW];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t b = blockIdx.x;
-    const int64_t t = targets[b];
-    float m = -INFINITY, z = 0.f;
-    for (int64_t r = warp; r < n; r += NW) {
-        if (r == t) continue;
-        const float a = c * warp_dot(q + b * ldq, x + r * ldx, d, lane);
-        const float mn = fmaxf(m, a);
-        z = z * exp2_from(m, mn) + exp2_from(a, mn);
-        m = mn;
-    }
-    if (lane == 0) sm[warp] = m, sz[warp] = z;
-    __syncthreads();
-    if (warp == 0) {
-        float M = -INFINITY, Z = 0.f;
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w]);
-        for (int w = 0; w < NW; ++w) Z += sz[w] * exp2_from(sm[w], M);
-        const bool has = t >= 0 && t < n;
-        const float tv = has ? c * warp_dot(q + b * ldq, x + t * ldx, d, lane) : -INFINITY;
-        float st[3];
-        finish_row(M, Z, tv, has, t == ignore, st);
-        if (lane == 0) loss[b] = st[2], stats[b] = st[0], stats[nq + b] = st[1], stats[2 * nq + b] = st[2];
-    }
-}
-
-// sum and count of the valid rows -> the reduced loss
-__global__ void xent_reduce_kernel(const float* loss_q, const int64_t* targets, int64_t ignore, int64_t nq, int mean,
-                                   float* loss) {
-    __shared__ float ss[NW];
-    __shared__ long long sc[NW];
-    float s = 0.f;
-    long long cnt = 0;
-    for (int64_t i = threadIdx.x; i < nq; i += NT) {
-        const bool ok = targets[i] != ignore;
-        s += ok ? loss_q[i] : 0.f;
-        cnt += ok;
-    }
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
     if ((threadIdx.x & 31) == 0) ss[threadIdx.x >> 5] = s, sc[threadIdx.x >> 5] = cnt;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < NW; ++w) ss[0] += ss[w], sc[0] += sc[w];
+        for (int w = 1; w < 32; ++w) ss[0] += ss[w], sc[0] += sc[w];
         *loss = mean ? ss[0] / static_cast<float>(sc[0]) : ss[0];
     }
 }
 
-// g_b of every query: the incoming gradient (divided by the valid queries for
-// the mean), 0 for an ignored one
-__global__ void __launch_bounds__(NT) xent_weights_kernel(const float* grad, const int64_t* targets, int64_t ignore,
-                                                          int64_t nq, int reduction, float* w) {
-    __shared__ long long sc[NW];
-    long long cnt = 0;
+// --------------------------------------------------------------- backward --
+
+// w_b = the incoming gradient of the query's loss (divided by the queries that
+// count for the mean), 0 for an ignored one; wmax = max |w_b|
+__global__ void __launch_bounds__(1024)
+    xent_weights_kernel(const float* grad, const int64_t* targets, int64_t ignore, int64_t nq, int reduction, float* w,
+                        float* wmax) {
+    __shared__ int sc[32];
+    __shared__ float sm[32];
+    int cnt = 0;
     if (reduction == RDB_REDUCE_MEAN) {
-        for (int64_t i = threadIdx.x; i < nq; i += NT) cnt += targets[i] != ignore;
-        for (int o = 16; o > 0; o >>= 1) cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+        for (int64_t i = threadIdx.x; i < nq; i += blockDim.x) cnt += targets[i] != ignore;
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
         if ((threadIdx.x & 31) == 0) sc[threadIdx.x >> 5] = cnt;
         __syncthreads();
-        cnt = 0;
-        for (int k = 0; k < NW; ++k) cnt += sc[k];
+        cnt = __reduce_add_sync(0xffffffffu, sc[threadIdx.x & 31]);
     }
-    for (int64_t i = threadIdx.x; i < nq; i += NT) {
-        float g = grad[reduction == RDB_REDUCE_NONE ? i : 0];
-        if (reduction == RDB_REDUCE_MEAN) g /= static_cast<float>(cnt);
-        w[i] = targets[i] == ignore ? 0.f : g;
+    float mx = 0.f;
+    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x) {
+        float g = 0.f;
+        if (targets[i] != ignore) {
+            g = grad[reduction == RDB_REDUCE_NONE ? i : 0];
+            if (reduction == RDB_REDUCE_MEAN) g /= static_cast<float>(cnt);
+        }
+        w[i] = g;
+        mx = fmaxf(mx, fabsf(g));  // a NaN weight makes its own products NaN
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mx;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 32; ++k) mx = fmaxf(mx, sm[k]);
+        *wmax = mx;
     }
 }
+
+// Queries weighted for dx = G^T (w q): out[b] = q[b] w_b / wmax, so that the
+// type's range is used whatever the size of the gradients (equal weights: the
+// query itself, unrounded); zero rows for ignored queries, whatever they hold.
+// fp32: three bf16 planes.
+template <typename T>
+__global__ void __launch_bounds__(NT)
+    xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const int64_t* targets, int64_t ignore,
+                         const float* w, const float* wmax, void* out, int64_t ldo) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 5);
+    if (b >= nq) return;
+    const bool skip = targets[b] == ignore;
+    const float f = skip || w[b] == 0.f ? 0.f : w[b] / *wmax;
+    for (int t = threadIdx.x & 31; t < d; t += 32) {
+        const float v = skip ? 0.f : to_f(q[b * ldq + t]) * f;
+        if constexpr (sizeof(T) == 4) {
+            float o[3];
+            split3(v, o);
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                static_cast<__nv_bfloat16*>(out)[(k * nq + b) * ldo + t] = __float2bfloat16_rn(o[k]);
+        } else {
+            static_cast<T*>(out)[b * ldo + t] = from_f<T>(v);
+        }
+    }
+}
+
+// fp32 rows -> three bf16 planes [3][n][ldo]
+__global__ void __launch_bounds__(NT)
+    xent_split_kernel(const float* x, int64_t n, int64_t ldx, int d, __nv_bfloat16* out, int64_t ldo) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 5);
+    if (r >= n) return;
+    for (int t = threadIdx.x & 31; t < d; t += 32) {
+        float o[3];
+        split3(x[r * ldx + t], o);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) out[(k * n + r) * ldo + t] = __float2bfloat16_rn(o[k]);
+    }
+}
+
+struct ProbArgs {
+    int64_t nq, n, row0;  // queries, rows of the piece, its first row
+    int nqb, njobs, nkb, nseg;
+    float c;
+    const int64_t* targets;
+    int64_t ignore;
+    const float* stats;
+    void* g;              // [planes][nq][ldg]
+    int64_t ldg;
+};
+
+// G tiles of one piece: 2^14 (p - [n = t])
+template <typename T>
+struct ProbPolicy {
+    static constexpr bool kInt8 = false;
+    const CUtensorMap *mq, *mx;
+    const ProbArgs& a;
+
+    using Job = TileJob;
+    struct Iter {
+        const ProbPolicy& p;
+        int i, step;
+        __device__ Iter(const ProbPolicy& pol, int pair, int npairs) : p(pol), i(pair), step(npairs) {}
+        __device__ __forceinline__ bool next(Job& j) {
+            if (i >= p.a.njobs) return false;
+            j.ma = p.mq;
+            j.mb = p.mx;
+            j.m0 = i % p.a.nqb * TT_M;
+            j.n0 = i / p.a.nqb * TT_N;
+            j.nn = TT_N;
+            j.k0 = 0;
+            j.nk = p.a.nkb;
+            j.nseg = p.a.nseg;
+            j.a_mn = j.b_mn = false;
+            i += step;
+            return true;
+        }
+    };
+    struct Epi {
+        float m, lz, hit;
+        int64_t tgt;
+        bool in, ignored;
+    };
+
+    __device__ __forceinline__ void begin(Epi& e, const Job& j, int row, int) const {
+        const int64_t b = j.m0 + row;
+        e.in = b < a.nq;
+        if (!e.in) return;
+        const int64_t t = a.targets[b];
+        e.ignored = t == a.ignore;
+        e.tgt = t - a.row0;
+        e.m = a.stats[b];
+        e.lz = a.stats[a.nq + b] - kGLog2;
+        e.hit = a.stats[2 * a.nq + b];
+    }
+
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
+        if (!e.in) return;
+        float v[32];
+        // two roundings, of the exponent relative to the largest logit and of
+        // the one relative to their sum: both small for the terms that count
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            v[i] = e.ignored ? 0.f : ex2(fmaf(__uint_as_float(r[i]), a.c, -e.m) - e.lz);
+        const int64_t c0 = static_cast<int64_t>(j.n0) + col;
+        const int64_t rel = e.tgt - c0;
+        if (rel >= 0 && rel < 32 && !e.ignored) {
+            const float h = kGScale * expm1f(-e.hit);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                v[i] = i == static_cast<int>(rel) ? h : v[i];
+        }
+        // columns behind the piece's last row are never read
+        if constexpr (sizeof(T) == 2) {
+            uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.g) + (j.m0 + row) * a.ldg + c0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[i] = make_uint4(pack16<T>(v[8 * i], v[8 * i + 1]), pack16<T>(v[8 * i + 2], v[8 * i + 3]),
+                                  pack16<T>(v[8 * i + 4], v[8 * i + 5]), pack16<T>(v[8 * i + 6], v[8 * i + 7]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.g) +
+                                                    (k * a.nq + j.m0 + row) * a.ldg + c0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        w[h] = pack16<__nv_bfloat16>(v[8 * i + 2 * h], v[8 * i + 2 * h + 1]);
+                        // what is left for the next plane
+                        v[8 * i + 2 * h] -= __uint_as_float(w[h] << 16);
+                        v[8 * i + 2 * h + 1] -= __uint_as_float(w[h] & 0xffff0000u);
+                    }
+                    o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void end(Epi&, const Job&, int, int) const {}
+};
 
 template <typename T>
-__device__ __forceinline__ float grad_logit(const T* q, const T* x, int d, float c, float m, float lz, float loss,
-                                            bool hit, int lane) {
-    const float a = c * warp_dot(q, x, d, lane);
-    return hit ? expm1f(-loss) : exp2f(a - m - lz);
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
+    xent_prob_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mx,
+                     const __grid_constant__ ProbArgs a, const bool bf16, const TileStatus st) {
+    extern __shared__ uint8_t smem_raw[];
+    const ProbPolicy<T> p{&mq, &mx, a};
+    tile_loop(smem_raw, p, bf16, st);
 }
 
-// one block per query (DX = false: dq) or per row (DX = true: dx); acc is the
-// block's [d] fp32 row of the workspace
-template <typename T, bool DX>
-__global__ void __launch_bounds__(NT)
-    xent_backward_kernel(const T* q, int64_t nq, int64_t ldq, const T* x, int64_t n, int64_t ldx, int d,
-                         const int64_t* targets, float scale, float c, int64_t ignore, const float* weight,
-                         const float* stats, T* out, int64_t ldo, float* acc_ws) {
-    __shared__ float w[NW];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t count = DX ? nq : n;
-    float* acc = acc_ws + (int64_t)blockIdx.x * d;
-    for (int64_t self = blockIdx.x; self < (DX ? n : nq); self += gridDim.x) {
-        for (int t = threadIdx.x; t < d; t += NT) acc[t] = 0.f;
-        for (int64_t o0 = 0; o0 < count; o0 += NW) {
-            const int64_t o = o0 + warp;
-            const int64_t b = DX ? o : self, r = DX ? self : o;
-            float v = 0.f;
-            if (o < count && targets[b] != ignore)
-                v = scale * weight[b] *
-                    grad_logit(q + b * ldq, x + r * ldx, d, c, stats[b], stats[nq + b], stats[2 * nq + b],
-                                targets[b] == r, lane);
-            if (lane == 0) w[warp] = v;
-            __syncthreads();
-            for (int k = 0; k < NW && o0 + k < count; ++k) {
-                if (targets[DX ? o0 + k : self] == ignore) continue;  // whatever an ignored query holds
-                const T* row = DX ? q + (o0 + k) * ldq : x + (o0 + k) * ldx;
-                for (int t = threadIdx.x; t < d; t += NT) acc[t] = fmaf(w[k], to_f(row[t]), acc[t]);
+struct GradArgs {
+    int64_t nq, n;         // queries, rows of the piece
+    int d, nseg;
+    int nt;                // column tiles of d
+    int q_blocks, q_split, q_per;  // dq: 256-query blocks, K splits, K blocks per split (0 blocks: not wanted)
+    int kc, kq;            // K blocks of the piece and of the queries
+    int x_blocks;          // dx: 256-row blocks (0: not wanted)
+    bool q_first;          // the longer tiles come first
+    bool add;              // a piece before this one wrote the partial sums
+    float* part;           // [q_split][nq][dp]
+    int dp;
+    void* dx;              // rows of the piece
+    int64_t lddx;
+    bool dx_vec;           // 16-byte stores allowed
+    float scale;
+    const float* wmax;
+};
+
+template <typename T>
+struct GradPolicy {
+    static constexpr bool kInt8 = false;
+    const CUtensorMap *gk, *gmn, *xmn, *qmn;
+    const GradArgs& a;
+
+    struct Job : TileJob {
+        bool is_dx;
+        int split;
+    };
+    struct Iter {
+        const GradPolicy& p;
+        int i, step;
+        __device__ Iter(const GradPolicy& pol, int pair, int npairs) : p(pol), i(pair), step(npairs) {}
+        __device__ __forceinline__ bool next(Job& j) {
+            const GradArgs& a = p.a;
+            const int nqj = a.q_blocks * a.nt * a.q_split, nxj = a.x_blocks * a.nt;
+            if (i >= nqj + nxj) return false;
+            const int head = a.q_first ? nqj : nxj;
+            j.is_dx = (i < head) != a.q_first;
+            int k = i < head ? i : i - head;
+            i += step;
+            j.nseg = a.nseg;
+            j.b_mn = true;
+            j.n0 = k % a.nt * TT_N;
+            k /= a.nt;
+            j.nn = min(TT_N, (a.d - j.n0 + 127) / 128 * 128);
+            if (j.is_dx) {
+                j.ma = p.gmn;
+                j.mb = p.qmn;
+                j.a_mn = true;
+                j.m0 = k * TT_M;
+                j.k0 = 0;
+                j.nk = a.kq;
+                j.split = 0;
+            } else {
+                j.ma = p.gk;
+                j.mb = p.xmn;
+                j.a_mn = false;
+                j.split = k / a.q_blocks;
+                j.m0 = k % a.q_blocks * TT_M;
+                j.k0 = j.split * a.q_per;
+                j.nk = min(a.q_per, a.kc - j.k0);
             }
-            __syncthreads();
+            return true;
         }
-        for (int t = threadIdx.x; t < d; t += NT) out[self * ldo + t] = from_f<T>(acc[t]);
+    };
+    struct Epi {
+        float f;
+    };
+
+    __device__ __forceinline__ void begin(Epi& e, const Job&, int, int) const {
+        e.f = a.scale * (1.f / kGScale) * *a.wmax;
+    }
+
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
+        const int64_t m = j.m0 + row;
+        const int t0 = j.n0 + col;
+        if (t0 >= a.d) return;
+        if (!j.is_dx) {
+            if (m >= a.nq) return;
+            // dp is a multiple of 32: the columns behind d hold zeros
+            float4* o = reinterpret_cast<float4*>(a.part + (j.split * a.nq + m) * a.dp + t0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float4 v = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                       __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+                if (a.add) {
+                    const float4 w = o[i];
+                    v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+                }
+                o[i] = v;
+            }
+            return;
+        }
+        if (m >= a.n) return;
+        T* o = static_cast<T*>(a.dx) + m * a.lddx + t0;
+        if (a.dx_vec && t0 + 32 <= a.d) {
+            uint4* o4 = reinterpret_cast<uint4*>(o);
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        w[h] = pack16<T>(__uint_as_float(r[8 * i + 2 * h]) * e.f,
+                                         __uint_as_float(r[8 * i + 2 * h + 1]) * e.f);
+                    o4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) w[h] = __float_as_uint(__uint_as_float(r[4 * i + h]) * e.f);
+                    o4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (t0 + i < a.d) o[i] = from_f<T>(__uint_as_float(r[i]) * e.f);
+        }
+    }
+
+    __device__ __forceinline__ void end(Epi&, const Job&, int, int) const {}
+};
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
+    xent_grad_kernel(const __grid_constant__ CUtensorMap gk, const __grid_constant__ CUtensorMap gmn,
+                     const __grid_constant__ CUtensorMap xmn, const __grid_constant__ CUtensorMap qmn,
+                     const __grid_constant__ GradArgs a, const bool bf16, const TileStatus st) {
+    extern __shared__ uint8_t smem_raw[];
+    const GradPolicy<T> p{&gk, &gmn, &xmn, &qmn, a};
+    tile_loop(smem_raw, p, bf16, st);
+}
+
+// dq_b = g_b scale 2^-14 (sum of the parts, in split order)
+template <typename T>
+__global__ void __launch_bounds__(NT)
+    xent_dq_kernel(const float* part, int splits, int64_t nq, int d, int dp, const int64_t* targets, int64_t ignore,
+                   const float* w, float scale, T* dq, int64_t lddq) {
+    const int64_t b = blockIdx.x;
+    const float f = w[b] * scale * (1.f / kGScale);
+    const bool skip = targets[b] == ignore;
+    for (int t = threadIdx.x; t < d; t += NT) {
+        float s = 0.f;
+        for (int k = 0; k < splits; ++k) s += part[(k * nq + b) * dp + t];
+        dq[b * lddq + t] = from_f<T>(skip ? 0.f : s * f);
     }
 }
+
+// -------------------------------------------------------------- host side --
 
 int check_common(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
                  const int64_t* targets, float scale, int reduction) {
@@ -188,7 +623,7 @@ int check_common(int dtype, const void* q, int64_t nq, int64_t ldq, const void* 
     RDB_CHECK_ARG(e != 0, "unknown dtype %d", dtype);
     RDB_CHECK_ARG(nq >= 0 && n >= 1 && d >= 1 && ldq >= d && ldx >= d, "bad shape");
     RDB_CHECK_ARG(nq < (1LL << 31) && n < (1LL << 31), "nq and n must be < 2^31");
-    RDB_CHECK_ARG(scale > 0.f && scale <= 3.0e38f, "scale must be positive and finite");
+    RDB_CHECK_ARG(scale > 0.f && scale <= 2.0e38f, "scale must be positive and finite");
     RDB_CHECK_ARG(reduction >= RDB_REDUCE_NONE && reduction <= RDB_REDUCE_SUM, "unknown reduction %d", reduction);
     RDB_CHECK_ARG(x && (nq == 0 || (q && targets)), "NULL pointer");
     RDB_CHECK_ARG((ldq * e) % 16 == 0 && (ldx * e) % 16 == 0, "row strides must be multiples of 16 bytes");
@@ -197,34 +632,282 @@ int check_common(int dtype, const void* q, int64_t nq, int64_t ldq, const void* 
     return RDB_OK;
 }
 
-template <typename T>
-int forward_t(const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
-              const int64_t* targets, float scale, int64_t ignore, float* loss_q, float* stats, cudaStream_t s) {
-    xent_forward_kernel<T><<<(unsigned)nq, NT, 0, s>>>(static_cast<const T*>(q), ldq, static_cast<const T*>(x), n, ldx,
-                                                       d, targets, (float)(scale * kLog2e), ignore, loss_q, stats, nq);
+CUtensorMapDataType map_type(int dtype) {
+    return dtype == RDB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// operand rows as 16-bit planes: the caller's rows, or the bf16 planes of fp32
+struct Planes {
+    const void* p;
+    int64_t ld, plane;  // elements
+    int count;
+};
+
+int operand_map(CUtensorMap* m, int dtype, const Planes& o, int64_t cols, int64_t rows, bool mn) {
+    return make_map_3d(m, map_type(dtype), 2, o.p, cols, rows, o.count, o.ld * 2,
+                       o.count > 1 ? o.plane * 2 : 0, mn ? 64 : 128);
+}
+
+struct Arena {
+    char* base;
+    size_t used = 0;
+    template <typename T>
+    T* take(size_t count) {
+        T* p = reinterpret_cast<T*>(base + used);
+        used += (count * sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+
+// rows of a piece: n split evenly into pieces of at most `most` (a multiple of 256)
+int64_t piece_rows(int64_t n, int64_t most) {
+    most = std::max<int64_t>(256, most / 256 * 256);
+    const int64_t pieces = (n + most - 1) / most;
+    return up((n + pieces - 1) / pieces, 256);
+}
+
+struct FwdPlan {
+    int64_t rows;  // rows per piece
+    int pieces, nqb, nkb, nseg, slots, nsplit[2];  // nsplit of a full and of the last piece
+};
+
+// Tiles of one piece per pair: as many splits as give every pair the same
+// number of tiles; a split costs about a seventh of a tile (its join and the
+// reload of the query's target).
+int fwd_splits(int nqb, int64_t ntiles, int pairs) {
+    int best = 1;
+    double best_cost = 1e30;
+    const int64_t most = std::min<int64_t>(ntiles, std::max<int64_t>(1, 16LL * pairs / nqb + 1));
+    for (int64_t s = 1; s <= most; ++s) {
+        const double per = (double)((ntiles + s - 1) / s);
+        const double cost = (double)((nqb * s + pairs - 1) / pairs) * (per + 0.15);
+        if (cost < best_cost) best_cost = cost, best = (int)s;
+    }
+    return best;
+}
+
+FwdPlan fwd_plan(int dtype, int64_t nq, int64_t n, int d) {
+    FwdPlan p;
+    const int64_t dp = up(d, 8);
+    // fp32: the planes of a piece stay in L2
+    p.rows = dtype == RDB_F32 ? piece_rows(n, (96LL << 20) / (6 * dp)) : up(n, 256);
+    p.pieces = (int)((n + p.rows - 1) / p.rows);
+    p.nqb = (int)std::max<int64_t>(1, (nq + TT_M - 1) / TT_M);
+    p.nkb = (d + 63) / 64;
+    p.nseg = dtype == RDB_F32 ? 6 : 1;
+    const int pairs = tile_pairs();
+    const int64_t last = n - (p.pieces - 1) * p.rows;
+    p.nsplit[0] = fwd_splits(p.nqb, p.rows / TT_N, pairs);
+    p.nsplit[1] = fwd_splits(p.nqb, (last + TT_N - 1) / TT_N, pairs);
+    p.slots = (p.pieces - 1) * p.nsplit[0] + p.nsplit[1];
+    return p;
+}
+
+struct FwdWs {
+    float *loss_q, *tdot;
+    float2* part;
+    __nv_bfloat16 *qp, *xp;
+    size_t bytes;
+};
+
+FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
+    FwdWs w{};
+    Arena a{static_cast<char*>(base)};
+    const int64_t dp = up(d, 8);
+    w.loss_q = a.take<float>(nq);
+    w.tdot = a.take<float>(nq);
+    w.part = a.take<float2>(2 * (size_t)p.slots * nq);
+    if (dtype == RDB_F32) {
+        w.qp = a.take<__nv_bfloat16>(3 * nq * dp);
+        w.xp = a.take<__nv_bfloat16>(3 * p.rows * dp);
+    }
+    w.bytes = a.used + 256;
+    return w;
+}
+
+struct BwdPlan {
+    int64_t rows;  // rows per piece
+    int pieces, planes, nqb, nt, nkb, nseg, kq, dp;
+    int q_split, q_per;
+    bool q_first;
+};
+
+BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool need_dx) {
+    BwdPlan p;
+    p.planes = dtype == RDB_F32 ? 3 : 1;
+    p.nseg = dtype == RDB_F32 ? 6 : 1;
+    const int64_t col = std::max<int64_t>(1, nq * 2 * p.planes);  // bytes of G per row
+    // G stays in L2 (64 MB) unless that made the pieces so narrow that the
+    // partial sums of dq (read and written once a piece) cost more than they save
+    int64_t most = (64LL << 20) / col;
+    if (most < 4096) most = std::max(most, std::min<int64_t>(4096, (2LL << 30) / col));
+    if (dtype == RDB_F32) most = std::min<int64_t>(most, (96LL << 20) / (6 * up(d, 8)));
+    p.rows = piece_rows(n, most);
+    p.pieces = (int)((n + p.rows - 1) / p.rows);
+    p.nqb = (int)std::max<int64_t>(1, (nq + TT_M - 1) / TT_M);
+    p.nt = (d + TT_N - 1) / TT_N;
+    p.nkb = (d + 63) / 64;
+    p.kq = (int)((nq + 63) / 64);
+    p.dp = (int)up(d, 32);
+    // K splits of dq: the split that ends first, tiles dealt out in turn; a
+    // tile costs about six K blocks on top of its own (fill, drain, store)
+    const int64_t pairs = tile_pairs(), kc = std::min(p.rows, up(n, 64)) / 64;
+    const int64_t nx = need_dx ? (p.rows + TT_M - 1) / TT_M * p.nt : 0, lx = (int64_t)p.kq * p.nseg + 6;
+    p.q_split = 1;
+    p.q_per = (int)kc;
+    if (need_dq) {
+        int64_t best = INT64_MAX;
+        for (int64_t s = 1; s <= std::min<int64_t>(kc, 64); ++s) {
+            if (s > 1 && s * nq * p.dp * 4 > (64LL << 20)) break;
+            const int64_t per = (kc + s - 1) / s, used = (kc + per - 1) / per;
+            const int64_t nj = (int64_t)p.nqb * p.nt * used, lq = per * p.nseg + 6;
+            const int64_t slack = (pairs - nj % pairs) % pairs;
+            const int64_t rest = std::max<int64_t>(0, nx - slack);
+            int64_t cost = (nj + pairs - 1) / pairs * std::max(lq, nx ? lx : lq) + (rest + pairs - 1) / pairs * lx;
+            if (nx) {
+                // either order: the longer tiles first
+                cost = std::min(cost, (nj + pairs - 1) / pairs * lq + (nx + pairs - 1) / pairs * lx);
+            }
+            cost += s / 4;  // parts to join
+            if (cost < best) best = cost, p.q_split = (int)used, p.q_per = (int)per;
+        }
+    }
+    p.q_first = (int64_t)p.q_per >= p.kq;
+    return p;
+}
+
+struct BwdWs {
+    float *w, *wmax, *part;
+    void *g, *qw;
+    __nv_bfloat16 *qp, *xp;
+    size_t bytes;
+};
+
+BwdWs bwd_ws(void* base, const BwdPlan& p, int dtype, int64_t nq, int d, bool need_dq, bool need_dx) {
+    BwdWs w{};
+    Arena a{static_cast<char*>(base)};
+    const int64_t d8 = up(d, 8);
+    w.w = a.take<float>(nq);
+    w.wmax = a.take<float>(1);
+    w.g = a.take<uint16_t>((size_t)p.planes * nq * p.rows);
+    if (need_dq) w.part = a.take<float>((size_t)p.q_split * nq * p.dp);
+    if (need_dx) w.qw = a.take<uint16_t>((size_t)p.planes * nq * d8);
+    if (dtype == RDB_F32) {
+        w.qp = a.take<__nv_bfloat16>(3 * nq * d8);
+        w.xp = a.take<__nv_bfloat16>(3 * p.rows * d8);
+    }
+    w.bytes = a.used + 256;
+    return w;
+}
+
+int split_rows(const void* x, int64_t n, int64_t ldx, int d, __nv_bfloat16* out, cudaStream_t s) {
+    xent_split_kernel<<<(unsigned)((n + NW - 1) / NW), NT, 0, s>>>(static_cast<const float*>(x), n, ldx, d, out,
+                                                                   up(d, 8));
     RDB_LAUNCH_CHECK();
     return RDB_OK;
 }
 
-constexpr int64_t kBlocks = 1024;
+// rows [r0, r0 + rows) as operand planes (fp32: split into xp first)
+int piece_operand(int dtype, const void* x, int64_t r0, int64_t rows, int64_t ldx, int d, __nv_bfloat16* xp, Planes* o,
+                  cudaStream_t s) {
+    const char* base = static_cast<const char*>(x) + r0 * ldx * (int64_t)elem_size(dtype);
+    if (dtype != RDB_F32) {
+        *o = {base, ldx, 0, 1};
+        return RDB_OK;
+    }
+    *o = {xp, up(d, 8), rows * up(d, 8), 3};
+    return split_rows(base, rows, ldx, d, xp, s);
+}
 
 template <typename T>
-int backward_t(const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
+int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
                const int64_t* targets, float scale, int64_t ignore, int reduction, const float* grad,
-               const float* stats, void* dq, int64_t lddq, void* dx, int64_t lddx, float* ws, cudaStream_t s) {
-    const T *tq = static_cast<const T*>(q), *tx = static_cast<const T*>(x);
-    const float c = (float)(scale * kLog2e);
-    float *weight = ws, *acc = ws + (nq + 63) / 64 * 64;
-    xent_weights_kernel<<<1, NT, 0, s>>>(grad, targets, ignore, nq, reduction, weight);
+               const float* stats, void* dq, int64_t lddq, void* dx, int64_t lddx, void* ws, cudaStream_t s) {
+    static bool attr_p[64] = {false}, attr_g[64] = {false};
+    const BwdPlan p = bwd_plan(dtype, nq, n, d, dq != nullptr, dx != nullptr);
+    const BwdWs w = bwd_ws(ws, p, dtype, nq, d, dq != nullptr, dx != nullptr);
+    const int64_t d8 = up(d, 8);
+    const TileStatus st = tile_status();
+    const bool bf16 = dtype != RDB_F16;
+    const int pairs = tile_pairs();
+    RDB_TRY(tile_smem_attr(xent_prob_kernel<T>, attr_p));
+    RDB_TRY(tile_smem_attr(xent_grad_kernel<T>, attr_g));
+
+    xent_weights_kernel<<<1, 1024, 0, s>>>(grad, targets, ignore, nq, reduction, w.w, w.wmax);
     RDB_LAUNCH_CHECK();
-    if (dq) {
-        xent_backward_kernel<T, false><<<(unsigned)(nq < kBlocks ? nq : kBlocks), NT, 0, s>>>(
-            tq, nq, ldq, tx, n, ldx, d, targets, scale, c, ignore, weight, stats, static_cast<T*>(dq), lddq, acc);
+    if (dx) {
+        xent_weighted_kernel<T><<<(unsigned)((nq + NW - 1) / NW), NT, 0, s>>>(static_cast<const T*>(q), nq, ldq, d,
+                                                                              targets, ignore, w.w, w.wmax, w.qw, d8);
         RDB_LAUNCH_CHECK();
     }
-    if (dx) {
-        xent_backward_kernel<T, true><<<(unsigned)(n < kBlocks ? n : kBlocks), NT, 0, s>>>(
-            tq, nq, ldq, tx, n, ldx, d, targets, scale, c, ignore, weight, stats, static_cast<T*>(dx), lddx, acc);
+    Planes qo;
+    RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
+    CUtensorMap mq, mqw;
+    RDB_TRY(operand_map(&mq, dtype, qo, d, nq, false));
+    mqw = mq;
+    if (dx) RDB_TRY(operand_map(&mqw, dtype, Planes{w.qw, d8, nq * d8, p.planes}, d, nq, true));
+
+    ProbArgs pa{};
+    pa.nq = nq;
+    pa.nqb = p.nqb;
+    pa.nkb = p.nkb;
+    pa.nseg = p.nseg;
+    pa.c = (float)(scale * kLog2e);
+    pa.targets = targets;
+    pa.ignore = ignore;
+    pa.stats = stats;
+    pa.g = w.g;
+    pa.ldg = p.rows;
+    GradArgs ga{};
+    ga.nq = nq;
+    ga.d = d;
+    ga.nseg = p.nseg;
+    ga.nt = p.nt;
+    ga.q_per = p.q_per;
+    ga.kq = p.kq;
+    ga.q_first = p.q_first;
+    ga.part = w.part;
+    ga.dp = p.dp;
+    ga.lddx = lddx;
+    ga.dx_vec = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (lddx * (int64_t)sizeof(T)) % 16 == 0;
+    ga.scale = scale;
+    ga.wmax = w.wmax;
+    const Planes go{w.g, p.rows, nq * p.rows, p.planes};
+
+    for (int i = 0; i < p.pieces; ++i) {
+        const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
+        Planes xo;
+        RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
+        CUtensorMap mx, mxmn, mgk, mgmn;
+        RDB_TRY(operand_map(&mx, dtype, xo, d, rows, false));
+        RDB_TRY(operand_map(&mxmn, dtype, xo, d, rows, true));
+        RDB_TRY(operand_map(&mgk, dtype, go, rows, nq, false));
+        RDB_TRY(operand_map(&mgmn, dtype, go, rows, nq, true));
+        pa.n = rows;
+        pa.row0 = r0;
+        const int64_t tiles = (rows + TT_N - 1) / TT_N * p.nqb;
+        RDB_CHECK_ARG(tiles < (1LL << 31), "too many tiles for one launch");
+        pa.njobs = (int)tiles;
+        xent_prob_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS, TT_SMEM, s>>>(mq, mx, pa, bf16,
+                                                                                                      st);
+        RDB_LAUNCH_CHECK();
+        ga.n = rows;
+        ga.kc = (int)((rows + 63) / 64);
+        ga.q_blocks = dq ? p.nqb : 0;
+        // a shorter last piece may leave splits without rows: their parts stay
+        ga.q_split = (ga.kc + p.q_per - 1) / p.q_per;
+        ga.x_blocks = dx ? (int)((rows + TT_M - 1) / TT_M) : 0;
+        ga.add = i > 0;
+        ga.dx = dx ? static_cast<T*>(dx) + r0 * lddx : nullptr;
+        const int64_t jobs = (int64_t)ga.nt * ((int64_t)ga.q_blocks * ga.q_split + ga.x_blocks);
+        RDB_CHECK_ARG(jobs < (1LL << 31), "too many tiles for one launch");
+        xent_grad_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM, s>>>(mgk, mgmn, mxmn,
+                                                                                                     mqw, ga, bf16, st);
+        RDB_LAUNCH_CHECK();
+    }
+    if (dq) {
+        xent_dq_kernel<T><<<(unsigned)nq, NT, 0, s>>>(w.part, p.q_split, nq, d, p.dp, targets, ignore, w.w, scale,
+                                                      static_cast<T*>(dq), lddq);
         RDB_LAUNCH_CHECK();
     }
     return RDB_OK;
@@ -238,8 +921,10 @@ using namespace rdb;
 extern "C" {
 
 size_t rdb_softmax_xent_workspace(int dtype, int64_t nq, int64_t n, int d, int reduction) {
-    (void)dtype, (void)n, (void)d, (void)reduction;
-    return 4 * (size_t)(nq > 0 ? nq : 0) + 256;
+    (void)reduction;
+    if (elem_size(dtype) == 0 || nq < 0 || n < 1 || d < 1) return 0;
+    const FwdPlan p = fwd_plan(dtype, nq, n, d);
+    return fwd_ws(nullptr, p, dtype, nq, d).bytes;
 }
 
 int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
@@ -247,28 +932,61 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
                      float* stats, void* ws, size_t ws_bytes, void* stream) {
     RDB_TRY(check_common(dtype, q, nq, ldq, x, n, ldx, d, targets, scale, reduction));
     RDB_CHECK_ARG((loss || (nq == 0 && reduction == RDB_REDUCE_NONE)) && (nq == 0 || stats), "NULL pointer");
-    if (!ws || ws_bytes < rdb_softmax_xent_workspace(dtype, nq, n, d, reduction))
-        return set_error(RDB_ERR_WORKSPACE, "workspace too small");
+    RDB_CHECK_ARG((reinterpret_cast<uintptr_t>(ws) & 15) == 0, "ws must be 16-byte aligned");
+    const FwdPlan p = fwd_plan(dtype, nq, n, d);
+    const FwdWs w = fwd_ws(ws, p, dtype, nq, d);
+    if (!ws || ws_bytes < w.bytes) return set_error(RDB_ERR_WORKSPACE, "workspace too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    float* loss_q = reduction == RDB_REDUCE_NONE ? loss : static_cast<float*>(ws);
+    float* loss_q = reduction == RDB_REDUCE_NONE ? loss : w.loss_q;
+    const float c = (float)(scale * kLog2e);
     if (nq > 0) {
-        if (dtype == RDB_F32)
-            RDB_TRY(forward_t<float>(q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, loss_q, stats, s));
-        else if (dtype == RDB_F16)
-            RDB_TRY(forward_t<__half>(q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, loss_q, stats, s));
-        else
-            RDB_TRY(forward_t<__nv_bfloat16>(q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, loss_q, stats, s));
+        static bool attr[64] = {false};
+        RDB_TRY(tile_smem_attr(xent_scan_kernel, attr));
+        const TileStatus st = tile_status();
+        Planes qo;
+        RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
+        CUtensorMap mq, mx;
+        RDB_TRY(operand_map(&mq, dtype, qo, d, nq, false));
+        FwdArgs a{};
+        a.nq = nq;
+        a.nqb = p.nqb;
+        a.nkb = p.nkb;
+        a.nseg = p.nseg;
+        a.c = c;
+        a.targets = targets;
+        a.part = w.part;
+        a.tdot = w.tdot;
+        for (int i = 0; i < p.pieces; ++i) {
+            const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
+            Planes xo;
+            RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
+            RDB_TRY(operand_map(&mx, dtype, xo, d, rows, false));
+            a.n = rows;
+            a.row0 = r0;
+            a.ntiles = (int)((rows + TT_N - 1) / TT_N);
+            a.nsplit = p.nsplit[i == p.pieces - 1];
+            a.slot0 = i * p.nsplit[0];
+            const int64_t units = (int64_t)a.nsplit * p.nqb;
+            RDB_CHECK_ARG(units < (1LL << 31), "too many tiles for one launch");
+            xent_scan_kernel<<<2 * (unsigned)std::min<int64_t>(tile_pairs(), units), TT_THREADS, TT_SMEM, s>>>(
+                mq, mx, a, dtype != RDB_F16, st);
+            RDB_LAUNCH_CHECK();
+        }
+        xent_join_kernel<<<(unsigned)((nq + 31) / 32), NT, 0, s>>>(w.part, 2 * p.slots, w.tdot, targets, ignore_index,
+                                                                   n, c, nq, stats, loss_q);
+        RDB_LAUNCH_CHECK();
     }
     if (reduction != RDB_REDUCE_NONE) {
-        xent_reduce_kernel<<<1, NT, 0, s>>>(loss_q, targets, ignore_index, nq, reduction == RDB_REDUCE_MEAN, loss);
+        xent_reduce_kernel<<<1, 1024, 0, s>>>(loss_q, targets, ignore_index, nq, reduction == RDB_REDUCE_MEAN, loss);
         RDB_LAUNCH_CHECK();
     }
     return RDB_OK;
 }
 
 size_t rdb_softmax_xent_backward_workspace(int dtype, int64_t nq, int64_t n, int d, int need_dq, int need_dx) {
-    (void)dtype, (void)n, (void)need_dq, (void)need_dx;
-    return 4 * ((size_t)(nq > 0 ? nq : 0) + (size_t)kBlocks * (size_t)(d > 0 ? d : 0)) + 512;
+    if (elem_size(dtype) == 0 || nq < 0 || n < 1 || d < 1) return 0;
+    const BwdPlan p = bwd_plan(dtype, nq, n, d, need_dq != 0, need_dx != 0);
+    return bwd_ws(nullptr, p, dtype, nq, d, need_dq != 0, need_dx != 0).bytes;
 }
 
 int rdb_softmax_xent_backward(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n,
@@ -278,6 +996,7 @@ int rdb_softmax_xent_backward(int dtype, const void* q, int64_t nq, int64_t ldq,
     RDB_TRY(check_common(dtype, q, nq, ldq, x, n, ldx, d, targets, scale, reduction));
     RDB_CHECK_ARG((!dq || lddq >= d) && (!dx || lddx >= d), "bad shape");
     RDB_CHECK_ARG(nq == 0 || (grad && stats), "NULL pointer");
+    RDB_CHECK_ARG((reinterpret_cast<uintptr_t>(ws) & 15) == 0, "ws must be 16-byte aligned");
     if (!ws || ws_bytes < rdb_softmax_xent_backward_workspace(dtype, nq, n, d, dq != nullptr, dx != nullptr))
         return set_error(RDB_ERR_WORKSPACE, "workspace too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -287,15 +1006,15 @@ int rdb_softmax_xent_backward(int dtype, const void* q, int64_t nq, int64_t ldq,
                                            (size_t)n, s));
         return RDB_OK;
     }
-    float* w = static_cast<float*>(ws);
+    if (!dq && !dx) return RDB_OK;
     if (dtype == RDB_F32)
-        return backward_t<float>(q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, reduction, grad, stats, dq,
-                                 lddq, dx, lddx, w, s);
+        return backward_t<float>(dtype, q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, reduction, grad, stats,
+                                 dq, lddq, dx, lddx, ws, s);
     if (dtype == RDB_F16)
-        return backward_t<__half>(q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, reduction, grad, stats, dq,
-                                  lddq, dx, lddx, w, s);
-    return backward_t<__nv_bfloat16>(q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, reduction, grad, stats,
-                                     dq, lddq, dx, lddx, w, s);
+        return backward_t<__half>(dtype, q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, reduction, grad,
+                                  stats, dq, lddq, dx, lddx, ws, s);
+    return backward_t<__nv_bfloat16>(dtype, q, nq, ldq, x, n, ldx, d, targets, scale, ignore_index, reduction, grad,
+                                     stats, dq, lddq, dx, lddx, ws, s);
 }
 
 }  // extern "C"
