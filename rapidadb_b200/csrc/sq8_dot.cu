@@ -161,21 +161,46 @@ struct DotPolicy {
         float xs;
     };
 
-    __device__ __forceinline__ void begin(Epi& e, const Job& j, int row, int) const {
-        const int64_t r = static_cast<int64_t>(j.m0) + row;
+    __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx& c) const {
+        const int64_t r = static_cast<int64_t>(j.m0) + c.row;
         e.xs = r < a.n ? a.xs[r] : 0.f;
+        // the tile's query scales
+        const int i = (c.grp * 4 + c.quad) * 32 + c.lane;
+        if (i < j.nn) reinterpret_cast<float*>(c.tile)[i] = j.n0 + i < a.nq ? a.qs[j.n0 + i] : 0.f;
     }
 
-    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
-        const int64_t x = static_cast<int64_t>(j.m0) + row, b0 = j.n0 + col;
-        if (x >= a.n) return;
-        T* o = static_cast<T*>(a.out) + b0 * a.ldo + x;
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
+                                          const uint32_t (&r)[32]) const {
+        const int64_t x = static_cast<int64_t>(j.m0) + c.row, b0 = j.n0 + col;
+        if (x >= a.n || b0 >= a.nq) return;
+        const float4* qs = reinterpret_cast<const float4*>(c.tile) + col / 4;
+        char* o = reinterpret_cast<char*>(static_cast<T*>(a.out) + b0 * a.ldo + x);
+        const int64_t step = a.ldo * static_cast<int64_t>(sizeof(T));
+        const int valid = static_cast<int>(min(static_cast<int64_t>(32), a.nq - b0));
+        const uint64_t xs2 = pack2(e.xs, e.xs);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (b0 + i < a.nq) o[i * a.ldo] = from_f<T>(score(__ldg(a.qs + b0 + i), e.xs, static_cast<int>(r[i])));
+        for (int i = 0; i < 32; i += 4) {
+            const float4 q = qs[i / 4];
+            float v[4];
+            unpack2(mul_f32x2(mul_f32x2(pack2(q.x, q.y), xs2),
+                              pack2(static_cast<float>(static_cast<int>(r[i])), static_cast<float>(static_cast<int>(r[i + 1])))),
+                    v[0], v[1]);
+            unpack2(mul_f32x2(mul_f32x2(pack2(q.z, q.w), xs2), pack2(static_cast<float>(static_cast<int>(r[i + 2])),
+                                                                     static_cast<float>(static_cast<int>(r[i + 3])))),
+                    v[2], v[3]);
+            if (valid == 32) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k, o += step) *reinterpret_cast<T*>(o) = from_f<T>(v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k, o += step)
+                    if (i + k < valid) *reinterpret_cast<T*>(o) = from_f<T>(v[k]);
+            }
+        }
     }
 
-    __device__ __forceinline__ void end(Epi&, const Job&, int, int) const {}
+    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
+    __device__ __forceinline__ void finish(const TileCtx&) const {}
 };
 
 template <typename T>

@@ -4,12 +4,17 @@
 // A CTA pair (cluster of 2, cta_group::2) computes one 256 x nn tile after the
 // other, nn <= 256, D = sum_k A[m, k] B[n, k]:
 //   warp 0      TMA producer: per K block of 128 bytes each CTA loads its 128
-//               rows of A and its nn / 2 rows of B into a 6-stage ring.
+//               rows of A and its nn / 2 rows of B into a 5-stage ring (4 to 6
+//               stages measure the same).
 //   warp 1      TMEM (two 256-column accumulators); the leader's lane 0 issues
 //               the MMAs and commits stage releases and finished accumulators.
-//   warps 2..9  epilogue, two per TMEM lane quadrant: a thread owns one row of
-//               its CTA's 128 and every other 32-column chunk of the tile,
-//               while the MMAs of the next tile fill the other accumulator.
+//   warps 2..17 epilogue, four per TMEM lane quadrant: a thread owns one row of
+//               its CTA's 128 and every fourth 32-column chunk of the tile (at
+//               most two).  It takes both into registers and releases the
+//               accumulator before it works on them, so the MMAs run up to two
+//               tiles ahead.  (Eight warps with one chunk in flight left the
+//               MMAs waiting: 4,096 x 131,072 x 128 forward 306 us, 137 us
+//               with no epilogue at all.)
 // An operand lies either K-major in memory (a row's K elements contiguous: one
 // box of 128 bytes x 128 rows per stage) or MN-major (the rows' index
 // contiguous: boxes of 64 elements x 64 K rows).  Both use the 128-byte
@@ -26,9 +31,10 @@
 //   P::Iter(p, pair, npairs)       the pair's tiles: bool next(job), the same
 //                                  sequence in every role
 //   P::Epi                         per-thread epilogue state
-//   p.begin(epi, job, row, half), p.chunk(epi, job, row, col, r),
-//   p.end(epi, job, row, half)     row of the tile, half of its chunks, 32
-//                                  accumulators from column col on
+//   p.begin(epi, job, ctx), p.chunk(epi, job, ctx, col, r), p.end(epi, job, ctx)
+//                                  r: 32 accumulators from column col on; what
+//                                  begin() writes to ctx.tile is seen by every
+//                                  chunk() of the tile; p.finish(ctx) once
 //
 // Every mbarrier wait is bounded: a role that gives up raises the CTA's abort
 // flag and the device status word (also in its host copy), waits (bounded) for
@@ -42,14 +48,17 @@ namespace {
 
 constexpr int TT_M = 256;         // rows of a pair's tile
 constexpr int TT_N = 256;         // largest columns of a tile
-constexpr int TT_STAGES = 6;
+constexpr int TT_STAGES = 5;
 constexpr int TT_A_BYTES = 16384;  // 128 rows x 128 bytes
 constexpr int TT_STAGE_BYTES = 2 * TT_A_BYTES;
 constexpr int TT_BLOCK_BYTES = 8192;  // 64 elements x 64 K rows (MN-major)
-constexpr int TT_EPI_WARPS = 8;
+constexpr int TT_EPI_WARPS = 16;
+constexpr int TT_GROUPS = TT_EPI_WARPS / 4;  // warps per TMEM lane quadrant
 constexpr int TT_THREADS = 64 + 32 * TT_EPI_WARPS;
 constexpr int TT_BAR_BYTES = 256;
-constexpr int TT_SMEM = TT_STAGES * TT_STAGE_BYTES + 1024 + TT_BAR_BYTES;
+constexpr int TT_STG_BYTES = 4096;           // per epilogue warp: 32 rows x 32 columns on their way out
+constexpr int TT_TILE_BYTES = 1024;          // or, per accumulator, a policy's values of the tile
+constexpr int TT_SMEM = TT_STAGES * TT_STAGE_BYTES + TT_EPI_WARPS * TT_STG_BYTES + TT_BAR_BYTES + 1024;
 static_assert(TT_SMEM <= 232448, "shared memory over 227 KB");
 
 // products of planes (A plane, B plane), largest first
@@ -119,6 +128,70 @@ __device__ __forceinline__ bool tt_epi_and(bool ok) {
     return r != 0;
 }
 
+// What an epilogue thread knows of its place.
+struct TileCtx {
+    int row;        // row of the pair's tile
+    int quad, grp;  // TMEM lane quadrant, which of its four warps
+    int lane;
+    uint8_t* stg;   // the warp's staging bytes (1024-byte aligned)
+    uint8_t* tile;  // this accumulator's TT_TILE_BYTES, shared by the CTA's epilogue: the
+                    // same memory as the staging bytes, so a policy uses one of them
+};
+
+// The four warps of one lane quadrant.
+__device__ __forceinline__ void tt_quad_sync(int quad) {
+    asm volatile("bar.sync %0, %1;" ::"r"(2 + quad), "n"(32 * TT_GROUPS) : "memory");
+}
+
+// ---- staged stores: a warp writes 32 rows of 64 or 128 bytes to its staging
+// bytes in the tensor map's swizzle (conflict-free: every lane its own row) and
+// one lane sends them with a TMA store, which clips at the matrix's edges.
+
+// byte offset of 16-byte unit u of row r: rows of 128 bytes, 128-byte swizzle
+__device__ __forceinline__ uint32_t stg_off128(int r, int u) {
+    return static_cast<uint32_t>(r * 128 + ((u ^ (r & 7)) << 4));
+}
+// rows of 64 bytes, 64-byte swizzle
+__device__ __forceinline__ uint32_t stg_off64(int r, int u) {
+    return static_cast<uint32_t>(r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+}
+
+// the staging bytes may be written again
+__device__ __forceinline__ void stg_wait_read(int lane) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+}
+
+template <bool ADD>
+__device__ __forceinline__ void stg_send(const CUtensorMap* map, const void* src, int lane, int x, int y, int z) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+        if (ADD)
+            asm volatile(
+                "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                    reinterpret_cast<uint64_t>(map)),
+                "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+                : "memory");
+        else
+            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                             reinterpret_cast<uint64_t>(map)),
+                         "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+                         : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+
+__device__ __forceinline__ void stg_drain(int lane) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 struct TileStatus {
     unsigned *word, *mirror;  // device status word, its copy in mapped host memory
 };
@@ -134,7 +207,8 @@ __device__ __forceinline__ void tt_give_up(volatile int* abort_flag, const TileS
 template <class P>
 __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const bool bf16, const TileStatus st) {
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + TT_STAGES * TT_STAGE_BYTES);
+    uint8_t* stg = smem + TT_STAGES * TT_STAGE_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(stg + TT_EPI_WARPS * TT_STG_BYTES);
     uint64_t* empty = full + TT_STAGES;
     uint64_t* tfull = empty + TT_STAGES;
     uint64_t* tempty = tfull + 2;
@@ -169,6 +243,7 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
     cluster_sync_all();  // both CTAs' barriers initialised before any remote use
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    static_assert(TT_N / 32 <= 2 * TT_GROUPS, "at most two chunks per epilogue warp");
 
     if (warp == 0) {
         if (lane == 0) {
@@ -292,9 +367,12 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
         }
     } else {
         // -------------------------------------------------- epilogue
-        const int quad = warp & 3;           // TMEM lanes this warp may read
-        const int half = (warp - 2) >> 2;    // which of every two 32-column chunks
-        const int row = static_cast<int>(rank) * 128 + quad * 32 + lane;  // row of the pair's tile
+        TileCtx ctx;
+        ctx.quad = warp & 3;  // TMEM lanes this warp may read
+        ctx.grp = (warp - 2) >> 2;
+        ctx.lane = lane;
+        ctx.row = static_cast<int>(rank) * 128 + ctx.quad * 32 + lane;
+        ctx.stg = stg + (warp - 2) * TT_STG_BYTES;
         const uint32_t tempty_lead = map_to_rank(&tempty[0], 0);
         typename P::Epi epi;
         typename P::Job j;
@@ -302,41 +380,34 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
         uint32_t tile = 0;
         for (; it.next(j); ++tile) {
             const int acc = tile & 1;
-            p.begin(epi, j, row, half);
+            // the buffer of two tiles ago: every warp has passed a barrier since
+            ctx.tile = stg + acc * TT_TILE_BYTES;
+            p.begin(epi, j, ctx);
             // all epilogue warps leave together if any wait gave up
             if (!tt_epi_and(mbar_wait(&tfull[acc], (tile >> 1) & 1, abort_flag))) {
                 tt_give_up(abort_flag, st, DEV_TIMEOUT_EPILOGUE);
                 break;
             }
             tc_fence_after();
+            const int c0 = ctx.grp * 32, c1 = c0 + TT_GROUPS * 32;
             const uint32_t tbase =
-                tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * TT_N);
-            const int nch = j.nn / 32;
+                tmem_base + (static_cast<uint32_t>(ctx.quad * 32) << 16) + static_cast<uint32_t>(acc * TT_N);
             uint32_t ra[32], rb[32];
-            if (half < nch) {
-                tmem_ld32_async(tbase + static_cast<uint32_t>(half * 32), ra);
-                tmem_ld_wait(ra);
-            }
-#pragma unroll 1
-            for (int c = half; c < nch; c += 4) {
-                // the next chunk's TMEM load is in flight while this one is processed
-                if (c + 2 < nch) tmem_ld32_async(tbase + static_cast<uint32_t>((c + 2) * 32), rb);
-                p.chunk(epi, j, row, c * 32, ra);
-                __syncwarp();  // the TMEM loads are warp-wide
-                if (c + 2 < nch) {
-                    tmem_ld_wait(rb);
-                    if (c + 4 < nch) tmem_ld32_async(tbase + static_cast<uint32_t>((c + 4) * 32), ra);
-                    p.chunk(epi, j, row, (c + 2) * 32, rb);
-                    __syncwarp();
-                    if (c + 4 < nch) tmem_ld_wait(ra);
-                }
-            }
+            if (c0 < j.nn) tmem_ld32_async(tbase + static_cast<uint32_t>(c0), ra);
+            if (c1 < j.nn) tmem_ld32_async(tbase + static_cast<uint32_t>(c1), rb);
+            tmem_ld_wait(ra);
+            tmem_ld_wait(rb);
             tc_fence_before();
             __syncwarp();
             if (lane == 0)
                 mbar_arrive_cluster_relaxed(tempty_lead + static_cast<uint32_t>(acc * sizeof(uint64_t)));
-            p.end(epi, j, row, half);
+            if (c0 < j.nn) p.chunk(epi, j, ctx, c0, ra);
+            __syncwarp();  // the staged stores are warp-wide
+            if (c1 < j.nn) p.chunk(epi, j, ctx, c1, rb);
+            __syncwarp();
+            p.end(epi, j, ctx);
         }
+        p.finish(ctx);
     }
     tc_fence_before();
     __syncthreads();
@@ -364,6 +435,23 @@ int make_map_3d(CUtensorMap* m, CUtensorMapDataType type, int elem, const void* 
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(m, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(RDB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return RDB_OK;
+}
+
+// planes x [rows, cols] matrices in boxes of 32 columns x 32 rows, for staged stores
+int make_store_map(CUtensorMap* m, CUtensorMapDataType type, int elem, const void* base, int64_t cols, int64_t rows,
+                   int64_t planes, int64_t ld_bytes, int64_t plane_bytes) {
+    auto fn = encode_fn();
+    if (!fn) return set_error(RDB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    if (planes == 1) plane_bytes = ld_bytes < (1LL << 40) / rows ? ld_bytes * rows : ld_bytes;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld_bytes), static_cast<cuuint64_t>(plane_bytes)};
+    cuuint32_t box[3] = {32, 32, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    elem == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(RDB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return RDB_OK;
 }

@@ -10,8 +10,7 @@
 // Forward: one pass over the rows.  The sum is taken in base 2 around a running
 // maximum in the epilogue of each 256 x 256 tile, c = scale log2 e,
 //   m = max_n c <q, x_n>,   z = sum_n 2^(c <q, x_n> - m),
-// held in fp32, one (m, z) per query, row split and epilogue half, joined by
-// xent_join_kernel.  The target's own term stays out of the running sum: with
+// held in fp32, one (m, z) per query and row split, joined by xent_join_kernel.  The target's own term stays out of the running sum: with
 // r = the sum of the other terms relative to the target's, loss = log1p(r), so
 // a query that finds its row keeps a loss near 0, and its p - 1 = expm1(-loss),
 // to full precision.
@@ -65,6 +64,20 @@ __device__ __forceinline__ float ex2(float v) {
     return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// (M, Z) of two sets of terms: the larger maximum, and the sums relative to it.
+// A set without finite terms has M = -inf and Z = 0 (or NaN).
+__device__ __forceinline__ void join(float& M, float& Z, float m, float z, float c) {
+    const float nm = fmaxf(M, m);
+    Z = Z * (M > -INFINITY ? ex2((M - nm) * c) : 1.f) + z * (m > -INFINITY ? ex2((m - nm) * c) : 1.f);
+    M = nm;
+}
+
 // two floats in the 16-bit type, a in the low half
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b);
@@ -96,7 +109,7 @@ struct FwdArgs {
     int nkb, nseg;
     float c;
     const int64_t* targets;
-    float2* part;        // [2 * slots][nq] (max <q, x>, z) of each split and half
+    float2* part;        // [slots][nq] (max <q, x>, z) of each split
     float* tdot;         // [nq] <q, x_t>
 };
 
@@ -142,15 +155,17 @@ struct FwdPolicy {
         int64_t tgt;     // target as a row of the piece (any value: not there)
     };
 
-    __device__ __forceinline__ void begin(Epi& e, const Job& j, int row, int) const {
+    __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx& c) const {
         if (!j.first) return;
         e.m = -INFINITY;
         e.mb = e.z = 0.f;
-        const int64_t b = j.m0 + row;
+        const int64_t b = j.m0 + c.row;
         e.tgt = b < a.nq ? a.targets[b] - a.row0 : -1;
     }
 
-    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
+                                          const uint32_t (&r)[32]) const {
+        if (j.m0 + c.row - c.lane >= a.nq) return;  // no query in this warp's 32 rows
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
@@ -163,39 +178,58 @@ struct FwdPolicy {
         const int64_t rel = e.tgt - c0;
         if (rel >= 0 && rel < 32 && e.tgt < a.n) {
             // the target's own term is kept apart
-            a.tdot[j.m0 + row] = pick32(v, static_cast<int>(rel));
+            a.tdot[j.m0 + c.row] = pick32(v, static_cast<int>(rel));
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 v[i] = i == static_cast<int>(rel) ? -INFINITY : v[i];
         }
-        float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
+        float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
 #pragma unroll
-        for (int i = 4; i < 32; i += 4) {
-            m0 = fmaxf(m0, fmaxf(v[i], v[i + 1]));
-            m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
+        for (int i = 6; i < 30; i += 4) {
+            m0 = max3(m0, v[i], v[i + 1]);
+            m1 = max3(m1, v[i + 2], v[i + 3]);
         }
+        m0 = max3(m0, v[30], v[31]);
         m0 = fmaxf(m0, m1);
         if (m0 > e.m) {
             e.z *= ex2((e.m - m0) * a.c);  // 0 before the first finite value
             e.m = m0;
             e.mb = m0 * a.c;
         }
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        // two columns per instruction
+        const uint64_t c2 = pack2(a.c, a.c), b2 = pack2(-e.mb, -e.mb);
+        uint64_t s0 = 0, s1 = 0;
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-            s0 += ex2(fmaf(v[i], a.c, -e.mb));
-            s1 += ex2(fmaf(v[i + 1], a.c, -e.mb));
-            s2 += ex2(fmaf(v[i + 2], a.c, -e.mb));
-            s3 += ex2(fmaf(v[i + 3], a.c, -e.mb));
+            float x0, x1, x2, x3;
+            unpack2(fma_f32x2(pack2(v[i], v[i + 1]), c2, b2), x0, x1);
+            unpack2(fma_f32x2(pack2(v[i + 2], v[i + 3]), c2, b2), x2, x3);
+            s0 = add_f32x2(s0, pack2(ex2(x0), ex2(x1)));
+            s1 = add_f32x2(s1, pack2(ex2(x2), ex2(x3)));
         }
-        e.z += (s0 + s1) + (s2 + s3);
+        float p0, p1;
+        unpack2(add_f32x2(s0, s1), p0, p1);
+        e.z += p0 + p1;
     }
 
-    __device__ __forceinline__ void end(Epi& e, const Job& j, int row, int half) const {
-        const int64_t b = j.m0 + row;
-        if (j.last && b < a.nq)
-            a.part[(2 * static_cast<int64_t>(a.slot0 + j.split) + half) * a.nq + b] = make_float2(e.m, e.z);
+    __device__ __forceinline__ void end(Epi& e, const Job& j, const TileCtx& c) const {
+        if (!j.last) return;
+        // the four warps of a row join through shared memory
+        float2* sh = reinterpret_cast<float2*>(c.stg - c.grp * 4 * TT_STG_BYTES);  // the first group's staging bytes
+        if (c.grp > 0) sh[c.grp * 32 + c.lane] = make_float2(e.m, e.z);
+        tt_quad_sync(c.quad);
+        const int64_t b = j.m0 + c.row;
+        if (c.grp == 0) {
+#pragma unroll
+            for (int g = 1; g < TT_GROUPS; ++g) {
+                const float2 o = sh[g * 32 + c.lane];
+                join(e.m, e.z, o.x, o.y, a.c);
+            }
+            if (b < a.nq) a.part[static_cast<int64_t>(a.slot0 + j.split) * a.nq + b] = make_float2(e.m, e.z);
+        }
+        tt_quad_sync(c.quad);  // read before the next unit writes
     }
+    __device__ __forceinline__ void finish(const TileCtx&) const {}
 };
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
@@ -208,28 +242,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
 
 // Joins the parts of 32 queries per block; stats and loss of each query.  An
 // ignored query has loss 0; one whose target is no row is NaN throughout.
-__global__ void __launch_bounds__(NT)
+constexpr int JG = 16;  // threads per query
+__global__ void __launch_bounds__(32 * JG)
     xent_join_kernel(const float2* part, int slots, const float* tdot, const int64_t* targets, int64_t ignore,
                      int64_t n, float c, int64_t nq, float* stats, float* loss) {
-    __shared__ float2 sh[NW][32];
+    __shared__ float2 sh[JG][32];
     const int qi = threadIdx.x & 31, g = threadIdx.x >> 5;
     const int64_t b = static_cast<int64_t>(blockIdx.x) * 32 + qi;
     float M = -INFINITY, Z = 0.f;
-    auto add = [&](float m, float z) {
-        const float nm = fmaxf(M, m);
-        Z = Z * (M > -INFINITY ? ex2((M - nm) * c) : (Z == Z ? 0.f : Z)) +
-            z * (m > -INFINITY ? ex2((m - nm) * c) : (z == z ? 0.f : z));
-        M = nm;
-    };
     if (b < nq)
-        for (int s = g; s < slots; s += NW) {
+        for (int s = g; s < slots; s += JG) {
             const float2 v = part[static_cast<int64_t>(s) * nq + b];
-            add(v.x, v.y);
+            join(M, Z, v.x, v.y, c);
         }
     sh[g][qi] = make_float2(M, Z);
     __syncthreads();
     if (g != 0 || b >= nq) return;
-    for (int k = 1; k < NW; ++k) add(sh[k][qi].x, sh[k][qi].y);
+    for (int k = 1; k < JG; ++k) join(M, Z, sh[k][qi].x, sh[k][qi].y, c);
     const int64_t t = targets[b];
     const bool ignored = t == ignore, has = t >= 0 && t < n;
     const float nan = __int_as_float(0x7fc00000);
@@ -359,15 +388,13 @@ struct ProbArgs {
     const int64_t* targets;
     int64_t ignore;
     const float* stats;
-    void* g;              // [planes][nq][ldg]
-    int64_t ldg;
 };
 
 // G tiles of one piece: 2^14 (p - [n = t])
 template <typename T>
 struct ProbPolicy {
     static constexpr bool kInt8 = false;
-    const CUtensorMap *mq, *mx;
+    const CUtensorMap *mq, *mx, *mg;
     const ProbArgs& a;
 
     using Job = TileJob;
@@ -393,74 +420,85 @@ struct ProbPolicy {
     struct Epi {
         float m, lz, hit;
         int64_t tgt;
-        bool in, ignored;
+        bool ignored;
     };
 
-    __device__ __forceinline__ void begin(Epi& e, const Job& j, int row, int) const {
-        const int64_t b = j.m0 + row;
-        e.in = b < a.nq;
-        if (!e.in) return;
+    __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx& c) const {
+        const int64_t b = j.m0 + c.row;
+        e.ignored = true;
+        e.tgt = -1;
+        e.m = e.lz = e.hit = 0.f;
+        if (b >= a.nq) return;
         const int64_t t = a.targets[b];
         e.ignored = t == a.ignore;
-        e.tgt = t - a.row0;
+        if (!e.ignored) e.tgt = t - a.row0;
         e.m = a.stats[b];
         e.lz = a.stats[a.nq + b] - kGLog2;
         e.hit = a.stats[2 * a.nq + b];
     }
 
-    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
-        if (!e.in) return;
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
+                                          const uint32_t (&r)[32]) const {
+        const int y = j.m0 + c.row - c.lane, x = j.n0 + col;
+        if (y >= a.nq || x >= a.n) return;
         float v[32];
         // two roundings, of the exponent relative to the largest logit and of
         // the one relative to their sum: both small for the terms that count
+        const uint64_t c2 = pack2(a.c, a.c), m2 = pack2(-e.m, -e.m), z2 = pack2(-e.lz, -e.lz);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            v[i] = e.ignored ? 0.f : ex2(fmaf(__uint_as_float(r[i]), a.c, -e.m) - e.lz);
-        const int64_t c0 = static_cast<int64_t>(j.n0) + col;
-        const int64_t rel = e.tgt - c0;
-        if (rel >= 0 && rel < 32 && !e.ignored) {
+        for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            unpack2(add_f32x2(fma_f32x2(pack2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), c2, m2), z2), x0, x1);
+            v[i] = ex2(x0);
+            v[i + 1] = ex2(x1);
+        }
+        if (e.ignored) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+        const int64_t rel = e.tgt - x;
+        if (rel >= 0 && rel < 32) {
             const float h = kGScale * expm1f(-e.hit);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 v[i] = i == static_cast<int>(rel) ? h : v[i];
         }
-        // columns behind the piece's last row are never read
-        if constexpr (sizeof(T) == 2) {
-            uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.g) + (j.m0 + row) * a.ldg + c0);
+        __syncwarp();
+        // (columns behind the piece's last row lie outside the map)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                o[i] = make_uint4(pack16<T>(v[8 * i], v[8 * i + 1]), pack16<T>(v[8 * i + 2], v[8 * i + 3]),
-                                  pack16<T>(v[8 * i + 4], v[8 * i + 5]), pack16<T>(v[8 * i + 6], v[8 * i + 7]));
-        } else {
+        for (int k = 0; k < (sizeof(T) == 2 ? 1 : 3); ++k) {
+            stg_wait_read(c.lane);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.g) +
-                                                    (k * a.nq + j.m0 + row) * a.ldg + c0);
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        w[h] = pack16<__nv_bfloat16>(v[8 * i + 2 * h], v[8 * i + 2 * h + 1]);
+                for (int h = 0; h < 4; ++h) {
+                    float &a0 = v[8 * i + 2 * h], &a1 = v[8 * i + 2 * h + 1];
+                    if constexpr (sizeof(T) == 2) {
+                        w[h] = pack16<T>(a0, a1);
+                    } else {
+                        w[h] = pack16<__nv_bfloat16>(a0, a1);
                         // what is left for the next plane
-                        v[8 * i + 2 * h] -= __uint_as_float(w[h] << 16);
-                        v[8 * i + 2 * h + 1] -= __uint_as_float(w[h] & 0xffff0000u);
+                        a0 -= __uint_as_float(w[h] << 16);
+                        a1 -= __uint_as_float(w[h] & 0xffff0000u);
                     }
-                    o[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                *reinterpret_cast<uint4*>(c.stg + stg_off64(c.lane, i)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+            stg_send<false>(mg, c.stg, c.lane, x, y, k);
         }
     }
 
-    __device__ __forceinline__ void end(Epi&, const Job&, int, int) const {}
+    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
+    __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
 
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     xent_prob_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mx,
-                     const __grid_constant__ ProbArgs a, const bool bf16, const TileStatus st) {
+                     const __grid_constant__ CUtensorMap mg, const __grid_constant__ ProbArgs a, const bool bf16, const TileStatus st) {
     extern __shared__ uint8_t smem_raw[];
-    const ProbPolicy<T> p{&mq, &mx, a};
+    const ProbPolicy<T> p{&mq, &mx, &mg, a};
     tile_loop(smem_raw, p, bf16, st);
 }
 
@@ -473,11 +511,9 @@ struct GradArgs {
     int x_blocks;          // dx: 256-row blocks (0: not wanted)
     bool q_first;          // the longer tiles come first
     bool add;              // a piece before this one wrote the partial sums
-    float* part;           // [q_split][nq][dp]
-    int dp;
-    void* dx;              // rows of the piece
+    void* dx;              // rows of the piece, where dx_tma is false
     int64_t lddx;
-    bool dx_vec;           // 16-byte stores allowed
+    bool dx_tma;           // the rows of dx have 16-byte strides
     float scale;
     const float* wmax;
 };
@@ -485,7 +521,7 @@ struct GradArgs {
 template <typename T>
 struct GradPolicy {
     static constexpr bool kInt8 = false;
-    const CUtensorMap *gk, *gmn, *xmn, *qmn;
+    const CUtensorMap *gk, *gmn, *xmn, *qmn, *mpart, *mdx;
     const GradArgs& a;
 
     struct Job : TileJob {
@@ -533,35 +569,28 @@ struct GradPolicy {
         float f;
     };
 
-    __device__ __forceinline__ void begin(Epi& e, const Job&, int, int) const {
-        e.f = a.scale * (1.f / kGScale) * *a.wmax;
+    __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx&) const {
+        e.f = j.is_dx ? a.scale * (1.f / kGScale) * *a.wmax : 1.f;
     }
 
-    __device__ __forceinline__ void chunk(Epi& e, const Job& j, int row, int col, const uint32_t (&r)[32]) const {
-        const int64_t m = j.m0 + row;
-        const int t0 = j.n0 + col;
-        if (t0 >= a.d) return;
-        if (!j.is_dx) {
-            if (m >= a.nq) return;
-            // dp is a multiple of 32: the columns behind d hold zeros
-            float4* o = reinterpret_cast<float4*>(a.part + (j.split * a.nq + m) * a.dp + t0);
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
+                                          const uint32_t (&r)[32]) const {
+        const int y = j.m0 + c.row - c.lane, x = j.n0 + col;
+        if (x >= a.d || y >= (j.is_dx ? a.n : a.nq)) return;
+        if (j.is_dx && !a.dx_tma) {
+            // rows that no tensor map can describe
+            if (y + c.lane >= a.n) return;
+            T* o = static_cast<T*>(a.dx) + static_cast<int64_t>(y + c.lane) * a.lddx + x;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float4 v = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
-                                       __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
-                if (a.add) {
-                    const float4 w = o[i];
-                    v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
-                }
-                o[i] = v;
-            }
+            for (int i = 0; i < 32; ++i)
+                if (x + i < a.d) o[i] = from_f<T>(__uint_as_float(r[i]) * e.f);
             return;
         }
-        if (m >= a.n) return;
-        T* o = static_cast<T*>(a.dx) + m * a.lddx + t0;
-        if (a.dx_vec && t0 + 32 <= a.d) {
-            uint4* o4 = reinterpret_cast<uint4*>(o);
-            if constexpr (sizeof(T) == 2) {
+        stg_wait_read(c.lane);
+        bool wide = true;
+        if constexpr (sizeof(T) == 2) {
+            if (j.is_dx) {
+                wide = false;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t w[4];
@@ -569,34 +598,37 @@ struct GradPolicy {
                     for (int h = 0; h < 4; ++h)
                         w[h] = pack16<T>(__uint_as_float(r[8 * i + 2 * h]) * e.f,
                                          __uint_as_float(r[8 * i + 2 * h + 1]) * e.f);
-                    o4[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) w[h] = __float_as_uint(__uint_as_float(r[4 * i + h]) * e.f);
-                    o4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(c.stg + stg_off64(c.lane, i)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (t0 + i < a.d) o[i] = from_f<T>(__uint_as_float(r[i]) * e.f);
         }
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(c.stg + stg_off128(c.lane, i)) =
+                    make_float4(__uint_as_float(r[4 * i]) * e.f, __uint_as_float(r[4 * i + 1]) * e.f,
+                                __uint_as_float(r[4 * i + 2]) * e.f, __uint_as_float(r[4 * i + 3]) * e.f);
+        }
+        if (j.is_dx)
+            stg_send<false>(mdx, c.stg, c.lane, x, y, 0);
+        else if (a.add)
+            stg_send<true>(mpart, c.stg, c.lane, x, y, j.split);
+        else
+            stg_send<false>(mpart, c.stg, c.lane, x, y, j.split);
     }
 
-    __device__ __forceinline__ void end(Epi&, const Job&, int, int) const {}
+    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
+    __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
 
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     xent_grad_kernel(const __grid_constant__ CUtensorMap gk, const __grid_constant__ CUtensorMap gmn,
                      const __grid_constant__ CUtensorMap xmn, const __grid_constant__ CUtensorMap qmn,
+                     const __grid_constant__ CUtensorMap mpart, const __grid_constant__ CUtensorMap mdx,
                      const __grid_constant__ GradArgs a, const bool bf16, const TileStatus st) {
     extern __shared__ uint8_t smem_raw[];
-    const GradPolicy<T> p{&gk, &gmn, &xmn, &qmn, a};
+    const GradPolicy<T> p{&gk, &gmn, &xmn, &qmn, &mpart, &mdx, a};
     tile_loop(smem_raw, p, bf16, st);
 }
 
@@ -716,7 +748,7 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
     const int64_t dp = up(d, 8);
     w.loss_q = a.take<float>(nq);
     w.tdot = a.take<float>(nq);
-    w.part = a.take<float2>(2 * (size_t)p.slots * nq);
+    w.part = a.take<float2>((size_t)p.slots * nq);
     if (dtype == RDB_F32) {
         w.qp = a.take<__nv_bfloat16>(3 * nq * dp);
         w.xp = a.take<__nv_bfloat16>(3 * p.rows * dp);
@@ -856,8 +888,6 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     pa.targets = targets;
     pa.ignore = ignore;
     pa.stats = stats;
-    pa.g = w.g;
-    pa.ldg = p.rows;
     GradArgs ga{};
     ga.nq = nq;
     ga.d = d;
@@ -866,13 +896,15 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     ga.q_per = p.q_per;
     ga.kq = p.kq;
     ga.q_first = p.q_first;
-    ga.part = w.part;
-    ga.dp = p.dp;
     ga.lddx = lddx;
-    ga.dx_vec = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (lddx * (int64_t)sizeof(T)) % 16 == 0;
+    ga.dx_tma = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (lddx * (int64_t)sizeof(T)) % 16 == 0;
     ga.scale = scale;
     ga.wmax = w.wmax;
     const Planes go{w.g, p.rows, nq * p.rows, p.planes};
+    CUtensorMap mpart = mq, mdx = mq;  // (any valid map where there is nothing to store)
+    if (dq)
+        RDB_TRY(make_store_map(&mpart, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, w.part, p.dp, nq, p.q_split, 4LL * p.dp,
+                               4LL * p.dp * nq));
 
     for (int i = 0; i < p.pieces; ++i) {
         const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
@@ -883,13 +915,15 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         RDB_TRY(operand_map(&mxmn, dtype, xo, d, rows, true));
         RDB_TRY(operand_map(&mgk, dtype, go, rows, nq, false));
         RDB_TRY(operand_map(&mgmn, dtype, go, rows, nq, true));
+        CUtensorMap mg;
+        RDB_TRY(make_store_map(&mg, map_type(dtype), 2, w.g, rows, nq, p.planes, 2 * p.rows, 2 * p.rows * nq));
         pa.n = rows;
         pa.row0 = r0;
         const int64_t tiles = (rows + TT_N - 1) / TT_N * p.nqb;
         RDB_CHECK_ARG(tiles < (1LL << 31), "too many tiles for one launch");
         pa.njobs = (int)tiles;
-        xent_prob_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS, TT_SMEM, s>>>(mq, mx, pa, bf16,
-                                                                                                      st);
+        xent_prob_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS, TT_SMEM, s>>>(mq, mx, mg, pa,
+                                                                                                      bf16, st);
         RDB_LAUNCH_CHECK();
         ga.n = rows;
         ga.kc = (int)((rows + 63) / 64);
@@ -899,10 +933,14 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         ga.x_blocks = dx ? (int)((rows + TT_M - 1) / TT_M) : 0;
         ga.add = i > 0;
         ga.dx = dx ? static_cast<T*>(dx) + r0 * lddx : nullptr;
+        if (ga.dx_tma)
+            RDB_TRY(make_store_map(&mdx, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(dtype),
+                                   (int)sizeof(T), ga.dx, d, rows, 1, lddx * (int64_t)sizeof(T), 0));
         const int64_t jobs = (int64_t)ga.nt * ((int64_t)ga.q_blocks * ga.q_split + ga.x_blocks);
         RDB_CHECK_ARG(jobs < (1LL << 31), "too many tiles for one launch");
-        xent_grad_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM, s>>>(mgk, mgmn, mxmn,
-                                                                                                     mqw, ga, bf16, st);
+        xent_grad_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM, s>>>(mgk, mgmn, mxmn, mqw,
+                                                                                                     mpart, mdx, ga, bf16,
+                                                                                                     st);
         RDB_LAUNCH_CHECK();
     }
     if (dq) {
@@ -972,7 +1010,7 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
                 mq, mx, a, dtype != RDB_F16, st);
             RDB_LAUNCH_CHECK();
         }
-        xent_join_kernel<<<(unsigned)((nq + 31) / 32), NT, 0, s>>>(w.part, 2 * p.slots, w.tdot, targets, ignore_index,
+        xent_join_kernel<<<(unsigned)((nq + 31) / 32), 32 * JG, 0, s>>>(w.part, p.slots, w.tdot, targets, ignore_index,
                                                                    n, c, nq, stats, loss_q);
         RDB_LAUNCH_CHECK();
     }
