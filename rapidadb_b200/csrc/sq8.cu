@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace rdb {
@@ -22,7 +24,7 @@ __device__ __forceinline__ float ld_any(int dtype, const void* p, int64_t i) {
     return __half2float(static_cast<const __half*>(p)[i]);
 }
 
-// one warp per row
+// one warp per row, any layout
 __global__ void sq8_encode_kernel(int dtype, const void* x, int64_t n, int64_t ldx, int d, int8_t* codes, int64_t ldc,
                                   float* scales) {
     const int lane = threadIdx.x & 31;
@@ -42,6 +44,112 @@ __global__ void sq8_encode_kernel(int dtype, const void* x, int64_t n, int64_t l
         codes[row * ldc + t] = static_cast<int8_t>(c);
     }
     if (lane == 0) scales[row] = scale;
+}
+
+// rint(x / scale) of the division's fp32 result, without the division: r = x *
+// (1 / scale) is within 127 * 2^-22 < 2^-15 of it (two roundings of 2^-24
+// relative each, and its own), so both round to the same integer unless r lies
+// within 2^-14 of a half.  Those (one in 10^4), and NaN and infinities, divide.
+__device__ __forceinline__ float code_of(float x, float scale, float inv, bool& near_half) {
+    const float r = x * inv, c = rintf(r);
+    near_half |= !(fabsf(fabsf(r - c) - 0.5f) > 6.103515625e-05f);
+    return c;
+}
+
+__device__ __forceinline__ uint32_t pack_codes(const float* c) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w |= (static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(c[i], -127.f), 127.f))) & 0xffu) << (8 * i);
+    return w;
+}
+
+template <typename T>
+__device__ __forceinline__ void load16(const void* p, float (&v)[16 / sizeof(T)]) {
+    const uint4 u = __ldg(static_cast<const uint4*>(p));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        } else {
+            v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+
+// The same codes from rows of 16-byte units (d * size a multiple of 16 bytes,
+// bases and strides aligned): one warp per row, which it reads once, U units a
+// lane held in registers.  The bytes of the row and of its codes bound it.
+template <typename T, int U>
+__global__ void __launch_bounds__(256)
+    sq8_encode_rows_kernel(const T* __restrict__ x, int64_t n, int64_t ldx, int units, int8_t* __restrict__ codes,
+                           int64_t ldc, float* __restrict__ scales) {
+    constexpr int E = 16 / sizeof(T);  // elements of a unit
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= n) return;
+    float v[U][E];
+    float amax = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u * 32 + lane < units) load16<T>(x + row * ldx + (u * 32 + lane) * E, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u * 32 + lane < units)
+#pragma unroll
+            for (int i = 0; i < E; ++i) amax = fmaxf(amax, fabsf(v[u][i]));
+    // amax >= 0: its bits order like integers
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+    const float scale = __fdiv_rn(amax, 127.f), inv = __fdiv_rn(1.f, scale);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (u * 32 + lane >= units) continue;
+        float c[E];
+        bool near_half = false;
+#pragma unroll
+        for (int i = 0; i < E; ++i) c[i] = code_of(v[u][i], scale, inv, near_half);
+        if (near_half) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) c[i] = scale > 0.f ? rintf(__fdiv_rn(v[u][i], scale)) : 0.f;
+        }
+        int8_t* o = codes + row * ldc + (u * 32 + lane) * E;
+        if constexpr (E == 8)
+            *reinterpret_cast<uint2*>(o) = make_uint2(pack_codes(c), pack_codes(c + 4));
+        else
+            *reinterpret_cast<uint32_t*>(o) = pack_codes(c);
+    }
+    // columns behind d are zero
+    for (int64_t t = (int64_t)units * E + lane; t < ldc; t += 32) codes[row * ldc + t] = 0;
+    if (lane == 0) scales[row] = scale;
+}
+
+template <typename T>
+bool encode_rows(const void* x, int64_t n, int64_t ldx, int d, int8_t* codes, int64_t ldc, float* scales,
+                 cudaStream_t s) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int units = d / E;
+    if (d % E != 0 || ldx % E != 0 || ldc % E != 0 || (reinterpret_cast<uintptr_t>(x) & 15) != 0 ||
+        (reinterpret_cast<uintptr_t>(codes) & (E - 1)) != 0 || units > 256)
+        return false;
+    const unsigned blocks = (unsigned)((n + 7) / 8);
+    const T* p = static_cast<const T*>(x);
+    if (units <= 32)
+        sq8_encode_rows_kernel<T, 1><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
+    else if (units <= 64)
+        sq8_encode_rows_kernel<T, 2><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
+    else if (units <= 96)
+        sq8_encode_rows_kernel<T, 3><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
+    else if (units <= 128)
+        sq8_encode_rows_kernel<T, 4><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
+    else if (units <= 192)
+        sq8_encode_rows_kernel<T, 6><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
+    else
+        sq8_encode_rows_kernel<T, 8><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
+    return true;
 }
 
 // per-row metric value of the dequantised row: |x^|^2 (L2), |x^| or
@@ -76,7 +184,11 @@ int rdb_sq8_encode(int dtype, const void* x, int64_t n, int64_t ldx, int d, int8
     if (n == 0) return RDB_OK;
     RDB_CHECK_ARG(x && codes && scales, "NULL pointer");
     const unsigned blocks = (unsigned)((n + 7) / 8);
-    sq8_encode_kernel<<<blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(dtype, x, n, ldx, d, codes, ldc, scales);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool done = dtype == RDB_F32   ? encode_rows<float>(x, n, ldx, d, codes, ldc, scales, s)
+                      : dtype == RDB_F16 ? encode_rows<__half>(x, n, ldx, d, codes, ldc, scales, s)
+                                         : encode_rows<__nv_bfloat16>(x, n, ldx, d, codes, ldc, scales, s);
+    if (!done) sq8_encode_kernel<<<blocks, 256, 0, s>>>(dtype, x, n, ldx, d, codes, ldc, scales);
     RDB_LAUNCH_CHECK();
     return RDB_OK;
 }

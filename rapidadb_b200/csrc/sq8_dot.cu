@@ -41,6 +41,7 @@ __device__ __forceinline__ float score(float qs, float xs, int acc) {
 
 constexpr int GV_THREADS = 256;
 constexpr int GV_LANES = 8;               // lanes per row: 128 bytes of a row per load
+constexpr int GV_BATCH = 6;               // 16-byte loads a lane has in flight (768 codes: the whole row)
 constexpr int GV_SMEM = 48 * 1024;        // query codes
 
 // NQ queries at most (rounded up to a power of two).  Four rows per warp.
@@ -57,35 +58,48 @@ __global__ void __launch_bounds__(GV_THREADS)
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, sub = lane & (GV_LANES - 1);
-    const int rows_per_block = GV_THREADS / GV_LANES;
     const int full = d / 16;  // 16-byte chunks that lie inside the row
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows_per_block; r0 < n;
-         r0 += static_cast<int64_t>(gridDim.x) * rows_per_block) {
-        const int64_t r = r0 + threadIdx.x / GV_LANES;
-        const bool in = r < n;
-        const int8_t* x = xc + (in ? r : 0) * ldx;
+    // every warp an equal, contiguous share of the rows, four at a time
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * (GV_THREADS / 32) + threadIdx.x / 32;
+    const int64_t nw = static_cast<int64_t>(gridDim.x) * (GV_THREADS / 32);
+    const int64_t end = (w + 1) * n / nw;
+    for (int64_t r0 = w * n / nw; r0 < end; r0 += 32 / GV_LANES) {
+        const int64_t r = r0 + lane / GV_LANES;
+        const bool in = r < end;
+        const int8_t* x = xc + (in ? r : r0) * ldx;
         int acc[NQ];
 #pragma unroll
         for (int b = 0; b < NQ; ++b) acc[b] = 0;
-#pragma unroll 4
-        for (int c = sub; c < chunks; c += GV_LANES) {
-            int4 v;
-            if (c < full) {
-                v = __ldg(reinterpret_cast<const int4*>(x) + c);
-            } else {
-                // the row's last bytes: nothing behind them is read
-                uint32_t w[4] = {0u, 0u, 0u, 0u};
-                for (int t = c * 16; t < d; ++t)
-                    w[(t & 15) >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(x[t])) << (8 * (t & 3));
-                v = make_int4(w[0], w[1], w[2], w[3]);
+        // GV_BATCH chunks a lane in flight at once
+        for (int c0 = sub; c0 < chunks; c0 += GV_LANES * GV_BATCH) {
+            int4 v[GV_BATCH];
+#pragma unroll
+            for (int k = 0; k < GV_BATCH; ++k) {
+                const int c = c0 + k * GV_LANES;
+                v[k] = make_int4(0, 0, 0, 0);
+                if (c < full) {
+                    v[k] = __ldg(reinterpret_cast<const int4*>(x) + c);
+                } else if (c < chunks) {
+                    // the row's last bytes: nothing behind them is read
+                    uint32_t b[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int t = 0; t < 16; ++t)
+                        if (c * 16 + t < d)
+                            b[t >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(x[c * 16 + t])) << (8 * (t & 3));
+                    v[k] = make_int4(b[0], b[1], b[2], b[3]);
+                }
             }
 #pragma unroll
-            for (int b = 0; b < NQ; ++b) {
-                const int4 q = *reinterpret_cast<const int4*>(sq + b * dp + c * 16);
-                acc[b] = __dp4a(v.x, q.x, acc[b]);
-                acc[b] = __dp4a(v.y, q.y, acc[b]);
-                acc[b] = __dp4a(v.z, q.z, acc[b]);
-                acc[b] = __dp4a(v.w, q.w, acc[b]);
+            for (int k = 0; k < GV_BATCH; ++k) {
+                const int c = min(c0 + k * GV_LANES, chunks - 1);
+#pragma unroll
+                for (int b = 0; b < NQ; ++b) {
+                    const int4 q = *reinterpret_cast<const int4*>(sq + b * dp + c * 16);
+                    acc[b] = __dp4a(v[k].x, q.x, acc[b]);
+                    acc[b] = __dp4a(v[k].y, q.y, acc[b]);
+                    acc[b] = __dp4a(v[k].z, q.z, acc[b]);
+                    acc[b] = __dp4a(v[k].w, q.w, acc[b]);
+                }
             }
         }
 #pragma unroll
@@ -164,16 +178,27 @@ struct DotPolicy {
     __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx& c) const {
         const int64_t r = static_cast<int64_t>(j.m0) + c.row;
         e.xs = r < a.n ? a.xs[r] : 0.f;
-        // the tile's query scales
-        const int i = (c.grp * 4 + c.quad) * 32 + c.lane;
-        if (i < j.nn) reinterpret_cast<float*>(c.tile)[i] = j.n0 + i < a.nq ? a.qs[j.n0 + i] : 0.f;
+        // the query scales of the warp's 64 columns
+        float* qs = reinterpret_cast<float*>(c.stg);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t b = static_cast<int64_t>(j.n0) + h * 128 + c.grp * 32 + c.lane;
+            qs[h * 32 + c.lane] = b < a.nq ? a.qs[b] : 0.f;
+        }
+        __syncwarp();
     }
 
-    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
+    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
+                                         const uint32_t (&rb)[32]) const {
+        chunk(e, j, c, 0, ra);
+        chunk(e, j, c, 1, rb);
+    }
+
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int h,
                                           const uint32_t (&r)[32]) const {
-        const int64_t x = static_cast<int64_t>(j.m0) + c.row, b0 = j.n0 + col;
+        const int64_t x = static_cast<int64_t>(j.m0) + c.row, b0 = static_cast<int64_t>(j.n0) + h * 128 + c.grp * 32;
         if (x >= a.n || b0 >= a.nq) return;
-        const float4* qs = reinterpret_cast<const float4*>(c.tile) + col / 4;
+        const float4* qs = reinterpret_cast<const float4*>(c.stg) + h * 8;
         char* o = reinterpret_cast<char*>(static_cast<T*>(a.out) + b0 * a.ldo + x);
         const int64_t step = a.ldo * static_cast<int64_t>(sizeof(T));
         const int valid = static_cast<int>(min(static_cast<int64_t>(32), a.nq - b0));
@@ -199,7 +224,6 @@ struct DotPolicy {
         }
     }
 
-    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
     __device__ __forceinline__ void finish(const TileCtx&) const {}
 };
 

@@ -31,10 +31,13 @@
 //   P::Iter(p, pair, npairs)       the pair's tiles: bool next(job), the same
 //                                  sequence in every role
 //   P::Epi                         per-thread epilogue state
-//   p.begin(epi, job, ctx), p.chunk(epi, job, ctx, col, r), p.end(epi, job, ctx)
-//                                  r: 32 accumulators from column col on; what
-//                                  begin() writes to ctx.tile is seen by every
-//                                  chunk() of the tile; p.finish(ctx) once
+//   p.begin(epi, job, ctx)         while the tile is still being multiplied
+//   p.tile(epi, job, ctx, ra, rb)  the warp's accumulators: 32 from column
+//                                  32 grp on, 32 from column 128 + 32 grp on
+//                                  (where the tile is that wide)
+//   p.finish(ctx)                  once, after the last tile
+// The epilogue's warps never wait for one another: they drift apart by up to
+// two tiles, so that one's exponentials overlap another's maxima and stores.
 //
 // Every mbarrier wait is bounded: a role that gives up raises the CTA's abort
 // flag and the device status word (also in its host copy), waits (bounded) for
@@ -57,7 +60,6 @@ constexpr int TT_GROUPS = TT_EPI_WARPS / 4;  // warps per TMEM lane quadrant
 constexpr int TT_THREADS = 64 + 32 * TT_EPI_WARPS;
 constexpr int TT_BAR_BYTES = 256;
 constexpr int TT_STG_BYTES = 4096;           // per epilogue warp: 32 rows x 32 columns on their way out
-constexpr int TT_TILE_BYTES = 1024;          // or, per accumulator, a policy's values of the tile
 constexpr int TT_SMEM = TT_STAGES * TT_STAGE_BYTES + TT_EPI_WARPS * TT_STG_BYTES + TT_BAR_BYTES + 1024;
 static_assert(TT_SMEM <= 232448, "shared memory over 227 KB");
 
@@ -111,37 +113,13 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc_i8(int m, int n) {
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void tt_epi_sync() {
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * TT_EPI_WARPS) : "memory");
-}
-
-__device__ __forceinline__ bool tt_epi_and(bool ok) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred pin, pout;\n\t"
-        "setp.ne.u32 pin, %1, 0;\n\t"
-        "bar.red.and.pred pout, 1, %2, pin;\n\t"
-        "selp.u32 %0, 1, 0, pout;\n\t}"
-        : "=r"(r)
-        : "r"(ok ? 1u : 0u), "n"(32 * TT_EPI_WARPS)
-        : "memory");
-    return r != 0;
-}
-
 // What an epilogue thread knows of its place.
 struct TileCtx {
     int row;        // row of the pair's tile
     int quad, grp;  // TMEM lane quadrant, which of its four warps
     int lane;
-    uint8_t* stg;   // the warp's staging bytes (1024-byte aligned)
-    uint8_t* tile;  // this accumulator's TT_TILE_BYTES, shared by the CTA's epilogue: the
-                    // same memory as the staging bytes, so a policy uses one of them
+    uint8_t* stg;   // the warp's TT_STG_BYTES (1024-byte aligned)
 };
-
-// The four warps of one lane quadrant.
-__device__ __forceinline__ void tt_quad_sync(int quad) {
-    asm volatile("bar.sync %0, %1;" ::"r"(2 + quad), "n"(32 * TT_GROUPS) : "memory");
-}
 
 // ---- staged stores: a warp writes 32 rows of 64 or 128 bytes to its staging
 // bytes in the tensor map's swizzle (conflict-free: every lane its own row) and
@@ -380,14 +358,12 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
         uint32_t tile = 0;
         for (; it.next(j); ++tile) {
             const int acc = tile & 1;
-            // the buffer of two tiles ago: every warp has passed a barrier since
-            ctx.tile = stg + acc * TT_TILE_BYTES;
             p.begin(epi, j, ctx);
-            // all epilogue warps leave together if any wait gave up
-            if (!tt_epi_and(mbar_wait(&tfull[acc], (tile >> 1) & 1, abort_flag))) {
+            if (!mbar_wait(&tfull[acc], (tile >> 1) & 1, abort_flag)) {
                 tt_give_up(abort_flag, st, DEV_TIMEOUT_EPILOGUE);
                 break;
             }
+            __syncwarp();
             tc_fence_after();
             const int c0 = ctx.grp * 32, c1 = c0 + TT_GROUPS * 32;
             const uint32_t tbase =
@@ -401,11 +377,8 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
             __syncwarp();
             if (lane == 0)
                 mbar_arrive_cluster_relaxed(tempty_lead + static_cast<uint32_t>(acc * sizeof(uint64_t)));
-            if (c0 < j.nn) p.chunk(epi, j, ctx, c0, ra);
-            __syncwarp();  // the staged stores are warp-wide
-            if (c1 < j.nn) p.chunk(epi, j, ctx, c1, rb);
+            p.tile(epi, j, ctx, ra, rb);
             __syncwarp();
-            p.end(epi, j, ctx);
         }
         p.finish(ctx);
     }

@@ -10,7 +10,8 @@
 // Forward: one pass over the rows.  The sum is taken in base 2 around a running
 // maximum in the epilogue of each 256 x 256 tile, c = scale log2 e,
 //   m = max_n c <q, x_n>,   z = sum_n 2^(c <q, x_n> - m),
-// held in fp32, one (m, z) per query and row split, joined by xent_join_kernel.  The target's own term stays out of the running sum: with
+// held in fp32, one (m, z) per query, row split and epilogue group, joined by
+// xent_join_kernel.  The target's own term stays out of the running sum: with
 // r = the sum of the other terms relative to the target's, loss = log1p(r), so
 // a query that finds its row keeps a loss near 0, and its p - 1 = expm1(-loss),
 // to full precision.
@@ -109,7 +110,7 @@ struct FwdArgs {
     int nkb, nseg;
     float c;
     const int64_t* targets;
-    float2* part;        // [slots][nq] (max <q, x>, z) of each split
+    float2* part;        // [slots * TT_GROUPS][nq] (max <q, x>, z) of each split and epilogue group
     float* tdot;         // [nq] <q, x_t>
 };
 
@@ -163,12 +164,9 @@ struct FwdPolicy {
         e.tgt = b < a.nq ? a.targets[b] - a.row0 : -1;
     }
 
-    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
-                                          const uint32_t (&r)[32]) const {
-        if (j.m0 + c.row - c.lane >= a.nq) return;  // no query in this warp's 32 rows
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    // 32 columns from column col on: columns behind the last row count as -inf,
+    // and so does the target's, which is kept apart
+    __device__ __forceinline__ void mask(const Epi& e, const Job& j, const TileCtx& c, int col, float (&v)[32]) const {
         const int64_t c0 = static_cast<int64_t>(j.n0) + col;
         if (c0 + 32 > a.n) {
 #pragma unroll
@@ -177,28 +175,24 @@ struct FwdPolicy {
         }
         const int64_t rel = e.tgt - c0;
         if (rel >= 0 && rel < 32 && e.tgt < a.n) {
-            // the target's own term is kept apart
             a.tdot[j.m0 + c.row] = pick32(v, static_cast<int>(rel));
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 v[i] = i == static_cast<int>(rel) ? -INFINITY : v[i];
         }
+    }
+    static __device__ __forceinline__ float largest(const float (&v)[32]) {
         float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
 #pragma unroll
         for (int i = 6; i < 30; i += 4) {
             m0 = max3(m0, v[i], v[i + 1]);
             m1 = max3(m1, v[i + 2], v[i + 3]);
         }
-        m0 = max3(m0, v[30], v[31]);
-        m0 = fmaxf(m0, m1);
-        if (m0 > e.m) {
-            e.z *= ex2((e.m - m0) * a.c);  // 0 before the first finite value
-            e.m = m0;
-            e.mb = m0 * a.c;
-        }
-        // two columns per instruction
-        const uint64_t c2 = pack2(a.c, a.c), b2 = pack2(-e.mb, -e.mb);
-        uint64_t s0 = 0, s1 = 0;
+        return fmaxf(max3(m0, v[30], v[31]), m1);
+    }
+    // sums of 2^(c v - c m), two columns per instruction
+    static __device__ __forceinline__ void add_terms(const float (&v)[32], uint64_t c2, uint64_t b2, uint64_t& s0,
+                                                     uint64_t& s1) {
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
             float x0, x1, x2, x3;
@@ -207,27 +201,36 @@ struct FwdPolicy {
             s0 = add_f32x2(s0, pack2(ex2(x0), ex2(x1)));
             s1 = add_f32x2(s1, pack2(ex2(x2), ex2(x3)));
         }
+    }
+
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
+                                          const uint32_t (&r)[32]) const {
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        mask(e, j, c, col, v);
+        const float mx = largest(v);
+        if (mx > e.m) {
+            e.z *= ex2((e.m - mx) * a.c);  // 0 before the first finite value
+            e.m = mx;
+            e.mb = mx * a.c;
+        }
+        const uint64_t c2 = pack2(a.c, a.c), b2 = pack2(-e.mb, -e.mb);
+        uint64_t s0 = 0, s1 = 0;
+        add_terms(v, c2, b2, s0, s1);
         float p0, p1;
         unpack2(add_f32x2(s0, s1), p0, p1);
         e.z += p0 + p1;
     }
 
-    __device__ __forceinline__ void end(Epi& e, const Job& j, const TileCtx& c) const {
-        if (!j.last) return;
-        // the four warps of a row join through shared memory
-        float2* sh = reinterpret_cast<float2*>(c.stg - c.grp * 4 * TT_STG_BYTES);  // the first group's staging bytes
-        if (c.grp > 0) sh[c.grp * 32 + c.lane] = make_float2(e.m, e.z);
-        tt_quad_sync(c.quad);
+    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
+                                         const uint32_t (&rb)[32]) const {
+        if (j.m0 + c.row - c.lane >= a.nq) return;  // no query in this warp's 32 rows
+        chunk(e, j, c, c.grp * 32, ra);
+        chunk(e, j, c, 128 + c.grp * 32, rb);
         const int64_t b = j.m0 + c.row;
-        if (c.grp == 0) {
-#pragma unroll
-            for (int g = 1; g < TT_GROUPS; ++g) {
-                const float2 o = sh[g * 32 + c.lane];
-                join(e.m, e.z, o.x, o.y, a.c);
-            }
-            if (b < a.nq) a.part[static_cast<int64_t>(a.slot0 + j.split) * a.nq + b] = make_float2(e.m, e.z);
-        }
-        tt_quad_sync(c.quad);  // read before the next unit writes
+        if (j.last && b < a.nq)
+            a.part[(static_cast<int64_t>(a.slot0 + j.split) * TT_GROUPS + c.grp) * a.nq + b] = make_float2(e.m, e.z);
     }
     __device__ __forceinline__ void finish(const TileCtx&) const {}
 };
@@ -242,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
 
 // Joins the parts of 32 queries per block; stats and loss of each query.  An
 // ignored query has loss 0; one whose target is no row is NaN throughout.
-constexpr int JG = 16;  // threads per query
+constexpr int JG = 32;  // threads per query
 __global__ void __launch_bounds__(32 * JG)
     xent_join_kernel(const float2* part, int slots, const float* tdot, const int64_t* targets, int64_t ignore,
                      int64_t n, float c, int64_t nq, float* stats, float* loss) {
@@ -489,7 +492,12 @@ struct ProbPolicy {
         }
     }
 
-    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
+    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
+                                         const uint32_t (&rb)[32]) const {
+        if (c.grp * 32 < j.nn) chunk(e, j, c, c.grp * 32, ra);
+        __syncwarp();
+        if (128 + c.grp * 32 < j.nn) chunk(e, j, c, 128 + c.grp * 32, rb);
+    }
     __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
 
@@ -617,7 +625,12 @@ struct GradPolicy {
             stg_send<false>(mpart, c.stg, c.lane, x, y, j.split);
     }
 
-    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
+    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
+                                         const uint32_t (&rb)[32]) const {
+        if (c.grp * 32 < j.nn) chunk(e, j, c, c.grp * 32, ra);
+        __syncwarp();
+        if (128 + c.grp * 32 < j.nn) chunk(e, j, c, 128 + c.grp * 32, rb);
+    }
     __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
 
@@ -748,7 +761,7 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
     const int64_t dp = up(d, 8);
     w.loss_q = a.take<float>(nq);
     w.tdot = a.take<float>(nq);
-    w.part = a.take<float2>((size_t)p.slots * nq);
+    w.part = a.take<float2>((size_t)TT_GROUPS * p.slots * nq);
     if (dtype == RDB_F32) {
         w.qp = a.take<__nv_bfloat16>(3 * nq * dp);
         w.xp = a.take<__nv_bfloat16>(3 * p.rows * dp);
@@ -1010,7 +1023,7 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
                 mq, mx, a, dtype != RDB_F16, st);
             RDB_LAUNCH_CHECK();
         }
-        xent_join_kernel<<<(unsigned)((nq + 31) / 32), 32 * JG, 0, s>>>(w.part, p.slots, w.tdot, targets, ignore_index,
+        xent_join_kernel<<<(unsigned)((nq + 31) / 32), 32 * JG, 0, s>>>(w.part, TT_GROUPS * p.slots, w.tdot, targets, ignore_index,
                                                                    n, c, nq, stats, loss_q);
         RDB_LAUNCH_CHECK();
     }
