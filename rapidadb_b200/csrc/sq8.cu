@@ -46,22 +46,35 @@ __global__ void sq8_encode_kernel(int dtype, const void* x, int64_t n, int64_t l
     if (lane == 0) scales[row] = scale;
 }
 
-// rint(x / scale) of the division's fp32 result, without the division: r = x *
-// (1 / scale) is within 127 * 2^-22 < 2^-15 of it (two roundings of 2^-24
-// relative each, and its own), so both round to the same integer unless r lies
-// within 2^-14 of a half.  Those (one in 10^4), and NaN and infinities, divide.
-__device__ __forceinline__ float code_of(float x, float scale, float inv, bool& near_half) {
-    const float r = x * inv, c = rintf(r);
-    near_half |= !(fabsf(fabsf(r - c) - 0.5f) > 6.103515625e-05f);
-    return c;
+// Codes without divisions or conversions.  kRound = 1.5 * 2^23: adding it rounds
+// to the nearest integer (ties to even) and leaves that integer, modulo 256, in
+// the sum's low byte.  t = x * (1 / scale) + kRound (one rounding) gives
+// rint(x / scale) unless x / scale lies next to a half: 1 / scale is off by
+// 2^-24 of itself and the quotient by its own rounding, at most 127 * 2^-23 <
+// 2^-16 together, so wherever the distance to the integer is below 1/2 - 2^-14
+// the two agree.  The others (one in 10^4), NaN, and whole rows with a subnormal
+// or infinite scale go through the division and the clamp.
+constexpr float kRound = 12582912.f, kNearHalf = 0.5f - 6.103515625e-05f;
+
+__device__ __forceinline__ uint32_t slow_code(float x, float scale) {
+    const float c = scale > 0.f ? rintf(__fdiv_rn(x, scale)) : 0.f;
+    return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(c, -127.f), 127.f)));
 }
 
-__device__ __forceinline__ uint32_t pack_codes(const float* c) {
-    uint32_t w = 0;
+// four codes in one word
+__device__ __forceinline__ uint32_t codes4(const float* x, float scale, float inv, bool fast) {
+    uint32_t t[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w |= (static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(c[i], -127.f), 127.f))) & 0xffu) << (8 * i);
-    return w;
+    for (int i = 0; i < 4; ++i) {
+        const float s = fmaf(x[i], inv, kRound);
+        fast &= fabsf(fmaf(x[i], inv, kRound - s)) < kNearHalf;
+        t[i] = __float_as_uint(s);
+    }
+    if (!fast) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = slow_code(x[i], scale);
+    }
+    return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
 template <typename T>
@@ -105,22 +118,16 @@ __global__ void __launch_bounds__(256)
     // amax >= 0: its bits order like integers
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     const float scale = __fdiv_rn(amax, 127.f), inv = __fdiv_rn(1.f, scale);
+    const bool fast = scale >= 1.17549435e-38f && scale < INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         if (u * 32 + lane >= units) continue;
-        float c[E];
-        bool near_half = false;
-#pragma unroll
-        for (int i = 0; i < E; ++i) c[i] = code_of(v[u][i], scale, inv, near_half);
-        if (near_half) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) c[i] = scale > 0.f ? rintf(__fdiv_rn(v[u][i], scale)) : 0.f;
-        }
         int8_t* o = codes + row * ldc + (u * 32 + lane) * E;
         if constexpr (E == 8)
-            *reinterpret_cast<uint2*>(o) = make_uint2(pack_codes(c), pack_codes(c + 4));
+            *reinterpret_cast<uint2*>(o) =
+                make_uint2(codes4(v[u], scale, inv, fast), codes4(v[u] + 4, scale, inv, fast));
         else
-            *reinterpret_cast<uint32_t*>(o) = pack_codes(c);
+            *reinterpret_cast<uint32_t*>(o) = codes4(v[u], scale, inv, fast);
     }
     // columns behind d are zero
     for (int64_t t = (int64_t)units * E + lane; t < ldc; t += 32) codes[row * ldc + t] = 0;

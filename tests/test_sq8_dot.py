@@ -103,6 +103,36 @@ def test_encode_equals_definition(device, n, d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_encode_next_to_halves(device, dtype):
+    """Quotients at and next to k + 1/2, subnormal scales, infinities and NaN:
+    the codes of the division's definition."""
+    k = torch.arange(-127, 127, dtype=torch.float32) + 0.5
+    rows = []
+    for s in (1.0, 0.37, 2.0 ** -20, 3e-5, 7.0):
+        base = torch.cat([k * s, torch.nextafter(k * s, torch.tensor(1e9)), torch.nextafter(k * s, torch.tensor(-1e9)),
+                          torch.tensor([127.0 * s] * 6)])
+        rows.append(base)
+    x = torch.stack(rows).to(dtype)
+    extra = x.clone()
+    extra[0, 5], extra[1, 700], extra[2, 0] = float("inf"), float("nan"), -float("inf")
+    tiny = (x[:2].float() * 2.0 ** -139).to(dtype)  # subnormal rows (zero rows in fp16)
+    x = torch.cat([x, extra, tiny])
+    assert x.shape[1] % 8 == 0
+    for v in (x, x[:, :-3]):
+        codes, scales = _C().sq8_encode(v.to(device))
+        xf = v.float().numpy()
+        amax = np.fmax.reduce(np.abs(xf), axis=1)
+        sc = (amax / np.float32(127)).astype(np.float32)
+        with np.errstate(all="ignore"):
+            c = np.rint(xf / sc[:, None])
+        c = np.where(np.isnan(c), -127, np.clip(c, -127, 127))  # a NaN quotient has the lowest code
+        c = np.where(sc[:, None] > 0, c, 0).astype(np.int8)
+        assert np.array_equal(scales.cpu().numpy(), sc)
+        assert np.array_equal(codes.cpu().numpy(), c)
+
+
+@pytest.mark.gpu
 def test_encode_strided_rows(device):
     """Columns of a wider matrix, a transposed matrix, and an odd base offset."""
     x = torch.randn(40, 301, device=device)
