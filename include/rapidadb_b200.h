@@ -99,9 +99,10 @@ int rdb_row_sqnorms(int dtype, const void* x, int64_t n, int d, float* out, void
  * holds (NaN included) reaches nothing.
  *   reduction  RDB_REDUCE_NONE: loss [nq]; _MEAN (over the queries that are
  *              not ignored; NaN when all are) / _SUM: loss [1].
- *   stats      [3, nq] fp32, saved for the backward pass: row 0 the largest
- *              logit m, row 1 log2 sum 2^(s' - m), both of s' = s log2 e;
- *              log sum exp = ln 2 (row 0 + row 1); row 2 the query's loss.
+ *   stats      [3 nq + 1] fp32, saved for the backward pass: nq largest
+ *              logits m and nq log2 sum 2^(s' - m), both of s' = s log2 e
+ *              (log sum exp = ln 2 (first + second)), nq losses, and for a
+ *              reduced loss the number of queries that count.
  *   grad       of the loss: [nq] or [1] as the loss, fp32.
  *   dq / dx    gradients in `dtype` (NULL: not wanted); sums over queries and
  *              rows run in fp32 in a fixed order. */
@@ -177,6 +178,12 @@ int rdb_sq8_encode(int dtype, const void* x, int64_t n, int64_t ldx, int d, int8
                    void* stream);
 int rdb_sq8_row_values(int metric, const int8_t* codes, const float* scales, int64_t n, int64_t ldc, int d,
                        float* out, void* stream);
+/* Copy of rows to a 16-byte stride (the layout the kernels read in place):
+ * row_bytes of each of `rows` rows, src_stride bytes apart (any alignment the
+ * elements have), to dst_stride (a multiple of 16) apart, zero behind them. */
+int rdb_pad_rows(const void* src, int64_t rows, int64_t row_bytes, int64_t src_stride, void* dst, int64_t dst_stride,
+                 void* stream);
+
 /* Scores of int8 codes (no reference counterpart; the int8 form of
  * dot_product_cuda, csrc/kernels/distance.cu:566-610):
  *   out[b, n] = (qs[b] * xs[n]) * sum_t qc[b, t] * xc[n, t]

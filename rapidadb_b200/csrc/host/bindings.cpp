@@ -47,7 +47,11 @@ PYBIND11_MODULE(_C, m) {
           "Dot product matrix [Q, N] of int8 codes with a scale per query and per row", py::arg("query_codes"),
           py::arg("query_scales"), py::arg("codes"), py::arg("scales"), py::arg("dtype") = at::kFloat,
           py::call_guard<py::gil_scoped_release>());
-    // ---- training: rapidadb_b200.losses wraps these for autograd
+    // ---- training: the loss rapidadb_b200.losses offers, and the calls behind it
+    m.def("softmax_cross_entropy_loss", &softmax_cross_entropy_loss,
+          "softmax cross entropy of queries against every database row, differentiable", py::arg("queries"),
+          py::arg("database"), py::arg("targets"), py::arg("scale") = 1.0, py::arg("ignore_index") = -100,
+          py::arg("reduction") = RDB_REDUCE_MEAN, py::call_guard<py::gil_scoped_release>());
     m.def("softmax_cross_entropy", &softmax_cross_entropy,
           "softmax cross entropy of queries against every database row: (loss, stats)", py::arg("queries"),
           py::arg("database"), py::arg("targets"), py::arg("scale") = 1.0, py::arg("ignore_index") = -100,

@@ -48,8 +48,11 @@ Result sq8_encode(const at::Tensor& vectors);
 // [nq, n] scores of int8 codes, one scale per query and per row (rdb_sq8_dot)
 at::Tensor sq8_dot_product(const at::Tensor& query_codes, const at::Tensor& query_scales, const at::Tensor& codes,
                            const at::Tensor& scales, at::ScalarType dtype);
-// softmax cross entropy of queries against every database row: (loss, stats),
-// and (dq, dx) (rdb_softmax_xent, rdb_softmax_xent_backward)
+// softmax cross entropy of queries against every database row: the loss with
+// its autograd node, and the two calls behind it, (loss, stats) and (dq, dx)
+// (rdb_softmax_xent, rdb_softmax_xent_backward)
+at::Tensor softmax_cross_entropy_loss(const at::Tensor& queries, const at::Tensor& database, const at::Tensor& targets,
+                                      double scale, int64_t ignore_index, int reduction);
 Result softmax_cross_entropy(const at::Tensor& queries, const at::Tensor& database, const at::Tensor& targets,
                              double scale, int64_t ignore_index, int reduction);
 Result softmax_cross_entropy_backward(const at::Tensor& grad, const at::Tensor& queries, const at::Tensor& database,

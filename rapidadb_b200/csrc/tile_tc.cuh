@@ -369,8 +369,9 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
             const uint32_t tbase =
                 tmem_base + (static_cast<uint32_t>(ctx.quad * 32) << 16) + static_cast<uint32_t>(acc * TT_N);
             uint32_t ra[32], rb[32];
-            if (c0 < j.nn) tmem_ld32_async(tbase + static_cast<uint32_t>(c0), ra);
-            if (c1 < j.nn) tmem_ld32_async(tbase + static_cast<uint32_t>(c1), rb);
+            // (columns behind a narrow tile hold older values, which no policy uses)
+            tmem_ld32_async(tbase + static_cast<uint32_t>(c0), ra);
+            tmem_ld32_async(tbase + static_cast<uint32_t>(c1), rb);
             tmem_ld_wait(ra);
             tmem_ld_wait(rb);
             tc_fence_before();

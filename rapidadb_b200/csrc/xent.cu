@@ -26,13 +26,14 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "tile_tc.cuh"
 
 namespace rdb {
 namespace {
 
-constexpr int NT = 256, NW = NT / 32;
+constexpr int NT = 256;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr double kLog2e = 1.4426950408889634;
 // G is held as 2^14 (p - [n = t]): the largest value is 2^14, and an fp16
@@ -93,20 +94,13 @@ __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// v = hi + mid + lo, each bf16: what the first two leave is exact in fp32
-__device__ __forceinline__ void split3(float v, float (&o)[3]) {
-    o[0] = __bfloat162float(__float2bfloat16_rn(v));
-    const float r = v - o[0];
-    o[1] = __bfloat162float(__float2bfloat16_rn(r));
-    o[2] = r - o[1];
-}
-
 // ---------------------------------------------------------------- forward --
 
 struct FwdArgs {
     int64_t nq, n;       // queries, rows of this piece
     int64_t row0;        // first row of the piece in the base
-    int nqb, ntiles, nsplit, slot0;
+    int nqb, nsplit, slot0;
+    int n32;             // 32-row groups of the piece, dealt evenly to the splits
     int nkb, nseg;
     float c;
     const int64_t* targets;
@@ -123,31 +117,33 @@ struct FwdPolicy {
         int split;
         bool first, last;
     };
+    // units of (query block, row split), query blocks first, so that the pairs
+    // in flight read the same rows
     struct Iter {
         const FwdPolicy& p;
-        int unit, step, t, hi, lo;
-        __device__ Iter(const FwdPolicy& pol, int pair, int npairs) : p(pol), unit(pair - npairs), step(npairs), t(0), hi(0), lo(0) {}
+        int unit, step, lo, at, hi;  // 32-row groups
+        __device__ Iter(const FwdPolicy& pol, int pair, int npairs) : p(pol), unit(pair - npairs), step(npairs), lo(0), at(0), hi(0) {}
         __device__ __forceinline__ bool next(Job& j) {
-            if (t == hi) {
+            if (at >= hi) {
                 unit += step;
                 if (unit >= p.a.nqb * p.a.nsplit) return false;
                 const int64_t sp = unit / p.a.nqb;
-                lo = t = static_cast<int>(sp * p.a.ntiles / p.a.nsplit);
-                hi = static_cast<int>((sp + 1) * p.a.ntiles / p.a.nsplit);
+                lo = at = static_cast<int>(sp * p.a.n32 / p.a.nsplit);
+                hi = static_cast<int>((sp + 1) * p.a.n32 / p.a.nsplit);
             }
             j.ma = p.mq;
             j.mb = p.mx;
             j.m0 = unit % p.a.nqb * TT_M;
-            j.n0 = t * TT_N;
-            j.nn = TT_N;
+            j.n0 = at * 32;
+            j.nn = min(TT_N, (hi - at) * 32);
             j.k0 = 0;
             j.nk = p.a.nkb;
             j.nseg = p.a.nseg;
             j.a_mn = j.b_mn = false;
             j.split = unit / p.a.nqb;
-            j.first = t == lo;
-            j.last = t == hi - 1;
-            ++t;
+            j.first = at == lo;
+            at += TT_N / 32;
+            j.last = at >= hi;
             return true;
         }
     };
@@ -226,8 +222,8 @@ struct FwdPolicy {
     __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
                                          const uint32_t (&rb)[32]) const {
         if (j.m0 + c.row - c.lane >= a.nq) return;  // no query in this warp's 32 rows
-        chunk(e, j, c, c.grp * 32, ra);
-        chunk(e, j, c, 128 + c.grp * 32, rb);
+        if (c.grp * 32 < j.nn) chunk(e, j, c, c.grp * 32, ra);
+        if (128 + c.grp * 32 < j.nn) chunk(e, j, c, 128 + c.grp * 32, rb);
         const int64_t b = j.m0 + c.row;
         if (j.last && b < a.nq)
             a.part[(static_cast<int64_t>(a.slot0 + j.split) * TT_GROUPS + c.grp) * a.nq + b] = make_float2(e.m, e.z);
@@ -243,60 +239,82 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     tile_loop(smem_raw, p, bf16, st);
 }
 
-// Joins the parts of 32 queries per block; stats and loss of each query.  An
-// ignored query has loss 0; one whose target is no row is NaN throughout.
 constexpr int JG = 32;  // threads per query
+// Joins the parts of 32 queries per block and step; stats and loss of each
+// query.  An ignored query has loss 0; one whose target is no row is NaN
+// throughout.  A single block also reduces the losses (total; the queries that
+// count behind the stats).
 __global__ void __launch_bounds__(32 * JG)
     xent_join_kernel(const float2* part, int slots, const float* tdot, const int64_t* targets, int64_t ignore,
-                     int64_t n, float c, int64_t nq, float* stats, float* loss) {
-    __shared__ float2 sh[JG][32];
+                     int64_t n, float c, int64_t nq, float* stats, float* loss, int reduction, float* total) {
+    __shared__ float2 sh[JG][33];
     const int qi = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int64_t b = static_cast<int64_t>(blockIdx.x) * 32 + qi;
-    float M = -INFINITY, Z = 0.f;
-    if (b < nq)
-        for (int s = g; s < slots; s += JG) {
-            const float2 v = part[static_cast<int64_t>(s) * nq + b];
-            join(M, Z, v.x, v.y, c);
+    float lsum = 0.f;
+    int count = 0;
+    for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * 32; b0 < nq; b0 += static_cast<int64_t>(gridDim.x) * 32) {
+        const int64_t b = b0 + qi;
+        float M = -INFINITY, Z = 0.f;
+        if (b < nq)
+#pragma unroll 4
+            for (int s = g; s < slots; s += JG) {
+                const float2 v = part[static_cast<int64_t>(s) * nq + b];
+                join(M, Z, v.x, v.y, c);
+            }
+        sh[g][qi] = make_float2(M, Z);
+        __syncthreads();
+        if (g == 0 && b < nq) {
+            const int used = min(JG, slots);
+            for (int k = 1; k < used; ++k) join(M, Z, sh[k][qi].x, sh[k][qi].y, c);
+            const int64_t t = targets[b];
+            const bool ignored = t == ignore, has = t >= 0 && t < n;
+            const float nan = __int_as_float(0x7fc00000);
+            // Z sums 2^(c v - c M); u: the target's exponent relative to that
+            const float Mc = M > -INFINITY ? M * c : 0.f;
+            const float td = has ? tdot[b] : -INFINITY;
+            const float u = fmaf(td, c, -Mc);
+            float m = Mc, lz, l;
+            if (u >= 0.f || (has && !(M > -INFINITY))) {
+                // the target is the largest (or the only) term
+                m = td * c;
+                const float rest = M > -INFINITY ? Z * ex2(-u) : 0.f * Z;
+                l = isfinite(td) ? log1pf(rest) : nan;
+                lz = log2f(rest + ex2(fmaf(td, c, -m)));
+            } else {
+                lz = log2f(Z + (has ? ex2(u) : 0.f));
+                l = kLn2 * (lz - u);
+            }
+            if (ignored) l = 0.f;
+            else if (!has) l = lz = nan;
+            stats[b] = m;
+            stats[nq + b] = lz;
+            stats[2 * nq + b] = l;
+            if (loss) loss[b] = l;
+            lsum += l;
+            count += !ignored;
         }
-    sh[g][qi] = make_float2(M, Z);
-    __syncthreads();
-    if (g != 0 || b >= nq) return;
-    for (int k = 1; k < JG; ++k) join(M, Z, sh[k][qi].x, sh[k][qi].y, c);
-    const int64_t t = targets[b];
-    const bool ignored = t == ignore, has = t >= 0 && t < n;
-    const float nan = __int_as_float(0x7fc00000);
-    // Z sums 2^(c v - c M); u: the target's exponent relative to that
-    const float Mc = M > -INFINITY ? M * c : 0.f;
-    const float td = has ? tdot[b] : -INFINITY;
-    const float u = fmaf(td, c, -Mc);
-    float m = Mc, lz, l;
-    if (u >= 0.f || (has && !(M > -INFINITY))) {
-        // the target is the largest (or the only) term
-        m = td * c;
-        const float rest = M > -INFINITY ? Z * ex2(-u) : 0.f * Z;
-        l = isfinite(td) ? log1pf(rest) : nan;
-        lz = log2f(rest + ex2(fmaf(td, c, -m)));
-    } else {
-        lz = log2f(Z + (has ? ex2(u) : 0.f));
-        l = kLn2 * (lz - u);
+        __syncthreads();
     }
-    if (ignored) l = 0.f;
-    else if (!has) l = lz = nan;
-    stats[b] = m;
-    stats[nq + b] = lz;
-    stats[2 * nq + b] = l;
-    if (loss) loss[b] = l;
+    if (reduction == RDB_REDUCE_NONE && blockIdx.x == 0 && threadIdx.x == 0) stats[3 * nq] = 0.f;
+    if (total && g == 0) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+        count = __reduce_add_sync(0xffffffffu, count);
+        if (qi == 0) {
+            *total = reduction == RDB_REDUCE_MEAN ? lsum / static_cast<float>(count) : lsum;
+            stats[3 * nq] = static_cast<float>(count);
+        }
+    }
 }
 
-// mean or sum of the losses of the queries that are not ignored
+// mean or sum of the losses of the queries that are not ignored, and their count
 __global__ void __launch_bounds__(1024)
-    xent_reduce_kernel(const float* loss_q, const int64_t* targets, int64_t ignore, int64_t nq, int mean, float* loss) {
+    xent_reduce_kernel(const int64_t* targets, int64_t ignore, int64_t nq, int reduction, float* stats, float* total) {
     __shared__ float ss[32];
     __shared__ int sc[32];
     float s = 0.f;
     int cnt = 0;
     for (int64_t i = threadIdx.x; i < nq; i += blockDim.x)
-        if (targets[i] != ignore) s += loss_q[i], ++cnt;
+        if (targets[i] != ignore) s += stats[2 * nq + i], ++cnt;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     cnt = __reduce_add_sync(0xffffffffu, cnt);
@@ -304,37 +322,30 @@ __global__ void __launch_bounds__(1024)
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 32; ++w) ss[0] += ss[w], sc[0] += sc[w];
-        *loss = mean ? ss[0] / static_cast<float>(sc[0]) : ss[0];
+        *total = reduction == RDB_REDUCE_MEAN ? ss[0] / static_cast<float>(sc[0]) : ss[0];
+        stats[3 * nq] = static_cast<float>(sc[0]);
     }
 }
 
 // --------------------------------------------------------------- backward --
 
-// w_b = the incoming gradient of the query's loss (divided by the queries that
-// count for the mean), 0 for an ignored one; wmax = max |w_b|
+// The weight w_b of a query's loss: g[b], or for a reduced loss g[0], over the
+// number of queries for the mean (0 when none count).
+struct Weight {
+    const float* g;
+    const float* count;  // nullptr: not a mean
+    __device__ __forceinline__ float all() const {
+        return count ? (*count > 0.f ? *g / *count : 0.f) : *g;
+    }
+};
+
+// largest |g_b| of the queries that count (reduction none)
 __global__ void __launch_bounds__(1024)
-    xent_weights_kernel(const float* grad, const int64_t* targets, int64_t ignore, int64_t nq, int reduction, float* w,
-                        float* wmax) {
-    __shared__ int sc[32];
+    xent_wmax_kernel(const float* grad, const int64_t* targets, int64_t ignore, int64_t nq, float* wmax) {
     __shared__ float sm[32];
-    int cnt = 0;
-    if (reduction == RDB_REDUCE_MEAN) {
-        for (int64_t i = threadIdx.x; i < nq; i += blockDim.x) cnt += targets[i] != ignore;
-        cnt = __reduce_add_sync(0xffffffffu, cnt);
-        if ((threadIdx.x & 31) == 0) sc[threadIdx.x >> 5] = cnt;
-        __syncthreads();
-        cnt = __reduce_add_sync(0xffffffffu, sc[threadIdx.x & 31]);
-    }
     float mx = 0.f;
-    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x) {
-        float g = 0.f;
-        if (targets[i] != ignore) {
-            g = grad[reduction == RDB_REDUCE_NONE ? i : 0];
-            if (reduction == RDB_REDUCE_MEAN) g /= static_cast<float>(cnt);
-        }
-        w[i] = g;
-        mx = fmaxf(mx, fabsf(g));  // a NaN weight makes its own products NaN
-    }
+    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x)
+        if (targets[i] != ignore) mx = fmaxf(mx, fabsf(grad[i]));  // a NaN weight makes its own products NaN
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mx;
@@ -345,48 +356,96 @@ __global__ void __launch_bounds__(1024)
     }
 }
 
-// Queries weighted for dx = G^T (w q): out[b] = q[b] w_b / wmax, so that the
-// type's range is used whatever the size of the gradients (equal weights: the
-// query itself, unrounded); zero rows for ignored queries, whatever they hold.
-// fp32: three bf16 planes.
+// 8 elements of a row from column t on as floats; what lies behind d is neither
+// read nor kept
 template <typename T>
-__global__ void __launch_bounds__(NT)
-    xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const int64_t* targets, int64_t ignore,
-                         const float* w, const float* wmax, void* out, int64_t ldo) {
-    const int64_t b = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 5);
-    if (b >= nq) return;
-    const bool skip = targets[b] == ignore;
-    const float f = skip || w[b] == 0.f ? 0.f : w[b] / *wmax;
-    for (int t = threadIdx.x & 31; t < d; t += 32) {
-        const float v = skip ? 0.f : to_f(q[b * ldq + t]) * f;
+__device__ __forceinline__ void load8(const T* row, int t, int d, float (&v)[8]) {
+    if (t + 8 <= d) {
         if constexpr (sizeof(T) == 4) {
-            float o[3];
-            split3(v, o);
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-                static_cast<__nv_bfloat16*>(out)[(k * nq + b) * ldo + t] = __float2bfloat16_rn(o[k]);
+            const float4 a = *reinterpret_cast<const float4*>(row + t), b = *reinterpret_cast<const float4*>(row + t + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
         } else {
-            static_cast<T*>(out)[b * ldo + t] = from_f<T>(v);
+            const uint4 u = *reinterpret_cast<const uint4*>(row + t);
+            const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = t + i < d ? to_f(row[t + i]) : 0.f;
     }
 }
 
-// fp32 rows -> three bf16 planes [3][n][ldo]
+// the three bf16 planes of 8 floats, plane stride in elements
+__device__ __forceinline__ void store_planes(const float (&v)[8], __nv_bfloat16* o, int64_t plane) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = v[i];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        uint32_t w[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            w[h] = pack16<__nv_bfloat16>(r[2 * h], r[2 * h + 1]);
+            // what is left for the next plane: exact in fp32
+            r[2 * h] -= __uint_as_float(w[h] << 16);
+            r[2 * h + 1] -= __uint_as_float(w[h] & 0xffff0000u);
+        }
+        *reinterpret_cast<uint4*>(o + k * plane) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Queries weighted for dx = G^T (w q): out[b] = q[b] w_b / max |w|, so that the
+// type's range is used whatever the size of the gradients (equal weights: the
+// query itself, unrounded); zero rows for ignored queries, whatever they hold.
+// fp32: three bf16 planes.  grad: nullptr for equal weights.
+template <typename T>
+__global__ void __launch_bounds__(NT)
+    xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const int64_t* targets, int64_t ignore,
+                         const float* grad, const float* wmax, void* out, int64_t ldo) {
+    const int64_t units = ldo / 8, total = nq * units;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * NT) {
+        const int64_t b = i / units;
+        const int t = static_cast<int>(i - b * units) * 8;
+        float v[8];
+        if (targets[b] == ignore) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        } else {
+            load8(q + b * ldq, t, d, v);
+            if (grad) {
+                const float f = grad[b] == 0.f ? 0.f : grad[b] / *wmax;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] *= f;
+            }
+        }
+        if constexpr (sizeof(T) == 4)
+            store_planes(v, static_cast<__nv_bfloat16*>(out) + b * ldo + t, nq * ldo);
+        else
+            *reinterpret_cast<uint4*>(static_cast<T*>(out) + b * ldo + t) =
+                make_uint4(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]), pack16<T>(v[6], v[7]));
+    }
+}
+
+// fp32 rows -> three bf16 planes [3][n][ldo], ldo a multiple of 8
 __global__ void __launch_bounds__(NT)
     xent_split_kernel(const float* x, int64_t n, int64_t ldx, int d, __nv_bfloat16* out, int64_t ldo) {
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 5);
-    if (r >= n) return;
-    for (int t = threadIdx.x & 31; t < d; t += 32) {
-        float o[3];
-        split3(x[r * ldx + t], o);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) out[(k * n + r) * ldo + t] = __float2bfloat16_rn(o[k]);
+    const int64_t units = ldo / 8, total = n * units;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * NT) {
+        const int64_t r = i / units;
+        const int t = static_cast<int>(i - r * units) * 8;
+        float v[8];
+        load8(x + r * ldx, t, d, v);
+        store_planes(v, out + r * ldo + t, n * ldo);
     }
 }
 
 struct ProbArgs {
     int64_t nq, n, row0;  // queries, rows of the piece, its first row
     int nqb, njobs, nkb, nseg;
+    int width;            // columns of a tile
     float c;
     const int64_t* targets;
     int64_t ignore;
@@ -410,8 +469,8 @@ struct ProbPolicy {
             j.ma = p.mq;
             j.mb = p.mx;
             j.m0 = i % p.a.nqb * TT_M;
-            j.n0 = i / p.a.nqb * TT_N;
-            j.nn = TT_N;
+            j.n0 = i / p.a.nqb * p.a.width;
+            j.nn = p.a.width;
             j.k0 = 0;
             j.nk = p.a.nkb;
             j.nseg = p.a.nseg;
@@ -523,7 +582,7 @@ struct GradArgs {
     int64_t lddx;
     bool dx_tma;           // the rows of dx have 16-byte strides
     float scale;
-    const float* wmax;
+    Weight w;              // what dx has to be multiplied with besides
 };
 
 template <typename T>
@@ -578,7 +637,7 @@ struct GradPolicy {
     };
 
     __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx&) const {
-        e.f = j.is_dx ? a.scale * (1.f / kGScale) * *a.wmax : 1.f;
+        e.f = j.is_dx ? a.scale * (1.f / kGScale) * a.w.all() : 1.f;
     }
 
     __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
@@ -645,18 +704,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     tile_loop(smem_raw, p, bf16, st);
 }
 
-// dq_b = g_b scale 2^-14 (sum of the parts, in split order)
+// dq_b = w_b scale 2^-14 (sum of the parts, in split order)
 template <typename T>
 __global__ void __launch_bounds__(NT)
     xent_dq_kernel(const float* part, int splits, int64_t nq, int d, int dp, const int64_t* targets, int64_t ignore,
-                   const float* w, float scale, T* dq, int64_t lddq) {
-    const int64_t b = blockIdx.x;
-    const float f = w[b] * scale * (1.f / kGScale);
-    const bool skip = targets[b] == ignore;
-    for (int t = threadIdx.x; t < d; t += NT) {
-        float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += part[(k * nq + b) * dp + t];
-        dq[b * lddq + t] = from_f<T>(skip ? 0.f : s * f);
+                   Weight w, bool equal, float scale, T* dq, int64_t lddq) {
+    const int64_t units = dp / 4, total = nq * units;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * NT) {
+        const int64_t b = i / units;
+        const int t = static_cast<int>(i - b * units) * 4;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int k = 0; k < splits; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(part + (k * nq + b) * dp + t);
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        const bool skip = targets[b] == ignore;
+        const float f = (equal ? w.all() : w.g[b]) * scale * (1.f / kGScale);
+        const float o[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (t + k < d) dq[b * lddq + t + k] = from_f<T>(skip ? 0.f : o[k]);
     }
 }
 
@@ -716,16 +785,16 @@ struct FwdPlan {
     int pieces, nqb, nkb, nseg, slots, nsplit[2];  // nsplit of a full and of the last piece
 };
 
-// Tiles of one piece per pair: as many splits as give every pair the same
-// number of tiles; a split costs about a seventh of a tile (its join and the
-// reload of the query's target).
-int fwd_splits(int nqb, int64_t ntiles, int pairs) {
+// Row splits of one piece: as many as give every pair the same number of rows
+// (in groups of 32); a split costs about a third of a tile (its fill and parts).
+int fwd_splits(int nqb, int64_t rows, int pairs) {
+    const int64_t n32 = (rows + 31) / 32;
     int best = 1;
     double best_cost = 1e30;
-    const int64_t most = std::min<int64_t>(ntiles, std::max<int64_t>(1, 16LL * pairs / nqb + 1));
+    const int64_t most = std::min<int64_t>(n32, std::max<int64_t>(1, 16LL * pairs / nqb + 1));
     for (int64_t s = 1; s <= most; ++s) {
-        const double per = (double)((ntiles + s - 1) / s);
-        const double cost = (double)((nqb * s + pairs - 1) / pairs) * (per + 0.15);
+        const double tiles = (double)((n32 + s - 1) / s) / (TT_N / 32);
+        const double cost = (double)((nqb * s + pairs - 1) / pairs) * (tiles + 0.3);
         if (cost < best_cost) best_cost = cost, best = (int)s;
     }
     return best;
@@ -741,15 +810,14 @@ FwdPlan fwd_plan(int dtype, int64_t nq, int64_t n, int d) {
     p.nkb = (d + 63) / 64;
     p.nseg = dtype == RDB_F32 ? 6 : 1;
     const int pairs = tile_pairs();
-    const int64_t last = n - (p.pieces - 1) * p.rows;
-    p.nsplit[0] = fwd_splits(p.nqb, p.rows / TT_N, pairs);
-    p.nsplit[1] = fwd_splits(p.nqb, (last + TT_N - 1) / TT_N, pairs);
+    p.nsplit[0] = fwd_splits(p.nqb, p.rows, pairs);
+    p.nsplit[1] = fwd_splits(p.nqb, n - (p.pieces - 1) * p.rows, pairs);
     p.slots = (p.pieces - 1) * p.nsplit[0] + p.nsplit[1];
     return p;
 }
 
 struct FwdWs {
-    float *loss_q, *tdot;
+    float* tdot;
     float2* part;
     __nv_bfloat16 *qp, *xp;
     size_t bytes;
@@ -759,7 +827,6 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
     FwdWs w{};
     Arena a{static_cast<char*>(base)};
     const int64_t dp = up(d, 8);
-    w.loss_q = a.take<float>(nq);
     w.tdot = a.take<float>(nq);
     w.part = a.take<float2>((size_t)TT_GROUPS * p.slots * nq);
     if (dtype == RDB_F32) {
@@ -822,7 +889,7 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
 }
 
 struct BwdWs {
-    float *w, *wmax, *part;
+    float *wmax, *part;
     void *g, *qw;
     __nv_bfloat16 *qp, *xp;
     size_t bytes;
@@ -832,7 +899,6 @@ BwdWs bwd_ws(void* base, const BwdPlan& p, int dtype, int64_t nq, int d, bool ne
     BwdWs w{};
     Arena a{static_cast<char*>(base)};
     const int64_t d8 = up(d, 8);
-    w.w = a.take<float>(nq);
     w.wmax = a.take<float>(1);
     w.g = a.take<uint16_t>((size_t)p.planes * nq * p.rows);
     if (need_dq) w.part = a.take<float>((size_t)p.q_split * nq * p.dp);
@@ -845,9 +911,27 @@ BwdWs bwd_ws(void* base, const BwdPlan& p, int dtype, int64_t nq, int d, bool ne
     return w;
 }
 
+unsigned elementwise_blocks(int64_t items) {
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + NT - 1) / NT, 8LL * num_sms()));
+}
+
+// tile width of the probability pass: 256, or narrower where that deals the
+// rows of few query blocks out more evenly (a tile costs about 48 columns more
+// than its width)
+int prob_width(int64_t rows, int nqb, int pairs) {
+    int best = TT_N;
+    double best_cost = 1e30;
+    for (int w = TT_N; w >= 64; w /= 2) {
+        const double jobs = (double)((rows + w - 1) / w) * nqb;
+        const double cost = std::ceil(jobs / pairs) * (w + 48);
+        if (cost < 0.97 * best_cost) best_cost = cost, best = w;
+    }
+    return best;
+}
+
 int split_rows(const void* x, int64_t n, int64_t ldx, int d, __nv_bfloat16* out, cudaStream_t s) {
-    xent_split_kernel<<<(unsigned)((n + NW - 1) / NW), NT, 0, s>>>(static_cast<const float*>(x), n, ldx, d, out,
-                                                                   up(d, 8));
+    xent_split_kernel<<<elementwise_blocks(n * up(d, 8) / 8), NT, 0, s>>>(static_cast<const float*>(x), n, ldx, d, out,
+                                                                          up(d, 8));
     RDB_LAUNCH_CHECK();
     return RDB_OK;
 }
@@ -878,11 +962,16 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     RDB_TRY(tile_smem_attr(xent_prob_kernel<T>, attr_p));
     RDB_TRY(tile_smem_attr(xent_grad_kernel<T>, attr_g));
 
-    xent_weights_kernel<<<1, 1024, 0, s>>>(grad, targets, ignore, nq, reduction, w.w, w.wmax);
-    RDB_LAUNCH_CHECK();
+    // equal weights (a reduced loss) are applied to the results
+    const bool equal = reduction != RDB_REDUCE_NONE;
+    const Weight wt{grad, reduction == RDB_REDUCE_MEAN ? stats + 3 * nq : nullptr};
     if (dx) {
-        xent_weighted_kernel<T><<<(unsigned)((nq + NW - 1) / NW), NT, 0, s>>>(static_cast<const T*>(q), nq, ldq, d,
-                                                                              targets, ignore, w.w, w.wmax, w.qw, d8);
+        if (!equal) {
+            xent_wmax_kernel<<<1, 1024, 0, s>>>(grad, targets, ignore, nq, w.wmax);
+            RDB_LAUNCH_CHECK();
+        }
+        xent_weighted_kernel<T><<<elementwise_blocks(nq * d8 / 8), NT, 0, s>>>(
+            static_cast<const T*>(q), nq, ldq, d, targets, ignore, equal ? nullptr : grad, w.wmax, w.qw, d8);
         RDB_LAUNCH_CHECK();
     }
     Planes qo;
@@ -912,7 +1001,7 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     ga.lddx = lddx;
     ga.dx_tma = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (lddx * (int64_t)sizeof(T)) % 16 == 0;
     ga.scale = scale;
-    ga.wmax = w.wmax;
+    ga.w = equal ? wt : Weight{w.wmax, nullptr};
     const Planes go{w.g, p.rows, nq * p.rows, p.planes};
     CUtensorMap mpart = mq, mdx = mq;  // (any valid map where there is nothing to store)
     if (dq)
@@ -932,7 +1021,8 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         RDB_TRY(make_store_map(&mg, map_type(dtype), 2, w.g, rows, nq, p.planes, 2 * p.rows, 2 * p.rows * nq));
         pa.n = rows;
         pa.row0 = r0;
-        const int64_t tiles = (rows + TT_N - 1) / TT_N * p.nqb;
+        pa.width = prob_width(rows, p.nqb, pairs);
+        const int64_t tiles = (rows + pa.width - 1) / pa.width * p.nqb;
         RDB_CHECK_ARG(tiles < (1LL << 31), "too many tiles for one launch");
         pa.njobs = (int)tiles;
         xent_prob_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS, TT_SMEM, s>>>(mq, mx, mg, pa,
@@ -957,8 +1047,9 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         RDB_LAUNCH_CHECK();
     }
     if (dq) {
-        xent_dq_kernel<T><<<(unsigned)nq, NT, 0, s>>>(w.part, p.q_split, nq, d, p.dp, targets, ignore, w.w, scale,
-                                                      static_cast<T*>(dq), lddq);
+        xent_dq_kernel<T><<<elementwise_blocks(nq * p.dp / 4), NT, 0, s>>>(w.part, p.q_split, nq, d, p.dp, targets,
+                                                                           ignore, wt, equal, scale,
+                                                                           static_cast<T*>(dq), lddq);
         RDB_LAUNCH_CHECK();
     }
     return RDB_OK;
@@ -982,13 +1073,12 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
                      const int64_t* targets, float scale, int64_t ignore_index, int reduction, float* loss,
                      float* stats, void* ws, size_t ws_bytes, void* stream) {
     RDB_TRY(check_common(dtype, q, nq, ldq, x, n, ldx, d, targets, scale, reduction));
-    RDB_CHECK_ARG((loss || (nq == 0 && reduction == RDB_REDUCE_NONE)) && (nq == 0 || stats), "NULL pointer");
+    RDB_CHECK_ARG(stats && (loss || (nq == 0 && reduction == RDB_REDUCE_NONE)), "NULL pointer");
     RDB_CHECK_ARG((reinterpret_cast<uintptr_t>(ws) & 15) == 0, "ws must be 16-byte aligned");
     const FwdPlan p = fwd_plan(dtype, nq, n, d);
     const FwdWs w = fwd_ws(ws, p, dtype, nq, d);
     if (!ws || ws_bytes < w.bytes) return set_error(RDB_ERR_WORKSPACE, "workspace too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    float* loss_q = reduction == RDB_REDUCE_NONE ? loss : w.loss_q;
     const float c = (float)(scale * kLog2e);
     if (nq > 0) {
         static bool attr[64] = {false};
@@ -1014,7 +1104,7 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
             RDB_TRY(operand_map(&mx, dtype, xo, d, rows, false));
             a.n = rows;
             a.row0 = r0;
-            a.ntiles = (int)((rows + TT_N - 1) / TT_N);
+            a.n32 = (int)((rows + 31) / 32);
             a.nsplit = p.nsplit[i == p.pieces - 1];
             a.slot0 = i * p.nsplit[0];
             const int64_t units = (int64_t)a.nsplit * p.nqb;
@@ -1023,12 +1113,16 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
                 mq, mx, a, dtype != RDB_F16, st);
             RDB_LAUNCH_CHECK();
         }
-        xent_join_kernel<<<(unsigned)((nq + 31) / 32), 32 * JG, 0, s>>>(w.part, TT_GROUPS * p.slots, w.tdot, targets, ignore_index,
-                                                                   n, c, nq, stats, loss_q);
+        // few parts: one block joins them all and reduces the losses too
+        const bool one = reduction != RDB_REDUCE_NONE && nq <= 512 && nq * p.slots * TT_GROUPS <= 16384;
+        xent_join_kernel<<<one ? 1u : (unsigned)std::min<int64_t>((nq + 31) / 32, 16LL * num_sms()), 32 * JG, 0, s>>>(
+            w.part, TT_GROUPS * p.slots, w.tdot, targets, ignore_index, n, c, nq, stats,
+            reduction == RDB_REDUCE_NONE ? loss : nullptr, reduction, one ? loss : nullptr);
         RDB_LAUNCH_CHECK();
+        if (one) return RDB_OK;
     }
     if (reduction != RDB_REDUCE_NONE) {
-        xent_reduce_kernel<<<1, 1024, 0, s>>>(loss_q, targets, ignore_index, nq, reduction == RDB_REDUCE_MEAN, loss);
+        xent_reduce_kernel<<<1, 1024, 0, s>>>(targets, ignore_index, nq, reduction, stats, loss);
         RDB_LAUNCH_CHECK();
     }
     return RDB_OK;

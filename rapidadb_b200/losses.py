@@ -18,24 +18,6 @@ from rapidadb_b200._lib import C
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-class _SoftmaxCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, queries, database, targets, scale, ignore_index, reduction):
-        loss, stats = C().softmax_cross_entropy(queries, database, targets, scale, ignore_index, reduction)
-        ctx.save_for_backward(queries, database, targets, stats)
-        ctx.call = (scale, ignore_index, reduction)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        queries, database, targets, stats = ctx.saved_tensors
-        dq, dx = C().softmax_cross_entropy_backward(grad, queries, database, targets, stats, *ctx.call,
-                                                    need_queries=ctx.needs_input_grad[0],
-                                                    need_database=ctx.needs_input_grad[1])
-        return dq, dx, None, None, None, None
-
-
 def softmax_cross_entropy(queries: torch.Tensor, database: torch.Tensor, targets: torch.Tensor,
                           scale: float = 1.0, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
     """Softmax cross entropy of ``queries`` against every row of ``database``.
@@ -56,10 +38,10 @@ def softmax_cross_entropy(queries: torch.Tensor, database: torch.Tensor, targets
 
     The loss is float32; gradients have their tensor's dtype.  Gradients are
     computed only for the inputs that require them, in a fixed order of sums
-    (the same inputs give the same bits), and once: there is no second
-    derivative.
+    (the same call gives the same bits), and once: a backward pass with
+    ``create_graph=True`` raises.  To capture a step into a CUDA graph, take the
+    gradients with ``torch.autograd.grad`` of leaves made inside the capture.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
-    return _SoftmaxCrossEntropy.apply(queries, database, targets, float(scale), int(ignore_index),
-                                      _REDUCTIONS[reduction])
+    return C().softmax_cross_entropy_loss(queries, database, targets, scale, ignore_index, _REDUCTIONS[reduction])
