@@ -135,11 +135,13 @@ struct DotArgs {
     int nqt, nxt;  // tiles of 256 queries, of 256 rows
     int nk;
     void* out;
+    int x_rows, q_rows;  // box rows
 };
 
 template <typename T>
 struct DotPolicy {
     static constexpr bool kInt8 = true;
+    static constexpr int kStages = 6, kStgBytes = 256;
     // rows are walked in groups of 8 tiles: the tiles in flight form a block of
     // both operands that L2 holds
     static constexpr int kGroup = 8;
@@ -167,6 +169,9 @@ struct DotPolicy {
             j.nk = a.nk;
             j.nseg = 1;
             j.a_mn = j.b_mn = false;
+            j.a_rows = a.x_rows;
+            j.b_rows = a.q_rows;
+            j.a_second = j.m0 + 128 < a.n;
             i += step;
             return true;
         }
@@ -182,7 +187,7 @@ struct DotPolicy {
         float* qs = reinterpret_cast<float*>(c.stg);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t b = static_cast<int64_t>(j.n0) + h * 128 + c.grp * 32 + c.lane;
+            const int64_t b = static_cast<int64_t>(j.n0) + (h ? c.col1 : c.col0) + c.lane;
             qs[h * 32 + c.lane] = b < a.nq ? a.qs[b] : 0.f;
         }
         __syncwarp();
@@ -196,7 +201,7 @@ struct DotPolicy {
 
     __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int h,
                                           const uint32_t (&r)[32]) const {
-        const int64_t x = static_cast<int64_t>(j.m0) + c.row, b0 = static_cast<int64_t>(j.n0) + h * 128 + c.grp * 32;
+        const int64_t x = static_cast<int64_t>(j.m0) + c.row, b0 = static_cast<int64_t>(j.n0) + (h ? c.col1 : c.col0);
         if (x >= a.n || b0 >= a.nq) return;
         const float4* qs = reinterpret_cast<const float4*>(c.stg) + h * 8;
         char* o = reinterpret_cast<char*>(static_cast<T*>(a.out) + b0 * a.ldo + x);
@@ -241,10 +246,11 @@ int launch_tile(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, cons
                 int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
     static bool attr[64] = {false};
     RDB_TRY(tile_smem_attr(sq8_tile_kernel<T>, attr));
+    DotArgs a{qs, xs, nq, n, ldo, (int)((nq + TT_N - 1) / TT_N), (int)((n + TT_M - 1) / TT_M), (d + 127) / 128, out,
+              tile_box_rows(n, 128), tile_box_rows((nq + 31) / 32 * 16, 128)};
     CUtensorMap mx, mq;
-    RDB_TRY(make_map_3d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, d, n, 1, ldx, 0, 128));
-    RDB_TRY(make_map_3d(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, d, nq, 1, ldq, 0, 128));
-    DotArgs a{qs, xs, nq, n, ldo, (int)((nq + TT_N - 1) / TT_N), (int)((n + TT_M - 1) / TT_M), (d + 127) / 128, out};
+    RDB_TRY(make_map_3d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, d, n, 1, ldx, 0, a.x_rows));
+    RDB_TRY(make_map_3d(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, d, nq, 1, ldq, 0, a.q_rows));
     const int64_t tiles = (int64_t)a.nqt * a.nxt;
     sq8_tile_kernel<T><<<2 * (unsigned)std::min<int64_t>(tile_pairs(), tiles), TT_THREADS, TT_SMEM, s>>>(
         mx, mq, a, tile_status());

@@ -4,8 +4,8 @@
 // A CTA pair (cluster of 2, cta_group::2) computes one 256 x nn tile after the
 // other, nn <= 256, D = sum_k A[m, k] B[n, k]:
 //   warp 0      TMA producer: per K block of 128 bytes each CTA loads its 128
-//               rows of A and its nn / 2 rows of B into a 5-stage ring (4 to 6
-//               stages measure the same).
+//               rows of A and its nn / 2 rows of B into a ring of 5 or more
+//               stages.
 //   warp 1      TMEM (two 256-column accumulators); the leader's lane 0 issues
 //               the MMAs and commits stage releases and finished accumulators.
 //   warps 2..17 epilogue, four per TMEM lane quadrant: a thread owns one row of
@@ -27,13 +27,14 @@
 //
 // A policy P supplies the tiles and what becomes of them:
 //   P::kInt8                       int8 operands, int32 accumulators
+//   P::kStages, P::kStgBytes       ring stages, staging bytes per epilogue warp
 //   P::Job                         TileJob and what the epilogue needs with it
 //   P::Iter(p, pair, npairs)       the pair's tiles: bool next(job), the same
 //                                  sequence in every role
 //   P::Epi                         per-thread epilogue state
 //   p.begin(epi, job, ctx)         while the tile is still being multiplied
 //   p.tile(epi, job, ctx, ra, rb)  the warp's accumulators: 32 from column
-//                                  32 grp on, 32 from column 128 + 32 grp on
+//                                  ctx.col0 on, 32 from column ctx.col1 on
 //                                  (where the tile is that wide)
 //   p.finish(ctx)                  once, after the last tile
 // The epilogue's warps never wait for one another: they drift apart by up to
@@ -51,7 +52,7 @@ namespace {
 
 constexpr int TT_M = 256;         // rows of a pair's tile
 constexpr int TT_N = 256;         // largest columns of a tile
-constexpr int TT_STAGES = 5;
+constexpr int TT_MAX_STAGES = 7;
 constexpr int TT_A_BYTES = 16384;  // 128 rows x 128 bytes
 constexpr int TT_STAGE_BYTES = 2 * TT_A_BYTES;
 constexpr int TT_BLOCK_BYTES = 8192;  // 64 elements x 64 K rows (MN-major)
@@ -59,8 +60,9 @@ constexpr int TT_EPI_WARPS = 16;
 constexpr int TT_GROUPS = TT_EPI_WARPS / 4;  // warps per TMEM lane quadrant
 constexpr int TT_THREADS = 64 + 32 * TT_EPI_WARPS;
 constexpr int TT_BAR_BYTES = 256;
-constexpr int TT_STG_BYTES = 4096;           // per epilogue warp: 32 rows x 32 columns on their way out
-constexpr int TT_SMEM = TT_STAGES * TT_STAGE_BYTES + TT_EPI_WARPS * TT_STG_BYTES + TT_BAR_BYTES + 1024;
+constexpr int TT_STG_BYTES = 4096;  // staging for 32 rows x 32 fp32 columns on their way out
+// every policy's shared memory: 7 stages, or 5 and staging for the stores
+constexpr int TT_SMEM = TT_MAX_STAGES * TT_STAGE_BYTES + TT_BAR_BYTES + 1024;
 static_assert(TT_SMEM <= 232448, "shared memory over 227 KB");
 
 // products of planes (A plane, B plane), largest first
@@ -74,6 +76,11 @@ struct TileJob {
     int k0, nk;                  // first K block and K blocks per product
     int nseg;                    // products of planes: 1 or 6
     bool a_mn, b_mn;
+    // rows of a CTA's box where the operand is K-major (the maps' box rows, a
+    // multiple of 8 up to 128).  A needs only the rows that exist: what an MMA
+    // reads behind them ends in accumulator rows that nobody uses.
+    int a_rows, b_rows;
+    bool a_second;               // the pair's second CTA has rows of A at all
 };
 
 __device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint32_t bar_cluster, void* dst, int x, int y,
@@ -116,9 +123,10 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc_i8(int m, int n) {
 // What an epilogue thread knows of its place.
 struct TileCtx {
     int row;        // row of the pair's tile
-    int quad, grp;  // TMEM lane quadrant, which of its four warps
+    int quad, grp;  // TMEM lane quadrant, which of its warps
+    int col0, col1; // first columns of its two chunks
     int lane;
-    uint8_t* stg;   // the warp's TT_STG_BYTES (1024-byte aligned)
+    uint8_t* stg;   // the warp's P::kStgBytes (1024-byte aligned if they are a multiple)
 };
 
 // ---- staged stores: a warp writes 32 rows of 64 or 128 bytes to its staging
@@ -185,8 +193,12 @@ __device__ __forceinline__ void tt_give_up(volatile int* abort_flag, const TileS
 template <class P>
 __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const bool bf16, const TileStatus st) {
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int TT_STAGES = P::kStages;
+    static_assert(TT_STAGES <= TT_MAX_STAGES &&
+                      TT_STAGES * TT_STAGE_BYTES + TT_EPI_WARPS * P::kStgBytes <= TT_MAX_STAGES * TT_STAGE_BYTES,
+                  "stages and staging over the block's shared memory");
     uint8_t* stg = smem + TT_STAGES * TT_STAGE_BYTES;
-    uint64_t* full = reinterpret_cast<uint64_t*>(stg + TT_EPI_WARPS * TT_STG_BYTES);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + TT_MAX_STAGES * TT_STAGE_BYTES);
     uint64_t* empty = full + TT_STAGES;
     uint64_t* tfull = empty + TT_STAGES;
     uint64_t* tempty = tfull + 2;
@@ -236,11 +248,16 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
                 const int half = j.nn / 2;
                 const int am = j.m0 + static_cast<int>(rank) * 128, bn = j.n0 + static_cast<int>(rank) * half;
                 const int b_blocks = j.b_mn ? half / 64 : 2;
-                const uint32_t bytes = 2u * (TT_A_BYTES + static_cast<uint32_t>(b_blocks) * TT_BLOCK_BYTES);
+                const bool load_a = leader || j.a_second;
+                const uint32_t bytes =
+                    (j.a_second ? 2u : 1u) * (j.a_mn ? TT_A_BYTES : static_cast<uint32_t>(j.a_rows) * 128u) +
+                    2u * (j.b_mn ? static_cast<uint32_t>(b_blocks) * TT_BLOCK_BYTES
+                                 : static_cast<uint32_t>(j.b_rows) * 128u);
                 for (int g = 0; g < j.nseg && ok; ++g) {
                     const int za = kSegA[g], zb = kSegB[g];
                     for (int kb = 0; kb < j.nk; ++kb) {
-                        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
+                        if (!mbar_try_wait(&empty[stage], phase ^ 1) &&
+                            !mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
                             ok = false;
                             break;
                         }
@@ -249,7 +266,8 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
                         const uint32_t bar = full_lead + static_cast<uint32_t>(stage * sizeof(uint64_t));
                         if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
                         const int k = (j.k0 + kb) * kElems;
-                        if (j.a_mn) {
+                        if (!load_a) {
+                        } else if (j.a_mn) {
                             tma_load_3d_pair(j.ma, bar, sa, am, k, za);
                             tma_load_3d_pair(j.ma, bar, sa + TT_BLOCK_BYTES, am + 64, k, za);
                         } else {
@@ -308,7 +326,7 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
                 const uint64_t a_step = j.a_mn ? 128 : 2, b_step = j.b_mn ? 128 : 2;
                 const int total = j.nseg * j.nk;
                 for (int kb = 0; kb < total; ++kb) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag)) {
+                    if (!mbar_try_wait(&full[stage], phase) && !mbar_wait(&full[stage], phase, abort_flag)) {
                         ok = false;
                         break;
                     }
@@ -349,8 +367,10 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
         ctx.quad = warp & 3;  // TMEM lanes this warp may read
         ctx.grp = (warp - 2) >> 2;
         ctx.lane = lane;
+        ctx.col0 = ctx.grp * 32;
+        ctx.col1 = ctx.col0 + TT_GROUPS * 32;
         ctx.row = static_cast<int>(rank) * 128 + ctx.quad * 32 + lane;
-        ctx.stg = stg + (warp - 2) * TT_STG_BYTES;
+        ctx.stg = stg + (warp - 2) * P::kStgBytes;
         const uint32_t tempty_lead = map_to_rank(&tempty[0], 0);
         typename P::Epi epi;
         typename P::Job j;
@@ -359,19 +379,17 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
         for (; it.next(j); ++tile) {
             const int acc = tile & 1;
             p.begin(epi, j, ctx);
-            if (!mbar_wait(&tfull[acc], (tile >> 1) & 1, abort_flag)) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (tile >> 1) & 1, abort_flag))) {
                 tt_give_up(abort_flag, st, DEV_TIMEOUT_EPILOGUE);
                 break;
             }
-            __syncwarp();
             tc_fence_after();
-            const int c0 = ctx.grp * 32, c1 = c0 + TT_GROUPS * 32;
             const uint32_t tbase =
                 tmem_base + (static_cast<uint32_t>(ctx.quad * 32) << 16) + static_cast<uint32_t>(acc * TT_N);
             uint32_t ra[32], rb[32];
             // (columns behind a narrow tile hold older values, which no policy uses)
-            tmem_ld32_async(tbase + static_cast<uint32_t>(c0), ra);
-            tmem_ld32_async(tbase + static_cast<uint32_t>(c1), rb);
+            tmem_ld32_async(tbase + static_cast<uint32_t>(ctx.col0), ra);
+            tmem_ld32_async(tbase + static_cast<uint32_t>(ctx.col1), rb);
             tmem_ld_wait(ra);
             tmem_ld_wait(rb);
             tc_fence_before();
@@ -442,6 +460,11 @@ int tile_smem_attr(K kernel, bool (&done)[64]) {
 }
 
 inline TileStatus tile_status() { return {device_status_word(), status_mirror_device()}; }
+
+// box rows of a K-major operand of `rows` rows in tiles of `width` per CTA
+inline int tile_box_rows(int64_t rows, int width) {
+    return static_cast<int>(rows < width ? (rows + 7) / 8 * 8 : width);
+}
 
 inline int tile_pairs() { return num_sms() / 2; }
 

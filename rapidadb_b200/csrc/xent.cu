@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "tile_f32.cuh"
 #include "tile_tc.cuh"
 
 namespace rdb {
@@ -100,16 +101,20 @@ struct FwdArgs {
     int64_t nq, n;       // queries, rows of this piece
     int64_t row0;        // first row of the piece in the base
     int nqb, nsplit, slot0;
+    int q_rows, width;   // box rows of the queries, columns of a tile
     int n32;             // 32-row groups of the piece, dealt evenly to the splits
     int nkb, nseg;
     float c;
     const int64_t* targets;
-    float2* part;        // [slots * TT_GROUPS][nq] (max <q, x>, z) of each split and epilogue group
+    int groups, parts;   // epilogue groups, parts per query: slots * groups
+    float2* part;        // [nq][parts] (max <q, x>, z) of each split and epilogue group
     float* tdot;         // [nq] <q, x_t>
+    unsigned* ticket;    // of the join, cleared here
 };
 
 struct FwdPolicy {
     static constexpr bool kInt8 = false;
+    static constexpr int kStages = 7, kStgBytes = 0;
     const CUtensorMap *mq, *mx;
     const FwdArgs& a;
 
@@ -135,14 +140,17 @@ struct FwdPolicy {
             j.mb = p.mx;
             j.m0 = unit % p.a.nqb * TT_M;
             j.n0 = at * 32;
-            j.nn = min(TT_N, (hi - at) * 32);
+            j.nn = min(p.a.width, (hi - at) * 32);
             j.k0 = 0;
             j.nk = p.a.nkb;
             j.nseg = p.a.nseg;
             j.a_mn = j.b_mn = false;
+            j.a_rows = p.a.q_rows;
+            j.b_rows = p.a.width / 2;
+            j.a_second = j.m0 + 128 < p.a.nq;
             j.split = unit / p.a.nqb;
             j.first = at == lo;
-            at += TT_N / 32;
+            at += p.a.width / 32;
             j.last = at >= hi;
             return true;
         }
@@ -222,11 +230,11 @@ struct FwdPolicy {
     __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
                                          const uint32_t (&rb)[32]) const {
         if (j.m0 + c.row - c.lane >= a.nq) return;  // no query in this warp's 32 rows
-        if (c.grp * 32 < j.nn) chunk(e, j, c, c.grp * 32, ra);
-        if (128 + c.grp * 32 < j.nn) chunk(e, j, c, 128 + c.grp * 32, rb);
+        if (c.col0 < j.nn) chunk(e, j, c, c.col0, ra);
+        if (c.col1 < j.nn) chunk(e, j, c, c.col1, rb);
         const int64_t b = j.m0 + c.row;
         if (j.last && b < a.nq)
-            a.part[(static_cast<int64_t>(a.slot0 + j.split) * TT_GROUPS + c.grp) * a.nq + b] = make_float2(e.m, e.z);
+            a.part[b * a.parts + (a.slot0 + j.split) * a.groups + c.grp] = make_float2(e.m, e.z);
     }
     __device__ __forceinline__ void finish(const TileCtx&) const {}
 };
@@ -235,36 +243,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     xent_scan_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mx,
                      const __grid_constant__ FwdArgs a, const bool bf16, const TileStatus st) {
     extern __shared__ uint8_t smem_raw[];
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
     const FwdPolicy p{&mq, &mx, a};
     tile_loop(smem_raw, p, bf16, st);
 }
 
-constexpr int JG = 32;  // threads per query
-// Joins the parts of 32 queries per block and step; stats and loss of each
-// query.  An ignored query has loss 0; one whose target is no row is NaN
-// throughout.  A single block also reduces the losses (total; the queries that
-// count behind the stats).
-__global__ void __launch_bounds__(32 * JG)
-    xent_join_kernel(const float2* part, int slots, const float* tdot, const int64_t* targets, int64_t ignore,
-                     int64_t n, float c, int64_t nq, float* stats, float* loss, int reduction, float* total) {
-    __shared__ float2 sh[JG][33];
-    const int qi = threadIdx.x & 31, g = threadIdx.x >> 5;
-    float lsum = 0.f;
-    int count = 0;
-    for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * 32; b0 < nq; b0 += static_cast<int64_t>(gridDim.x) * 32) {
-        const int64_t b = b0 + qi;
+// the same for at most 128 queries and fp32 rows as they are
+__global__ void __launch_bounds__(TF_THREADS, 1)
+    xent_scan_f32_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ F32Rows x,
+                         const __grid_constant__ FwdArgs a, const TileStatus st) {
+    extern __shared__ uint8_t smem_raw[];
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
+    const FwdPolicy p{&mq, nullptr, a};
+    tile_loop_f32(smem_raw, p, x, st);
+}
+
+// mean or sum of the losses of the queries that count, and their number, by one
+// block in index order
+__device__ void reduce_losses(float* stats, const int64_t* targets, int64_t ignore, int64_t nq, int reduction,
+                              float* total, float* ss, int* sc) {
+    float s = 0.f;
+    int cnt = 0;
+    for (int64_t i = threadIdx.x; i < nq; i += NT)
+        if (targets[i] != ignore) s += __ldcg(stats + 2 * nq + i), ++cnt;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if ((threadIdx.x & 31) == 0) ss[threadIdx.x >> 5] = s, sc[threadIdx.x >> 5] = cnt;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < NT / 32; ++w) ss[0] += ss[w], sc[0] += sc[w];
+        *total = reduction == RDB_REDUCE_MEAN ? ss[0] / static_cast<float>(sc[0]) : ss[0];
+        stats[3 * nq] = static_cast<float>(sc[0]);
+    }
+}
+
+// Joins the parts of each query, one warp per query; stats and loss of each.  An
+// ignored query has loss 0; one whose target is no row is NaN throughout.  For a
+// reduced loss the last block to finish sums the losses (in index order, whoever
+// it is) and leaves the number of queries that count behind the stats; `ticket`
+// was cleared by the scan.
+__global__ void __launch_bounds__(NT)
+    xent_join_kernel(const float2* part, int parts, const float* tdot, const int64_t* targets, int64_t ignore,
+                     int64_t n, float c, int64_t nq, float* stats, float* loss, int reduction, float* total,
+                     unsigned* ticket) {
+    __shared__ float ss[NT / 32];
+    __shared__ int sc[NT / 32];
+    __shared__ bool last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int64_t b = static_cast<int64_t>(blockIdx.x) * (NT / 32) + warp; b < nq;
+         b += static_cast<int64_t>(gridDim.x) * (NT / 32)) {
         float M = -INFINITY, Z = 0.f;
-        if (b < nq)
 #pragma unroll 4
-            for (int s = g; s < slots; s += JG) {
-                const float2 v = part[static_cast<int64_t>(s) * nq + b];
-                join(M, Z, v.x, v.y, c);
-            }
-        sh[g][qi] = make_float2(M, Z);
-        __syncthreads();
-        if (g == 0 && b < nq) {
-            const int used = min(JG, slots);
-            for (int k = 1; k < used; ++k) join(M, Z, sh[k][qi].x, sh[k][qi].y, c);
+        for (int s = lane; s < parts; s += 32) {
+            const float2 v = part[b * parts + s];
+            join(M, Z, v.x, v.y, c);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float m = __shfl_xor_sync(0xffffffffu, M, o), z = __shfl_xor_sync(0xffffffffu, Z, o);
+            // the same operands in the same order on both sides
+            float lo_m = lane & o ? m : M, lo_z = lane & o ? z : Z;
+            join(lo_m, lo_z, lane & o ? M : m, lane & o ? Z : z, c);
+            M = lo_m, Z = lo_z;
+        }
+        if (lane == 0) {
             const int64_t t = targets[b];
             const bool ignored = t == ignore, has = t >= 0 && t < n;
             const float nan = __int_as_float(0x7fc00000);
@@ -288,43 +331,28 @@ __global__ void __launch_bounds__(32 * JG)
             stats[b] = m;
             stats[nq + b] = lz;
             stats[2 * nq + b] = l;
-            if (loss) loss[b] = l;
-            lsum += l;
-            count += !ignored;
-        }
-        __syncthreads();
-    }
-    if (reduction == RDB_REDUCE_NONE && blockIdx.x == 0 && threadIdx.x == 0) stats[3 * nq] = 0.f;
-    if (total && g == 0) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
-        count = __reduce_add_sync(0xffffffffu, count);
-        if (qi == 0) {
-            *total = reduction == RDB_REDUCE_MEAN ? lsum / static_cast<float>(count) : lsum;
-            stats[3 * nq] = static_cast<float>(count);
+            if (reduction == RDB_REDUCE_NONE) loss[b] = l;
         }
     }
+    if (reduction == RDB_REDUCE_NONE) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) stats[3 * nq] = 0.f;
+        return;
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    reduce_losses(stats, targets, ignore, nq, reduction, total, ss, sc);
 }
 
-// mean or sum of the losses of the queries that are not ignored, and their count
-__global__ void __launch_bounds__(1024)
+// the reduced loss of no queries
+__global__ void __launch_bounds__(NT)
     xent_reduce_kernel(const int64_t* targets, int64_t ignore, int64_t nq, int reduction, float* stats, float* total) {
-    __shared__ float ss[32];
-    __shared__ int sc[32];
-    float s = 0.f;
-    int cnt = 0;
-    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x)
-        if (targets[i] != ignore) s += stats[2 * nq + i], ++cnt;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    cnt = __reduce_add_sync(0xffffffffu, cnt);
-    if ((threadIdx.x & 31) == 0) ss[threadIdx.x >> 5] = s, sc[threadIdx.x >> 5] = cnt;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 32; ++w) ss[0] += ss[w], sc[0] += sc[w];
-        *total = reduction == RDB_REDUCE_MEAN ? ss[0] / static_cast<float>(sc[0]) : ss[0];
-        stats[3 * nq] = static_cast<float>(sc[0]);
-    }
+    __shared__ float ss[NT / 32];
+    __shared__ int sc[NT / 32];
+    reduce_losses(stats, targets, ignore, nq, reduction, total, ss, sc);
 }
 
 // --------------------------------------------------------------- backward --
@@ -445,7 +473,7 @@ __global__ void __launch_bounds__(NT)
 struct ProbArgs {
     int64_t nq, n, row0;  // queries, rows of the piece, its first row
     int nqb, njobs, nkb, nseg;
-    int width;            // columns of a tile
+    int q_rows, width;    // box rows of the queries, columns of a tile
     float c;
     const int64_t* targets;
     int64_t ignore;
@@ -456,6 +484,7 @@ struct ProbArgs {
 template <typename T>
 struct ProbPolicy {
     static constexpr bool kInt8 = false;
+    static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
     const CUtensorMap *mq, *mx, *mg;
     const ProbArgs& a;
 
@@ -475,6 +504,9 @@ struct ProbPolicy {
             j.nk = p.a.nkb;
             j.nseg = p.a.nseg;
             j.a_mn = j.b_mn = false;
+            j.a_rows = p.a.q_rows;
+            j.b_rows = p.a.width / 2;
+            j.a_second = j.m0 + 128 < p.a.nq;
             i += step;
             return true;
         }
@@ -553,9 +585,9 @@ struct ProbPolicy {
 
     __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
                                          const uint32_t (&rb)[32]) const {
-        if (c.grp * 32 < j.nn) chunk(e, j, c, c.grp * 32, ra);
+        if (c.col0 < j.nn) chunk(e, j, c, c.col0, ra);
         __syncwarp();
-        if (128 + c.grp * 32 < j.nn) chunk(e, j, c, 128 + c.grp * 32, rb);
+        if (c.col1 < j.nn) chunk(e, j, c, c.col1, rb);
     }
     __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
@@ -569,10 +601,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     tile_loop(smem_raw, p, bf16, st);
 }
 
+__global__ void __launch_bounds__(TF_THREADS, 1)
+    xent_prob_f32_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mg,
+                         const __grid_constant__ F32Rows x, const __grid_constant__ ProbArgs a, const TileStatus st) {
+    extern __shared__ uint8_t smem_raw[];
+    const ProbPolicy<float> p{&mq, nullptr, &mg, a};
+    tile_loop_f32(smem_raw, p, x, st);
+}
+
 struct GradArgs {
     int64_t nq, n;         // queries, rows of the piece
     int d, nseg;
-    int nt;                // column tiles of d
+    int nt, width;         // column tiles of d, their columns
+    int q_rows;            // box rows of G as dq's operand
     int q_blocks, q_split, q_per;  // dq: 256-query blocks, K splits, K blocks per split (0 blocks: not wanted)
     int kc, kq;            // K blocks of the piece and of the queries
     int x_blocks;          // dx: 256-row blocks (0: not wanted)
@@ -588,6 +629,7 @@ struct GradArgs {
 template <typename T>
 struct GradPolicy {
     static constexpr bool kInt8 = false;
+    static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
     const CUtensorMap *gk, *gmn, *xmn, *qmn, *mpart, *mdx;
     const GradArgs& a;
 
@@ -609,14 +651,17 @@ struct GradPolicy {
             i += step;
             j.nseg = a.nseg;
             j.b_mn = true;
-            j.n0 = k % a.nt * TT_N;
+            j.b_rows = 128;
+            j.n0 = k % a.nt * a.width;
             k /= a.nt;
-            j.nn = min(TT_N, (a.d - j.n0 + 127) / 128 * 128);
+            j.nn = min(a.width, (a.d - j.n0 + 127) / 128 * 128);
             if (j.is_dx) {
                 j.ma = p.gmn;
                 j.mb = p.qmn;
                 j.a_mn = true;
+                j.a_rows = 128;
                 j.m0 = k * TT_M;
+                j.a_second = j.m0 + 128 < a.n;
                 j.k0 = 0;
                 j.nk = a.kq;
                 j.split = 0;
@@ -626,6 +671,8 @@ struct GradPolicy {
                 j.a_mn = false;
                 j.split = k / a.q_blocks;
                 j.m0 = k % a.q_blocks * TT_M;
+                j.a_rows = a.q_rows;
+                j.a_second = j.m0 + 128 < a.nq;
                 j.k0 = j.split * a.q_per;
                 j.nk = min(a.q_per, a.kc - j.k0);
             }
@@ -645,12 +692,18 @@ struct GradPolicy {
         const int y = j.m0 + c.row - c.lane, x = j.n0 + col;
         if (x >= a.d || y >= (j.is_dx ? a.n : a.nq)) return;
         if (j.is_dx && !a.dx_tma) {
-            // rows that no tensor map can describe
-            if (y + c.lane >= a.n) return;
-            T* o = static_cast<T*>(a.dx) + static_cast<int64_t>(y + c.lane) * a.lddx + x;
+            stg_wait_read(c.lane);
+            // rows that no tensor map can describe: transposed in the staging
+            // bytes, so that a store writes 32 columns of one row
+            float* t = reinterpret_cast<float*>(c.stg);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (x + i < a.d) o[i] = from_f<T>(__uint_as_float(r[i]) * e.f);
+            for (int i = 0; i < 32; ++i) t[c.lane * 32 + ((i + c.lane) & 31)] = __uint_as_float(r[i]) * e.f;
+            __syncwarp();
+            T* o = static_cast<T*>(a.dx) + static_cast<int64_t>(y) * a.lddx + x + c.lane;
+            const int rows = static_cast<int>(min(static_cast<int64_t>(32), a.n - y));
+            if (x + c.lane < a.d)
+                for (int i = 0; i < rows; ++i, o += a.lddx) *o = from_f<T>(t[i * 32 + ((c.lane + i) & 31)]);
+            __syncwarp();
             return;
         }
         stg_wait_read(c.lane);
@@ -686,9 +739,9 @@ struct GradPolicy {
 
     __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
                                          const uint32_t (&rb)[32]) const {
-        if (c.grp * 32 < j.nn) chunk(e, j, c, c.grp * 32, ra);
+        if (c.col0 < j.nn) chunk(e, j, c, c.col0, ra);
         __syncwarp();
-        if (128 + c.grp * 32 < j.nn) chunk(e, j, c, 128 + c.grp * 32, rb);
+        if (c.col1 < j.nn) chunk(e, j, c, c.col1, rb);
     }
     __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
@@ -702,6 +755,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     const GradPolicy<T> p{&gk, &gmn, &xmn, &qmn, &mpart, &mdx, a};
     tile_loop(smem_raw, p, bf16, st);
+}
+
+// dq of at most 128 queries from fp32 rows as they are
+__global__ void __launch_bounds__(TF_THREADS, 1)
+    xent_grad_f32_kernel(const __grid_constant__ CUtensorMap gk, const __grid_constant__ CUtensorMap mpart,
+                         const __grid_constant__ F32Rows x, const __grid_constant__ GradArgs a, const TileStatus st) {
+    extern __shared__ uint8_t smem_raw[];
+    const GradPolicy<float> p{&gk, nullptr, nullptr, nullptr, &mpart, nullptr, a};
+    tile_loop_f32(smem_raw, p, x, st);
 }
 
 // dq_b = w_b scale 2^-14 (sum of the parts, in split order)
@@ -757,9 +819,10 @@ struct Planes {
     int count;
 };
 
-int operand_map(CUtensorMap* m, int dtype, const Planes& o, int64_t cols, int64_t rows, bool mn) {
+// box_rows: of a K-major operand; 0: MN-major
+int operand_map(CUtensorMap* m, int dtype, const Planes& o, int64_t cols, int64_t rows, int box_rows) {
     return make_map_3d(m, map_type(dtype), 2, o.p, cols, rows, o.count, o.ld * 2,
-                       o.count > 1 ? o.plane * 2 : 0, mn ? 64 : 128);
+                       o.count > 1 ? o.plane * 2 : 0, box_rows ? box_rows : 64);
 }
 
 struct Arena {
@@ -782,41 +845,53 @@ int64_t piece_rows(int64_t n, int64_t most) {
 
 struct FwdPlan {
     int64_t rows;  // rows per piece
-    int pieces, nqb, nkb, nseg, slots, nsplit[2];  // nsplit of a full and of the last piece
+    bool direct;
+    int pieces, nqb, nkb, nseg, groups, workers, slots, width, nsplit[2];  // nsplit of a full and of the last piece
 };
 
 // Row splits of one piece: as many as give every pair the same number of rows
-// (in groups of 32); a split costs about a third of a tile (its fill and parts).
+// (in groups of 32), for the number of rounds that costs least; a split costs
+// about a third of a tile (its fill and parts).
 int fwd_splits(int nqb, int64_t rows, int pairs) {
     const int64_t n32 = (rows + 31) / 32;
-    int best = 1;
+    int64_t best = 1;
     double best_cost = 1e30;
-    const int64_t most = std::min<int64_t>(n32, std::max<int64_t>(1, 16LL * pairs / nqb + 1));
-    for (int64_t s = 1; s <= most; ++s) {
+    for (int64_t round = 1; round <= 16; ++round) {
+        const int64_t s = std::max<int64_t>(1, std::min<int64_t>(n32, round * pairs / nqb));
         const double tiles = (double)((n32 + s - 1) / s) / (TT_N / 32);
         const double cost = (double)((nqb * s + pairs - 1) / pairs) * (tiles + 0.3);
-        if (cost < best_cost) best_cost = cost, best = (int)s;
+        if (cost < best_cost) best_cost = cost, best = s;
     }
-    return best;
+    return (int)best;
 }
+
+// fp32 rows are split on the way (tile_f32.cuh) where one block of 128 queries
+// reads them; more queries share planes written once per piece.
+bool f32_direct(int dtype, int64_t nq) { return dtype == RDB_F32 && nq <= 128; }
 
 FwdPlan fwd_plan(int dtype, int64_t nq, int64_t n, int d) {
     FwdPlan p;
     const int64_t dp = up(d, 8);
+    p.direct = f32_direct(dtype, nq);
     // fp32: the planes of a piece stay in L2
-    p.rows = dtype == RDB_F32 ? piece_rows(n, (96LL << 20) / (6 * dp)) : up(n, 256);
+    p.rows = dtype == RDB_F32 && !p.direct ? piece_rows(n, (96LL << 20) / (6 * dp)) : up(n, 256);
     p.pieces = (int)((n + p.rows - 1) / p.rows);
     p.nqb = (int)std::max<int64_t>(1, (nq + TT_M - 1) / TT_M);
     p.nkb = (d + 63) / 64;
     p.nseg = dtype == RDB_F32 ? 6 : 1;
-    const int pairs = tile_pairs();
-    p.nsplit[0] = fwd_splits(p.nqb, p.rows, pairs);
-    p.nsplit[1] = fwd_splits(p.nqb, n - (p.pieces - 1) * p.rows, pairs);
+    p.groups = p.direct ? TF_GROUPS : TT_GROUPS;
+    p.workers = p.direct ? num_sms() : tile_pairs();
+    p.nsplit[0] = fwd_splits(p.nqb, std::min(p.rows, n), p.workers);
+    p.nsplit[1] = fwd_splits(p.nqb, n - (p.pieces - 1) * p.rows, p.workers);
+    // (few rows in all: a narrow tile is all a split has)
+    p.width = p.direct ? TF_N
+                       : (int)std::min<int64_t>(TT_N, up((up(p.rows, 32) / 32 + p.nsplit[0] - 1) / p.nsplit[0] * 32, 64));
     p.slots = (p.pieces - 1) * p.nsplit[0] + p.nsplit[1];
     return p;
 }
 
 struct FwdWs {
+    unsigned* ticket;
     float* tdot;
     float2* part;
     __nv_bfloat16 *qp, *xp;
@@ -827,11 +902,12 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
     FwdWs w{};
     Arena a{static_cast<char*>(base)};
     const int64_t dp = up(d, 8);
+    w.ticket = a.take<unsigned>(1);
     w.tdot = a.take<float>(nq);
-    w.part = a.take<float2>((size_t)TT_GROUPS * p.slots * nq);
+    w.part = a.take<float2>((size_t)p.groups * p.slots * nq);
     if (dtype == RDB_F32) {
         w.qp = a.take<__nv_bfloat16>(3 * nq * dp);
-        w.xp = a.take<__nv_bfloat16>(3 * p.rows * dp);
+        if (!p.direct) w.xp = a.take<__nv_bfloat16>(3 * p.rows * dp);
     }
     w.bytes = a.used + 256;
     return w;
@@ -839,13 +915,18 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
 
 struct BwdPlan {
     int64_t rows;  // rows per piece
+    bool direct;   // fp32 rows split on the way (dq, probabilities)
     int pieces, planes, nqb, nt, nkb, nseg, kq, dp;
-    int q_split, q_per;
+    int q_nt, q_width, q_split, q_per;  // dq: column tiles, K splits, K blocks per split
     bool q_first;
 };
 
+// Rounds of `jobs` tiles dealt out in turn to `workers`.
+int64_t rounds(int64_t jobs, int64_t workers) { return (jobs + workers - 1) / workers; }
+
 BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool need_dx) {
     BwdPlan p;
+    p.direct = f32_direct(dtype, nq);
     p.planes = dtype == RDB_F32 ? 3 : 1;
     p.nseg = dtype == RDB_F32 ? 6 : 1;
     const int64_t col = std::max<int64_t>(1, nq * 2 * p.planes);  // bytes of G per row
@@ -853,7 +934,7 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
     // partial sums of dq (read and written once a piece) cost more than they save
     int64_t most = (64LL << 20) / col;
     if (most < 4096) most = std::max(most, std::min<int64_t>(4096, (2LL << 30) / col));
-    if (dtype == RDB_F32) most = std::min<int64_t>(most, (96LL << 20) / (6 * up(d, 8)));
+    if (dtype == RDB_F32 && !p.direct) most = std::min<int64_t>(most, (96LL << 20) / (6 * up(d, 8)));
     p.rows = piece_rows(n, most);
     p.pieces = (int)((n + p.rows - 1) / p.rows);
     p.nqb = (int)std::max<int64_t>(1, (nq + TT_M - 1) / TT_M);
@@ -861,24 +942,28 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
     p.nkb = (d + 63) / 64;
     p.kq = (int)((nq + 63) / 64);
     p.dp = (int)up(d, 32);
+    p.q_width = p.direct ? TF_N : TT_N;
+    p.q_nt = (d + p.q_width - 1) / p.q_width;
     // K splits of dq: the split that ends first, tiles dealt out in turn; a
-    // tile costs about six K blocks on top of its own (fill, drain, store)
-    const int64_t pairs = tile_pairs(), kc = std::min(p.rows, up(n, 64)) / 64;
-    const int64_t nx = need_dx ? (p.rows + TT_M - 1) / TT_M * p.nt : 0, lx = (int64_t)p.kq * p.nseg + 6;
+    // tile costs about six K blocks on top of its own (fill, drain, store).
+    // Direct dq tiles have a launch of their own.
+    const int64_t workers = p.direct ? num_sms() : tile_pairs(), kc = std::min(p.rows, up(n, 64)) / 64;
+    const int64_t nx = need_dx && !p.direct ? (p.rows + TT_M - 1) / TT_M * p.nt : 0, lx = (int64_t)p.kq * p.nseg + 6;
     p.q_split = 1;
     p.q_per = (int)kc;
     if (need_dq) {
         int64_t best = INT64_MAX;
-        for (int64_t s = 1; s <= std::min<int64_t>(kc, 64); ++s) {
+        const int64_t most_splits = std::min<int64_t>(kc, p.direct ? 160 : 64);
+        for (int64_t s = 1; s <= most_splits; ++s) {
             if (s > 1 && s * nq * p.dp * 4 > (64LL << 20)) break;
             const int64_t per = (kc + s - 1) / s, used = (kc + per - 1) / per;
-            const int64_t nj = (int64_t)p.nqb * p.nt * used, lq = per * p.nseg + 6;
-            const int64_t slack = (pairs - nj % pairs) % pairs;
-            const int64_t rest = std::max<int64_t>(0, nx - slack);
-            int64_t cost = (nj + pairs - 1) / pairs * std::max(lq, nx ? lx : lq) + (rest + pairs - 1) / pairs * lx;
+            if (used < s) continue;
+            const int64_t nj = (int64_t)p.nqb * p.q_nt * used, lq = per * p.nseg + 6;
+            int64_t cost = rounds(nj, workers) * lq + rounds(nx, workers) * lx;
             if (nx) {
-                // either order: the longer tiles first
-                cost = std::min(cost, (nj + pairs - 1) / pairs * lq + (nx + pairs - 1) / pairs * lx);
+                // tiles of the second kind fill the first's last round
+                const int64_t rest = std::max<int64_t>(0, nx - (rounds(nj, workers) * workers - nj));
+                cost = std::min(cost, rounds(nj, workers) * std::max(lq, lx) + rounds(rest, workers) * lx);
             }
             cost += s / 4;  // parts to join
             if (cost < best) best = cost, p.q_split = (int)used, p.q_per = (int)per;
@@ -905,7 +990,7 @@ BwdWs bwd_ws(void* base, const BwdPlan& p, int dtype, int64_t nq, int d, bool ne
     if (need_dx) w.qw = a.take<uint16_t>((size_t)p.planes * nq * d8);
     if (dtype == RDB_F32) {
         w.qp = a.take<__nv_bfloat16>(3 * nq * d8);
-        w.xp = a.take<__nv_bfloat16>(3 * p.rows * d8);
+        if (!p.direct) w.xp = a.take<__nv_bfloat16>(3 * p.rows * d8);
     }
     w.bytes = a.used + 256;
     return w;
@@ -952,14 +1037,19 @@ template <typename T>
 int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
                const int64_t* targets, float scale, int64_t ignore, int reduction, const float* grad,
                const float* stats, void* dq, int64_t lddq, void* dx, int64_t lddx, void* ws, cudaStream_t s) {
-    static bool attr_p[64] = {false}, attr_g[64] = {false};
+    static bool attr_p[64] = {false}, attr_g[64] = {false}, attr_dp[64] = {false}, attr_dg[64] = {false};
     const BwdPlan p = bwd_plan(dtype, nq, n, d, dq != nullptr, dx != nullptr);
     const BwdWs w = bwd_ws(ws, p, dtype, nq, d, dq != nullptr, dx != nullptr);
     const int64_t d8 = up(d, 8);
     const TileStatus st = tile_status();
     const bool bf16 = dtype != RDB_F16;
     const int pairs = tile_pairs();
-    RDB_TRY(tile_smem_attr(xent_prob_kernel<T>, attr_p));
+    if (p.direct) {
+        RDB_TRY(tile_f32_smem_attr(xent_prob_f32_kernel, attr_dp));
+        RDB_TRY(tile_f32_smem_attr(xent_grad_f32_kernel, attr_dg));
+    } else {
+        RDB_TRY(tile_smem_attr(xent_prob_kernel<T>, attr_p));
+    }
     RDB_TRY(tile_smem_attr(xent_grad_kernel<T>, attr_g));
 
     // equal weights (a reduced loss) are applied to the results
@@ -977,14 +1067,15 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     Planes qo;
     RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
     CUtensorMap mq, mqw;
-    RDB_TRY(operand_map(&mq, dtype, qo, d, nq, false));
+    RDB_TRY(operand_map(&mq, dtype, qo, d, nq, tile_box_rows(nq, 128)));
     mqw = mq;
-    if (dx) RDB_TRY(operand_map(&mqw, dtype, Planes{w.qw, d8, nq * d8, p.planes}, d, nq, true));
+    if (dx) RDB_TRY(operand_map(&mqw, dtype, Planes{w.qw, d8, nq * d8, p.planes}, d, nq, 0));
 
     ProbArgs pa{};
     pa.nq = nq;
     pa.nqb = p.nqb;
     pa.nkb = p.nkb;
+    pa.q_rows = tile_box_rows(nq, 128);
     pa.nseg = p.nseg;
     pa.c = (float)(scale * kLog2e);
     pa.targets = targets;
@@ -995,6 +1086,8 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     ga.d = d;
     ga.nseg = p.nseg;
     ga.nt = p.nt;
+    ga.width = TT_N;
+    ga.q_rows = tile_box_rows(nq, 128);
     ga.q_per = p.q_per;
     ga.kq = p.kq;
     ga.q_first = p.q_first;
@@ -1010,40 +1103,58 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
 
     for (int i = 0; i < p.pieces; ++i) {
         const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
-        Planes xo;
-        RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
-        CUtensorMap mx, mxmn, mgk, mgmn;
-        RDB_TRY(operand_map(&mx, dtype, xo, d, rows, false));
-        RDB_TRY(operand_map(&mxmn, dtype, xo, d, rows, true));
-        RDB_TRY(operand_map(&mgk, dtype, go, rows, nq, false));
-        RDB_TRY(operand_map(&mgmn, dtype, go, rows, nq, true));
-        CUtensorMap mg;
+        const F32Rows xr{static_cast<const float*>(x) + r0 * ldx, ldx, rows, d};  // (direct only)
+        CUtensorMap mx, mxmn = mq, mgk, mgmn, mg;
+        RDB_TRY(operand_map(&mgk, dtype, go, rows, nq, ga.q_rows));
+        RDB_TRY(operand_map(&mgmn, dtype, go, rows, nq, 0));
         RDB_TRY(make_store_map(&mg, map_type(dtype), 2, w.g, rows, nq, p.planes, 2 * p.rows, 2 * p.rows * nq));
         pa.n = rows;
         pa.row0 = r0;
-        pa.width = prob_width(rows, p.nqb, pairs);
+        pa.width = p.direct ? TF_N : prob_width(rows, p.nqb, pairs);
         const int64_t tiles = (rows + pa.width - 1) / pa.width * p.nqb;
         RDB_CHECK_ARG(tiles < (1LL << 31), "too many tiles for one launch");
         pa.njobs = (int)tiles;
-        xent_prob_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS, TT_SMEM, s>>>(mq, mx, mg, pa,
-                                                                                                      bf16, st);
+        if (p.direct) {
+            xent_prob_f32_kernel<<<(unsigned)std::min<int64_t>(num_sms(), tiles), TF_THREADS, TF_SMEM, s>>>(mq, mg, xr,
+                                                                                                           pa, st);
+        } else {
+            Planes xo;
+            RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
+            RDB_TRY(operand_map(&mx, dtype, xo, d, rows, pa.width / 2));
+            RDB_TRY(operand_map(&mxmn, dtype, xo, d, rows, 0));
+            xent_prob_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS, TT_SMEM, s>>>(
+                mq, mx, mg, pa, bf16, st);
+        }
         RDB_LAUNCH_CHECK();
+
         ga.n = rows;
         ga.kc = (int)((rows + 63) / 64);
-        ga.q_blocks = dq ? p.nqb : 0;
         // a shorter last piece may leave splits without rows: their parts stay
         ga.q_split = (ga.kc + p.q_per - 1) / p.q_per;
-        ga.x_blocks = dx ? (int)((rows + TT_M - 1) / TT_M) : 0;
         ga.add = i > 0;
         ga.dx = dx ? static_cast<T*>(dx) + r0 * lddx : nullptr;
         if (ga.dx_tma)
             RDB_TRY(make_store_map(&mdx, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(dtype),
                                    (int)sizeof(T), ga.dx, d, rows, 1, lddx * (int64_t)sizeof(T), 0));
+        if (p.direct && dq) {
+            GradArgs gq = ga;
+            gq.nt = p.q_nt;
+            gq.width = p.q_width;
+            gq.q_blocks = 1;
+            gq.x_blocks = 0;
+            gq.q_first = true;
+            const int64_t jobs = (int64_t)gq.nt * gq.q_split;
+            xent_grad_f32_kernel<<<(unsigned)std::min<int64_t>(num_sms(), jobs), TF_THREADS, TF_SMEM, s>>>(mgk, mpart, xr,
+                                                                                                          gq, st);
+            RDB_LAUNCH_CHECK();
+        }
+        ga.q_blocks = dq && !p.direct ? p.nqb : 0;
+        ga.x_blocks = dx ? (int)((rows + TT_M - 1) / TT_M) : 0;
         const int64_t jobs = (int64_t)ga.nt * ((int64_t)ga.q_blocks * ga.q_split + ga.x_blocks);
+        if (jobs == 0) continue;
         RDB_CHECK_ARG(jobs < (1LL << 31), "too many tiles for one launch");
-        xent_grad_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM, s>>>(mgk, mgmn, mxmn, mqw,
-                                                                                                     mpart, mdx, ga, bf16,
-                                                                                                     st);
+        xent_grad_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM, s>>>(
+            mgk, mgmn, mxmn, mqw, mpart, mdx, ga, bf16, st);
         RDB_LAUNCH_CHECK();
     }
     if (dq) {
@@ -1081,27 +1192,32 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const float c = (float)(scale * kLog2e);
     if (nq > 0) {
-        static bool attr[64] = {false};
-        RDB_TRY(tile_smem_attr(xent_scan_kernel, attr));
+        static bool attr[64] = {false}, attr_d[64] = {false};
+        if (p.direct)
+            RDB_TRY(tile_f32_smem_attr(xent_scan_f32_kernel, attr_d));
+        else
+            RDB_TRY(tile_smem_attr(xent_scan_kernel, attr));
         const TileStatus st = tile_status();
         Planes qo;
         RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
         CUtensorMap mq, mx;
-        RDB_TRY(operand_map(&mq, dtype, qo, d, nq, false));
+        RDB_TRY(operand_map(&mq, dtype, qo, d, nq, tile_box_rows(nq, 128)));
         FwdArgs a{};
+        a.q_rows = tile_box_rows(nq, 128);
+        a.width = p.width;
         a.nq = nq;
         a.nqb = p.nqb;
         a.nkb = p.nkb;
         a.nseg = p.nseg;
         a.c = c;
         a.targets = targets;
+        a.groups = p.groups;
+        a.parts = p.slots * p.groups;
         a.part = w.part;
+        a.ticket = w.ticket;
         a.tdot = w.tdot;
         for (int i = 0; i < p.pieces; ++i) {
             const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
-            Planes xo;
-            RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
-            RDB_TRY(operand_map(&mx, dtype, xo, d, rows, false));
             a.n = rows;
             a.row0 = r0;
             a.n32 = (int)((rows + 31) / 32);
@@ -1109,20 +1225,24 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
             a.slot0 = i * p.nsplit[0];
             const int64_t units = (int64_t)a.nsplit * p.nqb;
             RDB_CHECK_ARG(units < (1LL << 31), "too many tiles for one launch");
-            xent_scan_kernel<<<2 * (unsigned)std::min<int64_t>(tile_pairs(), units), TT_THREADS, TT_SMEM, s>>>(
-                mq, mx, a, dtype != RDB_F16, st);
+            const unsigned workers = (unsigned)std::min<int64_t>(p.workers, units);
+            if (p.direct) {
+                const F32Rows xr{static_cast<const float*>(x), ldx, n, d};
+                xent_scan_f32_kernel<<<workers, TF_THREADS, TF_SMEM, s>>>(mq, xr, a, st);
+            } else {
+                Planes xo;
+                RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
+                RDB_TRY(operand_map(&mx, dtype, xo, d, rows, p.width / 2));
+                xent_scan_kernel<<<2 * workers, TT_THREADS, TT_SMEM, s>>>(mq, mx, a, dtype != RDB_F16, st);
+            }
             RDB_LAUNCH_CHECK();
         }
-        // few parts: one block joins them all and reduces the losses too
-        const bool one = reduction != RDB_REDUCE_NONE && nq <= 512 && nq * p.slots * TT_GROUPS <= 16384;
-        xent_join_kernel<<<one ? 1u : (unsigned)std::min<int64_t>((nq + 31) / 32, 16LL * num_sms()), 32 * JG, 0, s>>>(
-            w.part, TT_GROUPS * p.slots, w.tdot, targets, ignore_index, n, c, nq, stats,
-            reduction == RDB_REDUCE_NONE ? loss : nullptr, reduction, one ? loss : nullptr);
+        xent_join_kernel<<<(unsigned)std::min<int64_t>((nq + NT / 32 - 1) / (NT / 32), 16LL * num_sms()), NT, 0, s>>>(
+            w.part, p.slots * p.groups, w.tdot, targets, ignore_index, n, c, nq, stats, loss, reduction, loss,
+            w.ticket);
         RDB_LAUNCH_CHECK();
-        if (one) return RDB_OK;
-    }
-    if (reduction != RDB_REDUCE_NONE) {
-        xent_reduce_kernel<<<1, 1024, 0, s>>>(targets, ignore_index, nq, reduction, stats, loss);
+    } else if (reduction != RDB_REDUCE_NONE) {
+        xent_reduce_kernel<<<1, NT, 0, s>>>(targets, ignore_index, nq, reduction, stats, loss);
         RDB_LAUNCH_CHECK();
     }
     return RDB_OK;
