@@ -12,10 +12,15 @@
 //   warp 0        TMA producer of A's planes (3 boxes a stage)
 //   warp 1        TMEM (two 128-column accumulators); lane 0 issues the MMAs
 //   warps 2..9    converters: two rows' 256 bytes per load, the next K block's
-//                 loads in flight while this one is split
+//                 loads in flight while this one is split; P::kBMn says which
+//                 way B lies (below)
 //   warps 10..17  epilogue, two per TMEM lane quadrant; policies as in
 //                 tile_tc.cuh
-// A stage is 96 KB (three planes of both operands): two of them.
+// A stage is 96 KB (three planes of both operands): two of them.  What bounds it
+// is shared memory: per K block the MMAs read 192 KB of operands, 96 KB are
+// written, 32 KB pass through L1, 2,500 cycles at 128 bytes a cycle, where the
+// products alone take 1,536.  128 x 100,000 x 768 forward: 144 us (the rows' HBM
+// time is 47); with the planes written to memory first 430.
 //
 // B is K-major (tile rows = matrix rows, K along the row) or MN-major (tile rows
 // = matrix columns, K = matrix rows).
@@ -60,32 +65,67 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 //   K-major   tile row 16 w + 2 i + l / 16, K element 4 (l % 16)
 //   MN-major  K row 8 w + i, column 4 l
 // so a warp's load is two whole 256-byte pieces of rows, or one of 512 bytes.
-__device__ __forceinline__ void tf_load(const F32Rows& x, const TileJob& j, int kb, int w, int lane, float4 (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        int64_t row;
-        int col;
-        bool in;
-        if (j.b_mn) {
-            row = static_cast<int64_t>(j.k0 + kb) * 64 + 8 * w + i;
-            col = j.n0 + 4 * lane;
-            in = row < x.n;
-        } else {
-            const int r = 16 * w + 2 * i + lane / 16;
-            row = static_cast<int64_t>(j.n0) + r;
-            col = (j.k0 + kb) * 64 + 4 * (lane & 15);
-            in = row < x.n && r < j.nn;
-        }
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float* p = x.p + row * x.ld + col;
-        if (in && col + 4 <= x.d) {
-            v[i] = __ldg(reinterpret_cast<const float4*>(p));
-        } else if (in && col < x.d) {
-            // the row's last columns: nothing behind them is read
-            v[i].x = p[0];
-            if (col + 1 < x.d) v[i].y = p[1];
-            if (col + 2 < x.d) v[i].z = p[2];
-        }
+struct TfSource {
+    const float* p;  // group 0
+    int64_t step;    // elements from one group to the next
+    int rows;        // groups i with 2 i < rows (K-major), i < rows (MN-major) exist
+    int cols;        // columns of the matrix from this lane's first on
+};
+
+__device__ __forceinline__ TfSource tf_source(const F32Rows& x, const TileJob& j, int kb, int w, int lane) {
+    TfSource s;
+    int64_t row, left;
+    int col;
+    if (j.b_mn) {
+        row = static_cast<int64_t>(j.k0 + kb) * 64 + 8 * w;
+        col = j.n0 + 4 * lane;
+        left = x.n - row;
+        s.step = x.ld;
+    } else {
+        const int r = 16 * w + lane / 16;
+        row = static_cast<int64_t>(j.n0) + r;
+        col = (j.k0 + kb) * 64 + 4 * (lane & 15);
+        left = min(x.n - row, static_cast<int64_t>(j.nn - r));
+        s.step = 2 * x.ld;
+    }
+    s.rows = static_cast<int>(max(static_cast<int64_t>(0), min(left, static_cast<int64_t>(16))));
+    s.cols = x.d - col;
+    s.p = x.p + row * x.ld + col;
+    return s;
+}
+
+__device__ __forceinline__ float4 tf_load(const TfSource& s, bool mn, int i) {
+    const bool in = (mn ? i : 2 * i) < s.rows;
+    const float* p = s.p + i * s.step;
+    if (in && s.cols >= 4) return __ldg(reinterpret_cast<const float4*>(p));
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in && s.cols > 0) {
+        // the row's last columns: nothing behind them is read
+        v.x = p[0];
+        if (s.cols > 1) v.y = p[1];
+        if (s.cols > 2) v.z = p[2];
+    }
+    return v;
+}
+
+// Asks for a K block's lines in L2, some K blocks ahead of its loads.
+constexpr int TF_AHEAD = 5;
+__device__ __forceinline__ void tf_prefetch(const F32Rows& x, const TileJob& j, int kb, int w, int lane) {
+    if (kb >= j.nk) return;
+    // one lane per 128-byte line
+    if (j.b_mn) {
+        // 8 rows of 512 bytes
+        const int64_t row = static_cast<int64_t>(j.k0 + kb) * 64 + 8 * w + lane / 4;
+        const int col = j.n0 + 32 * (lane & 3);
+        if (row < x.n && col < x.d)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(x.p + row * x.ld + col) : "memory");
+    } else {
+        // 16 rows of 256 bytes
+        const int r = 16 * w + lane / 2;
+        const int64_t row = static_cast<int64_t>(j.n0) + r;
+        const int col = (j.k0 + kb) * 64 + 32 * (lane & 1);
+        if (row < x.n && r < j.nn && col < x.d)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(x.p + row * x.ld + col) : "memory");
     }
 }
 
@@ -95,29 +135,41 @@ __device__ __forceinline__ uint32_t tf_pack(float a, float b) {
     return r;
 }
 
-__device__ __forceinline__ void tf_store(const TileJob& j, int w, int lane, float4 (&v)[8], uint8_t* planes) {
+// the three planes of group i, 8 bytes each
+__device__ __forceinline__ void tf_store(bool mn, int i, int w, int lane, const float4& v, uint8_t* planes) {
+    uint32_t off;
+    if (mn) {
+        const int k = 8 * w + i, c = 4 * lane;  // 64-column block, K row, 16-byte unit, swizzled by the row
+        off = static_cast<uint32_t>((c >> 6) * TT_BLOCK_BYTES + k * 128 + ((((c & 63) >> 3) ^ (k & 7)) << 4) +
+                                    ((c & 4) << 1));
+    } else {
+        const int r = 16 * w + 2 * i + lane / 16, c = 4 * (lane & 15);
+        off = static_cast<uint32_t>(r * 128 + (((c >> 3) ^ (r & 7)) << 4) + ((c & 4) << 1));
+    }
+    float a = v.x, b = v.y, c = v.z, d = v.w;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const uint32_t lo = tf_pack(a, b), hi = tf_pack(c, d);
+        *reinterpret_cast<uint2*>(planes + k * TF_PLANE + off) = make_uint2(lo, hi);
+        if (k == 2) break;
+        // what is left for the next plane: exact in fp32
+        a -= __uint_as_float(lo << 16);
+        b -= __uint_as_float(lo & 0xffff0000u);
+        c -= __uint_as_float(hi << 16);
+        d -= __uint_as_float(hi & 0xffff0000u);
+    }
+}
+
+// Writes the K block in v to `planes`, and every group's successor from `next`
+// into its place as soon as it is written: a load has the time of a whole K
+// block to arrive.
+template <bool MN>
+__device__ __forceinline__ void tf_convert(int w, int lane, float4 (&v)[8], uint8_t* planes, const TfSource& next,
+                                           bool more) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        uint32_t off;
-        if (j.b_mn) {
-            const int k = 8 * w + i, c = 4 * lane;  // 64-column block, K row, 16-byte unit, swizzled by the row
-            off = static_cast<uint32_t>((c >> 6) * TT_BLOCK_BYTES + k * 128 + ((((c & 63) >> 3) ^ (k & 7)) << 4) +
-                                        ((c & 4) << 1));
-        } else {
-            const int r = 16 * w + 2 * i + lane / 16, c = 4 * (lane & 15);
-            off = static_cast<uint32_t>(r * 128 + (((c >> 3) ^ (r & 7)) << 4) + ((c & 4) << 1));
-        }
-        float a = v[i].x, b = v[i].y, c = v[i].z, d = v[i].w;
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            const uint32_t lo = tf_pack(a, b), hi = tf_pack(c, d);
-            *reinterpret_cast<uint2*>(planes + k * TF_PLANE + off) = make_uint2(lo, hi);
-            // what is left for the next plane: exact in fp32
-            a -= __uint_as_float(lo << 16);
-            b -= __uint_as_float(lo & 0xffff0000u);
-            c -= __uint_as_float(hi << 16);
-            d -= __uint_as_float(hi & 0xffff0000u);
-        }
+        tf_store(MN, i, w, lane, v[i], planes);
+        if (more) v[i] = tf_load(next, MN, i);
     }
 }
 
@@ -259,24 +311,31 @@ __device__ __forceinline__ void tile_loop_f32(uint8_t* smem_raw, const P& p, con
         typename P::Iter it(p, cta, nctas);
         bool more = it.next(jn);
         float4 v[8];
-        if (more) tf_load(x, jn, 0, w, lane, v);
+        if (more) {
+            const TfSource src = tf_source(x, jn, 0, w, lane);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = tf_load(src, P::kBMn, i);
+            for (int kb = 1; kb < TF_AHEAD; ++kb) tf_prefetch(x, jn, kb, w, lane);
+        }
         bool ok = true;
         while (ok && more) {
             j = jn;
             more = it.next(jn);
             for (int kb = 0; kb < j.nk; ++kb) {
+                const bool inner = kb + 1 < j.nk;
+                const TfSource next = inner ? tf_source(x, j, kb + 1, w, lane) : tf_source(x, jn, 0, w, lane);
+                if (kb + TF_AHEAD < j.nk)
+                    tf_prefetch(x, j, kb + TF_AHEAD, w, lane);
+                else if (more)
+                    tf_prefetch(x, jn, kb + TF_AHEAD - j.nk, w, lane);
                 if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag))) {
                     ok = false;
                     break;
                 }
-                tf_store(j, w, lane, v, smem + stage * TF_STAGE_BYTES + 3 * TF_PLANE);
+                tf_convert<P::kBMn>(w, lane, v, smem + stage * TF_STAGE_BYTES + 3 * TF_PLANE, next, inner || more);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[stage]);
-                if (kb + 1 < j.nk)
-                    tf_load(x, j, kb + 1, w, lane, v);
-                else if (more)
-                    tf_load(x, jn, 0, w, lane, v);
                 if (++stage == TF_STAGES) {
                     stage = 0;
                     phase ^= 1;

@@ -18,7 +18,7 @@
 //
 // Backward: the rows in pieces of C.  Per piece one launch recomputes the
 // logits and writes G / (g_b scale) = p - [n = t] as a [nq, C] workspace in the
-// operands' type (about 64 MB, so that it stays in L2), one launch multiplies
+// operands' type (at most 512 MB), one launch multiplies
 // it both ways: dx rows directly (K = nq), dq into fp32 partial sums (K = C,
 // split over several tiles when there are few queries), joined at the end.
 // No atomics: every sum has a fixed order.
@@ -115,6 +115,7 @@ struct FwdArgs {
 struct FwdPolicy {
     static constexpr bool kInt8 = false;
     static constexpr int kStages = 7, kStgBytes = 0;
+    static constexpr bool kBMn = false;  // (tile_f32.cuh)
     const CUtensorMap *mq, *mx;
     const FwdArgs& a;
 
@@ -485,6 +486,7 @@ template <typename T>
 struct ProbPolicy {
     static constexpr bool kInt8 = false;
     static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
+    static constexpr bool kBMn = false;
     const CUtensorMap *mq, *mx, *mg;
     const ProbArgs& a;
 
@@ -630,6 +632,7 @@ template <typename T>
 struct GradPolicy {
     static constexpr bool kInt8 = false;
     static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
+    static constexpr bool kBMn = true;
     const CUtensorMap *gk, *gmn, *xmn, *qmn, *mpart, *mdx;
     const GradArgs& a;
 
@@ -873,8 +876,8 @@ FwdPlan fwd_plan(int dtype, int64_t nq, int64_t n, int d) {
     FwdPlan p;
     const int64_t dp = up(d, 8);
     p.direct = f32_direct(dtype, nq);
-    // fp32: the planes of a piece stay in L2
-    p.rows = dtype == RDB_F32 && !p.direct ? piece_rows(n, (96LL << 20) / (6 * dp)) : up(n, 256);
+    // fp32: 256 MB of planes at a time
+    p.rows = dtype == RDB_F32 && !p.direct ? piece_rows(n, (256LL << 20) / (6 * dp)) : up(n, 256);
     p.pieces = (int)((n + p.rows - 1) / p.rows);
     p.nqb = (int)std::max<int64_t>(1, (nq + TT_M - 1) / TT_M);
     p.nkb = (d + 63) / 64;
@@ -930,11 +933,14 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
     p.planes = dtype == RDB_F32 ? 3 : 1;
     p.nseg = dtype == RDB_F32 ? 6 : 1;
     const int64_t col = std::max<int64_t>(1, nq * 2 * p.planes);  // bytes of G per row
-    // G stays in L2 (64 MB) unless that made the pieces so narrow that the
-    // partial sums of dq (read and written once a piece) cost more than they save
-    int64_t most = (64LL << 20) / col;
+    // G of a piece: 512 MB.  Pieces that stay in L2 (64 MB) have fewer tiles to
+    // deal out and more launches, and the products are bound by the tensor
+    // cores, not by reading G: 4,096 x 131,072 x 768 both gradients 2,013 us at
+    // 64 MB, 1,971 at 128, 1,924 at 256, 1,865 at 512.  At least 4,096 rows
+    // within 2 GB: the partial sums of dq are read and written once a piece.
+    int64_t most = (512LL << 20) / col;
     if (most < 4096) most = std::max(most, std::min<int64_t>(4096, (2LL << 30) / col));
-    if (dtype == RDB_F32 && !p.direct) most = std::min<int64_t>(most, (96LL << 20) / (6 * up(d, 8)));
+    if (dtype == RDB_F32 && !p.direct) most = std::min<int64_t>(most, (256LL << 20) / (6 * up(d, 8)));
     p.rows = piece_rows(n, most);
     p.pieces = (int)((n + p.rows - 1) / p.rows);
     p.nqb = (int)std::max<int64_t>(1, (nq + TT_M - 1) / TT_M);
