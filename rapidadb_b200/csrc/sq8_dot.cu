@@ -200,17 +200,11 @@ struct DotPolicy {
         __syncwarp();
     }
 
-    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
-                                         const uint32_t (&rb)[32]) const {
-        chunk(e, j, c, 0, ra);
-        chunk(e, j, c, 1, rb);
-    }
-
-    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int h,
+    __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
                                           const uint32_t (&r)[32]) const {
-        const int64_t x = static_cast<int64_t>(j.m0) + c.row, b0 = static_cast<int64_t>(j.n0) + (h ? c.col1 : c.col0);
+        const int64_t x = static_cast<int64_t>(j.m0) + c.row, b0 = static_cast<int64_t>(j.n0) + col;
         if (x >= a.n || b0 >= a.nq) return;
-        const float4* qs = reinterpret_cast<const float4*>(c.stg) + h * 8;
+        const float4* qs = reinterpret_cast<const float4*>(c.stg) + (col == c.col0 ? 0 : 8);
         char* o = reinterpret_cast<char*>(static_cast<T*>(a.out) + b0 * a.ldo + x);
         const int64_t step = a.ldo * static_cast<int64_t>(sizeof(T));
         const int valid = static_cast<int>(min(static_cast<int64_t>(32), a.nq - b0));
@@ -236,6 +230,7 @@ struct DotPolicy {
         }
     }
 
+    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
     __device__ __forceinline__ void finish(const TileCtx&) const {}
 };
 

@@ -10,7 +10,10 @@
 //
 // One CTA per SM, tiles of 128 x 128, K blocks of 64:
 //   warp 0        TMA producer of A's planes (3 boxes a stage)
-//   warp 1        TMEM (two 128-column accumulators); lane 0 issues the MMAs
+//   warp 1        TMEM; lane 0 issues the MMAs.  Two accumulators of 2 x 128
+//                 columns: the product of the largest planes, and the others, so
+//                 that the cut at every instruction (towards zero) touches the
+//                 large sum 4 times a K block and not 24
 //   warps 2..9    converters: two rows' 256 bytes per load, the next K block's
 //                 loads in flight while this one is split; P::kBMn says which
 //                 way B lies (below)
@@ -202,7 +205,7 @@ __device__ __forceinline__ void tile_loop_f32(uint8_t* smem_raw, const P& p, con
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc_t<false>(tmem_slot, 2 * TF_N);
+        tmem_alloc_t<false>(tmem_slot, 4 * TF_N);
         tmem_relinquish_t<false>();
     }
     tc_fence_before();
@@ -265,7 +268,7 @@ __device__ __forceinline__ void tile_loop_f32(uint8_t* smem_raw, const P& p, con
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * TF_N);
+                const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 2 * TF_N);
                 const uint32_t idesc = tc_idesc(true, 128, TF_N) | (j.b_mn ? 1u << 16 : 0u);
                 for (int kb = 0; kb < j.nk; ++kb) {
                     if (!mbar_try_wait(&full[stage], phase) && !mbar_wait(&full[stage], phase, abort_flag)) {
@@ -282,8 +285,8 @@ __device__ __forceinline__ void tile_loop_f32(uint8_t* smem_raw, const P& p, con
                         const uint64_t b_step = j.b_mn ? 128 : 2;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            umma_f16(d_tmem, adesc + 2 * k, bdesc + b_step * k, idesc,
-                                     (kb > 0 || g > 0 || k > 0) ? 1u : 0u);
+                            umma_f16(d_tmem + (g < 5 ? TF_N : 0), adesc + 2 * k, bdesc + b_step * k, idesc,
+                                     (kb > 0 || k > 0 || (g > 0 && g < 5)) ? 1u : 0u);
                     }
                     any = true;
                     umma_commit(&empty[stage]);
@@ -366,17 +369,26 @@ __device__ __forceinline__ void tile_loop_f32(uint8_t* smem_raw, const P& p, con
             }
             tc_fence_after();
             const uint32_t tbase =
-                tmem_base + (static_cast<uint32_t>(ctx.quad * 32) << 16) + static_cast<uint32_t>(acc * TF_N);
-            uint32_t ra[32], rb[32];
-            tmem_ld32_async(tbase + static_cast<uint32_t>(ctx.col0), ra);
-            tmem_ld32_async(tbase + static_cast<uint32_t>(ctx.col1), rb);
-            tmem_ld_wait(ra);
-            tmem_ld_wait(rb);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[acc]);
-            p.tile(epi, j, ctx, ra, rb);
-            __syncwarp();
+                tmem_base + (static_cast<uint32_t>(ctx.quad * 32) << 16) + static_cast<uint32_t>(acc * 2 * TF_N);
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                const int col = h ? ctx.col1 : ctx.col0;
+                uint32_t ra[32], rb[32];
+                tmem_ld32_async(tbase + static_cast<uint32_t>(col), ra);
+                tmem_ld32_async(tbase + static_cast<uint32_t>(TF_N + col), rb);
+                tmem_ld_wait(ra);
+                tmem_ld_wait(rb);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) ra[i] = __float_as_uint(__uint_as_float(ra[i]) + __uint_as_float(rb[i]));
+                if (h) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tempty[acc]);
+                }
+                if (col < j.nn) p.chunk(epi, j, ctx, col, ra);
+                __syncwarp();
+            }
+            p.end(epi, j, ctx);
         }
         p.finish(ctx);
     }
@@ -384,7 +396,7 @@ __device__ __forceinline__ void tile_loop_f32(uint8_t* smem_raw, const P& p, con
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_t<false>(tmem_base, 2 * TF_N);
+        tmem_dealloc_t<false>(tmem_base, 4 * TF_N);
     }
 }
 

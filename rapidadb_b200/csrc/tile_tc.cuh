@@ -33,9 +33,10 @@
 //                                  sequence in every role
 //   P::Epi                         per-thread epilogue state
 //   p.begin(epi, job, ctx)         while the tile is still being multiplied
-//   p.tile(epi, job, ctx, ra, rb)  the warp's accumulators: 32 from column
-//                                  ctx.col0 on, 32 from column ctx.col1 on
-//                                  (where the tile is that wide)
+//   p.chunk(epi, job, ctx, col, r) 32 accumulators of the warp's rows, from
+//                                  column col on (two chunks where the tile is
+//                                  that wide)
+//   p.end(epi, job, ctx)           after the tile's chunks
 //   p.finish(ctx)                  once, after the last tile
 // The epilogue's warps never wait for one another: they drift apart by up to
 // two tiles, so that one's exponentials overlap another's maxima and stores.
@@ -65,16 +66,18 @@ constexpr int TT_STG_BYTES = 4096;  // staging for 32 rows x 32 fp32 columns on 
 constexpr int TT_SMEM = TT_MAX_STAGES * TT_STAGE_BYTES + TT_BAR_BYTES + 1024;
 static_assert(TT_SMEM <= 232448, "shared memory over 227 KB");
 
-// products of planes (A plane, B plane), largest first
-__device__ constexpr int kSegA[6] = {0, 0, 1, 0, 2, 1};
-__device__ constexpr int kSegB[6] = {0, 1, 0, 2, 0, 1};
+// products of planes (A plane, B plane), the largest last: an accumulator is cut
+// (rounded towards zero) at every instruction, which costs a sum least while it
+// is small
+__device__ constexpr int kSegA[6] = {1, 2, 0, 1, 0, 0};
+__device__ constexpr int kSegB[6] = {1, 0, 2, 0, 1, 0};
 
 struct TileJob {
     const CUtensorMap *ma, *mb;  // 3-D maps: (contiguous axis, rows, planes)
     int m0, n0;                  // first row of the pair's tile, first column
     int nn;                      // columns: a multiple of 32 (64 per CTA and block when b_mn)
     int k0, nk;                  // first K block and K blocks per product
-    int nseg;                    // products of planes: 1 or 6
+    int nseg;                    // products of planes, the last of kSegA / B: 1 or 6
     bool a_mn, b_mn;
     // rows of a CTA's box where the operand is K-major (the maps' box rows, a
     // multiple of 8 up to 128).  A needs only the rows that exist: what an MMA
@@ -168,8 +171,10 @@ __device__ __forceinline__ void stg_send(const CUtensorMap* map, const void* src
     }
 }
 
+// everything sent has been written
 __device__ __forceinline__ void stg_drain(int lane) {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
 }
 
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
@@ -254,7 +259,7 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
                     2u * (j.b_mn ? static_cast<uint32_t>(b_blocks) * TT_BLOCK_BYTES
                                  : static_cast<uint32_t>(j.b_rows) * 128u);
                 for (int g = 0; g < j.nseg && ok; ++g) {
-                    const int za = kSegA[g], zb = kSegB[g];
+                    const int za = kSegA[6 - j.nseg + g], zb = kSegB[6 - j.nseg + g];
                     for (int kb = 0; kb < j.nk; ++kb) {
                         if (!mbar_try_wait(&empty[stage], phase ^ 1) &&
                             !mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
@@ -396,8 +401,11 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
             __syncwarp();
             if (lane == 0)
                 mbar_arrive_cluster_relaxed(tempty_lead + static_cast<uint32_t>(acc * sizeof(uint64_t)));
-            p.tile(epi, j, ctx, ra, rb);
+            if (ctx.col0 < j.nn) p.chunk(epi, j, ctx, ctx.col0, ra);
             __syncwarp();
+            if (ctx.col1 < j.nn) p.chunk(epi, j, ctx, ctx.col1, rb);
+            __syncwarp();
+            p.end(epi, j, ctx);
         }
         p.finish(ctx);
     }

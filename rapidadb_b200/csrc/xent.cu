@@ -37,9 +37,12 @@ namespace {
 constexpr int NT = 256;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr double kLog2e = 1.4426950408889634;
-// G is held as 2^14 (p - [n = t]): the largest value is 2^14, and an fp16
-// probability keeps its 11 bits down to 2^-28 (2^-14 without the factor).  A
-// power of two: exact for every type.
+// G is held per query as 2^14 (p - [n = t]) / (1 - p_t): the target's entry, by
+// far the largest of most rows, is -2^14 exactly, the others add up to 2^14, so
+// that rounding G to 16 bits costs dq little (rounding p_t - 1 itself doubled its
+// error) and fp16 keeps 11 bits of every entry down to 2^-28 of its row's sum.
+// What it leaves, w (1 - p_t), multiplies dq exactly and enters dx with the
+// query, rounded once there.
 constexpr float kGScale = 16384.f, kGLog2 = 14.f;
 
 inline int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
@@ -108,14 +111,13 @@ struct FwdArgs {
     const int64_t* targets;
     int groups, parts;   // epilogue groups, parts per query: slots * groups
     float2* part;        // [nq][parts] (max <q, x>, z) of each split and epilogue group
-    float* tdot;         // [nq] <q, x_t>
     unsigned* ticket;    // of the join, cleared here
 };
 
 struct FwdPolicy {
     static constexpr bool kInt8 = false;
     static constexpr int kStages = 7, kStgBytes = 0;
-    static constexpr bool kBMn = false;  // (tile_f32.cuh)
+    [[maybe_unused]] static constexpr bool kBMn = false;  // (tile_f32.cuh)
     const CUtensorMap *mq, *mx;
     const FwdArgs& a;
 
@@ -170,8 +172,8 @@ struct FwdPolicy {
     }
 
     // 32 columns from column col on: columns behind the last row count as -inf,
-    // and so does the target's, which is kept apart
-    __device__ __forceinline__ void mask(const Epi& e, const Job& j, const TileCtx& c, int col, float (&v)[32]) const {
+    // and so does the target's, whose term is kept apart
+    __device__ __forceinline__ void mask(const Epi& e, const Job& j, int col, float (&v)[32]) const {
         const int64_t c0 = static_cast<int64_t>(j.n0) + col;
         if (c0 + 32 > a.n) {
 #pragma unroll
@@ -179,8 +181,7 @@ struct FwdPolicy {
                 if (c0 + i >= a.n) v[i] = -INFINITY;
         }
         const int64_t rel = e.tgt - c0;
-        if (rel >= 0 && rel < 32 && e.tgt < a.n) {
-            a.tdot[j.m0 + c.row] = pick32(v, static_cast<int>(rel));
+        if (rel >= 0 && rel < 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
                 v[i] = i == static_cast<int>(rel) ? -INFINITY : v[i];
@@ -210,10 +211,11 @@ struct FwdPolicy {
 
     __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
                                           const uint32_t (&r)[32]) const {
+        if (j.m0 + c.row - c.lane >= a.nq) return;  // no query in this warp's 32 rows
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        mask(e, j, c, col, v);
+        mask(e, j, col, v);
         const float mx = largest(v);
         if (mx > e.m) {
             e.z *= ex2((e.m - mx) * a.c);  // 0 before the first finite value
@@ -228,11 +230,7 @@ struct FwdPolicy {
         e.z += p0 + p1;
     }
 
-    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
-                                         const uint32_t (&rb)[32]) const {
-        if (j.m0 + c.row - c.lane >= a.nq) return;  // no query in this warp's 32 rows
-        if (c.col0 < j.nn) chunk(e, j, c, c.col0, ra);
-        if (c.col1 < j.nn) chunk(e, j, c, c.col1, rb);
+    __device__ __forceinline__ void end(Epi& e, const Job& j, const TileCtx& c) const {
         const int64_t b = j.m0 + c.row;
         if (j.last && b < a.nq)
             a.part[b * a.parts + (a.slot0 + j.split) * a.groups + c.grp] = make_float2(e.m, e.z);
@@ -279,14 +277,28 @@ __device__ void reduce_losses(float* stats, const int64_t* targets, int64_t igno
     }
 }
 
-// Joins the parts of each query, one warp per query; stats and loss of each.  An
+// <q, x> of two rows by one warp: fp32 fma chains of d / 32 elements, joined
+template <typename T>
+__device__ __forceinline__ float warp_dot(const T* q, const T* x, int d, int lane) {
+    float s = 0.f;
+    for (int t = lane; t < d; t += 32) s = fmaf(to_f(q[t]), to_f(x[t]), s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
+// Joins the parts of each query, one warp per query; stats and loss of each.  The
+// target's logit is computed here, in rounded fp32: the tensor cores cut their
+// sums towards zero, which shifts the largest logits of a query alike, and only
+// the target's shift would remain in the loss (7e-6 of it at d = 768).  An
 // ignored query has loss 0; one whose target is no row is NaN throughout.  For a
 // reduced loss the last block to finish sums the losses (in index order, whoever
 // it is) and leaves the number of queries that count behind the stats; `ticket`
 // was cleared by the scan.
+template <typename T>
 __global__ void __launch_bounds__(NT)
-    xent_join_kernel(const float2* part, int parts, const float* tdot, const int64_t* targets, int64_t ignore,
-                     int64_t n, float c, int64_t nq, float* stats, float* loss, int reduction, float* total,
+    xent_join_kernel(const float2* part, int parts, const T* q, int64_t ldq, const T* x, int64_t ldx, int d,
+                     const int64_t* targets, int64_t ignore, int64_t n, float c, int64_t nq, float* stats, float* loss, int reduction, float* total,
                      unsigned* ticket) {
     __shared__ float ss[NT / 32];
     __shared__ int sc[NT / 32];
@@ -308,13 +320,13 @@ __global__ void __launch_bounds__(NT)
             join(lo_m, lo_z, lane & o ? M : m, lane & o ? Z : z, c);
             M = lo_m, Z = lo_z;
         }
+        const int64_t t = targets[b];
+        const bool ignored = t == ignore, has = t >= 0 && t < n;
+        const float td = has ? warp_dot(q + b * ldq, x + t * ldx, d, lane) : -INFINITY;
         if (lane == 0) {
-            const int64_t t = targets[b];
-            const bool ignored = t == ignore, has = t >= 0 && t < n;
             const float nan = __int_as_float(0x7fc00000);
             // Z sums 2^(c v - c M); u: the target's exponent relative to that
             const float Mc = M > -INFINITY ? M * c : 0.f;
-            const float td = has ? tdot[b] : -INFINITY;
             const float u = fmaf(td, c, -Mc);
             float m = Mc, lz, l;
             if (u >= 0.f || (has && !(M > -INFINITY))) {
@@ -358,31 +370,40 @@ __global__ void __launch_bounds__(NT)
 
 // --------------------------------------------------------------- backward --
 
-// The weight w_b of a query's loss: g[b], or for a reduced loss g[0], over the
-// number of queries for the mean (0 when none count).
-struct Weight {
+// u_b = w_b (1 - p_t) of a query, w_b the weight of its loss: g[b], or for a
+// reduced loss g[0], over the number of queries for the mean (0 when none count).
+struct Weights {
     const float* g;
-    const float* count;  // nullptr: not a mean
-    __device__ __forceinline__ float all() const {
-        return count ? (*count > 0.f ? *g / *count : 0.f) : *g;
+    const float* count;   // nullptr: not a mean
+    const float* loss;    // [nq]
+    const int64_t* targets;
+    int64_t ignore;
+    bool equal;
+    __device__ __forceinline__ float u(int64_t b) const {
+        if (targets[b] == ignore) return 0.f;
+        float w = g[equal ? 0 : b];
+        if (count) w = *count > 0.f ? w / *count : 0.f;
+        return w * -expm1f(-loss[b]);
     }
 };
 
-// largest |g_b| of the queries that count (reduction none)
-__global__ void __launch_bounds__(1024)
-    xent_wmax_kernel(const float* grad, const int64_t* targets, int64_t ignore, int64_t nq, float* wmax) {
-    __shared__ float sm[32];
+// largest |u_b|, by one block (every thread gets it); a NaN makes its own
+// products NaN
+__device__ float largest_weight(const Weights& w, int64_t nq, float* sm) {
     float mx = 0.f;
-    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x)
-        if (targets[i] != ignore) mx = fmaxf(mx, fabsf(grad[i]));  // a NaN weight makes its own products NaN
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x) mx = fmaxf(mx, fabsf(w.u(i)));
+    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mx;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 32; ++k) mx = fmaxf(mx, sm[k]);
-        *wmax = mx;
-    }
+    mx = sm[0];
+    for (int k = 1; k < static_cast<int>(blockDim.x / 32); ++k) mx = fmaxf(mx, sm[k]);
+    return mx;
+}
+
+__global__ void __launch_bounds__(1024) xent_wmax_kernel(const Weights w, int64_t nq, float* wmax) {
+    __shared__ float sm[32];
+    const float mx = largest_weight(w, nq, sm);
+    if (threadIdx.x == 0) *wmax = mx;
 }
 
 // 8 elements of a row from column t on as floats; what lies behind d is neither
@@ -424,30 +445,36 @@ __device__ __forceinline__ void store_planes(const float (&v)[8], __nv_bfloat16*
     }
 }
 
-// Queries weighted for dx = G^T (w q): out[b] = q[b] w_b / max |w|, so that the
-// type's range is used whatever the size of the gradients (equal weights: the
-// query itself, unrounded); zero rows for ignored queries, whatever they hold.
-// fp32: three bf16 planes.  grad: nullptr for equal weights.
+// Queries as an operand of dx = G^T (u q): out[b] = q[b] u_b / max |u|, so that
+// the type's range is used whatever the size of the gradients; zero rows for
+// ignored queries, whatever they hold.  fp32: three bf16 planes.  scan: every
+// block finds max |u| itself (few queries) and the first one leaves it in wmax.
 template <typename T>
 __global__ void __launch_bounds__(NT)
-    xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const int64_t* targets, int64_t ignore,
-                         const float* grad, const float* wmax, void* out, int64_t ldo) {
+    xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const Weights w, bool scan, float* wmax, void* out,
+                         int64_t ldo) {
+    __shared__ float sm[NT / 32];
+    float mx;
+    if (scan) {
+        mx = largest_weight(w, nq, sm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *wmax = mx;
+    } else {
+        mx = *wmax;
+    }
     const int64_t units = ldo / 8, total = nq * units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * NT) {
         const int64_t b = i / units;
         const int t = static_cast<int>(i - b * units) * 8;
         float v[8];
-        if (targets[b] == ignore) {
+        if (w.targets[b] == w.ignore) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = 0.f;
         } else {
             load8(q + b * ldq, t, d, v);
-            if (grad) {
-                const float f = grad[b] == 0.f ? 0.f : grad[b] / *wmax;
+            const float u = w.u(b), f = u == 0.f ? 0.f : u / mx;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] *= f;
-            }
+            for (int k = 0; k < 8; ++k) v[k] *= f;
         }
         if constexpr (sizeof(T) == 4)
             store_planes(v, static_cast<__nv_bfloat16*>(out) + b * ldo + t, nq * ldo);
@@ -481,12 +508,12 @@ struct ProbArgs {
     const float* stats;
 };
 
-// G tiles of one piece: 2^14 (p - [n = t])
+// G tiles of one piece: 2^14 (p - [n = t]) / (1 - p_t)
 template <typename T>
 struct ProbPolicy {
     static constexpr bool kInt8 = false;
     static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
-    static constexpr bool kBMn = false;
+    [[maybe_unused]] static constexpr bool kBMn = false;
     const CUtensorMap *mq, *mx, *mg;
     const ProbArgs& a;
 
@@ -514,23 +541,23 @@ struct ProbPolicy {
         }
     };
     struct Epi {
-        float m, lz, hit;
+        float m, lz;
         int64_t tgt;
-        bool ignored;
+        bool zero;  // an ignored query, one whose target is certain, or none
     };
 
     __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx& c) const {
         const int64_t b = j.m0 + c.row;
-        e.ignored = true;
+        e.zero = true;
         e.tgt = -1;
-        e.m = e.lz = e.hit = 0.f;
+        e.m = e.lz = 0.f;
         if (b >= a.nq) return;
         const int64_t t = a.targets[b];
-        e.ignored = t == a.ignore;
-        if (!e.ignored) e.tgt = t - a.row0;
+        const float rest = -expm1f(-a.stats[2 * a.nq + b]);  // 1 - p_t
+        e.zero = t == a.ignore || rest == 0.f;
+        if (!e.zero) e.tgt = t - a.row0;
         e.m = a.stats[b];
-        e.lz = a.stats[a.nq + b] - kGLog2;
-        e.hit = a.stats[2 * a.nq + b];
+        e.lz = a.stats[a.nq + b] + log2f(rest) - kGLog2;
     }
 
     __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
@@ -548,16 +575,15 @@ struct ProbPolicy {
             v[i] = ex2(x0);
             v[i + 1] = ex2(x1);
         }
-        if (e.ignored) {
+        if (e.zero) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
         }
         const int64_t rel = e.tgt - x;
         if (rel >= 0 && rel < 32) {
-            const float h = kGScale * expm1f(-e.hit);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-                v[i] = i == static_cast<int>(rel) ? h : v[i];
+                v[i] = i == static_cast<int>(rel) ? -kGScale : v[i];
         }
         __syncwarp();
         // (columns behind the piece's last row lie outside the map)
@@ -585,12 +611,7 @@ struct ProbPolicy {
         }
     }
 
-    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
-                                         const uint32_t (&rb)[32]) const {
-        if (c.col0 < j.nn) chunk(e, j, c, c.col0, ra);
-        __syncwarp();
-        if (c.col1 < j.nn) chunk(e, j, c, c.col1, rb);
-    }
+    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
     __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
 
@@ -625,27 +646,39 @@ struct GradArgs {
     int64_t lddx;
     bool dx_tma;           // the rows of dx have 16-byte strides
     float scale;
-    Weight w;              // what dx has to be multiplied with besides
+    const float* wmax;     // what dx has to be multiplied with besides
 };
 
 template <typename T>
 struct GradPolicy {
     static constexpr bool kInt8 = false;
     static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
-    static constexpr bool kBMn = true;
+    [[maybe_unused]] static constexpr bool kBMn = true;
     const CUtensorMap *gk, *gmn, *xmn, *qmn, *mpart, *mdx;
     const GradArgs& a;
 
     struct Job : TileJob {
-        bool is_dx;
+        bool is_dx, more;  // more: adds to what this CTA stored before
         int split;
     };
+    // Of fp32 operands a tile's K axis is walked in runs of 8 blocks (32 cuts of
+    // the large accumulator), added up in rounded fp32 where the result lies, by
+    // the one CTA that owns the tile.
+    static constexpr int kRun = sizeof(T) == 4 ? 8 : 1 << 30;
     struct Iter {
         const GradPolicy& p;
-        int i, step;
-        __device__ Iter(const GradPolicy& pol, int pair, int npairs) : p(pol), i(pair), step(npairs) {}
+        int i, step, left;  // K blocks of the last tile still to do
+        __device__ Iter(const GradPolicy& pol, int pair, int npairs) : p(pol), i(pair), step(npairs), left(0) {}
         __device__ __forceinline__ bool next(Job& j) {
             const GradArgs& a = p.a;
+            if (left > 0) {
+                j.more = true;
+                j.k0 += kRun;
+                j.nk = min(left, kRun);
+                left -= j.nk;
+                return true;
+            }
+            j.more = false;
             const int nqj = a.q_blocks * a.nt * a.q_split, nxj = a.x_blocks * a.nt;
             if (i >= nqj + nxj) return false;
             const int head = a.q_first ? nqj : nxj;
@@ -679,6 +712,8 @@ struct GradPolicy {
                 j.k0 = j.split * a.q_per;
                 j.nk = min(a.q_per, a.kc - j.k0);
             }
+            left = max(0, j.nk - kRun);
+            j.nk -= left;
             return true;
         }
     };
@@ -687,7 +722,7 @@ struct GradPolicy {
     };
 
     __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx&) const {
-        e.f = j.is_dx ? a.scale * (1.f / kGScale) * a.w.all() : 1.f;
+        e.f = j.is_dx ? a.scale * (1.f / kGScale) * *a.wmax : 1.f;
     }
 
     __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
@@ -705,11 +740,18 @@ struct GradPolicy {
             T* o = static_cast<T*>(a.dx) + static_cast<int64_t>(y) * a.lddx + x + c.lane;
             const int rows = static_cast<int>(min(static_cast<int64_t>(32), a.n - y));
             if (x + c.lane < a.d)
-                for (int i = 0; i < rows; ++i, o += a.lddx) *o = from_f<T>(t[i * 32 + ((c.lane + i) & 31)]);
+                for (int i = 0; i < rows; ++i, o += a.lddx) {
+                    float v = t[i * 32 + ((c.lane + i) & 31)];
+                    if (kRun < 1 << 30 && j.more) v += to_f(*o);
+                    *o = from_f<T>(v);
+                }
             __syncwarp();
             return;
         }
-        stg_wait_read(c.lane);
+        if (j.more)
+            stg_drain(c.lane);  // what is added to has been written
+        else
+            stg_wait_read(c.lane);
         bool wide = true;
         if constexpr (sizeof(T) == 2) {
             if (j.is_dx) {
@@ -732,20 +774,17 @@ struct GradPolicy {
                     make_float4(__uint_as_float(r[4 * i]) * e.f, __uint_as_float(r[4 * i + 1]) * e.f,
                                 __uint_as_float(r[4 * i + 2]) * e.f, __uint_as_float(r[4 * i + 3]) * e.f);
         }
-        if (j.is_dx)
+        if (j.is_dx && j.more)
+            stg_send<true>(mdx, c.stg, c.lane, x, y, 0);
+        else if (j.is_dx)
             stg_send<false>(mdx, c.stg, c.lane, x, y, 0);
-        else if (a.add)
+        else if (a.add || j.more)
             stg_send<true>(mpart, c.stg, c.lane, x, y, j.split);
         else
             stg_send<false>(mpart, c.stg, c.lane, x, y, j.split);
     }
 
-    __device__ __forceinline__ void tile(Epi& e, const Job& j, const TileCtx& c, const uint32_t (&ra)[32],
-                                         const uint32_t (&rb)[32]) const {
-        if (c.col0 < j.nn) chunk(e, j, c, c.col0, ra);
-        __syncwarp();
-        if (c.col1 < j.nn) chunk(e, j, c, c.col1, rb);
-    }
+    __device__ __forceinline__ void end(Epi&, const Job&, const TileCtx&) const {}
     __device__ __forceinline__ void finish(const TileCtx& c) const { stg_drain(c.lane); }
 };
 
@@ -769,11 +808,11 @@ __global__ void __launch_bounds__(TF_THREADS, 1)
     tile_loop_f32(smem_raw, p, x, st);
 }
 
-// dq_b = w_b scale 2^-14 (sum of the parts, in split order)
+// dq_b = u_b scale 2^-14 (sum of the parts, in split order)
 template <typename T>
 __global__ void __launch_bounds__(NT)
-    xent_dq_kernel(const float* part, int splits, int64_t nq, int d, int dp, const int64_t* targets, int64_t ignore,
-                   Weight w, bool equal, float scale, T* dq, int64_t lddq) {
+    xent_dq_kernel(const float* part, int splits, int64_t nq, int d, int dp, const Weights w, float scale, T* dq,
+                   int64_t lddq) {
     const int64_t units = dp / 4, total = nq * units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * NT) {
@@ -785,8 +824,8 @@ __global__ void __launch_bounds__(NT)
             const float4 v = *reinterpret_cast<const float4*>(part + (k * nq + b) * dp + t);
             s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
-        const bool skip = targets[b] == ignore;
-        const float f = (equal ? w.all() : w.g[b]) * scale * (1.f / kGScale);
+        const bool skip = w.targets[b] == w.ignore;
+        const float f = w.u(b) * scale * (1.f / kGScale);
         const float o[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -895,7 +934,6 @@ FwdPlan fwd_plan(int dtype, int64_t nq, int64_t n, int d) {
 
 struct FwdWs {
     unsigned* ticket;
-    float* tdot;
     float2* part;
     __nv_bfloat16 *qp, *xp;
     size_t bytes;
@@ -906,7 +944,6 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
     Arena a{static_cast<char*>(base)};
     const int64_t dp = up(d, 8);
     w.ticket = a.take<unsigned>(1);
-    w.tdot = a.take<float>(nq);
     w.part = a.take<float2>((size_t)p.groups * p.slots * nq);
     if (dtype == RDB_F32) {
         w.qp = a.take<__nv_bfloat16>(3 * nq * dp);
@@ -1058,16 +1095,22 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     }
     RDB_TRY(tile_smem_attr(xent_grad_kernel<T>, attr_g));
 
-    // equal weights (a reduced loss) are applied to the results
-    const bool equal = reduction != RDB_REDUCE_NONE;
-    const Weight wt{grad, reduction == RDB_REDUCE_MEAN ? stats + 3 * nq : nullptr};
+    const Weights wt{grad,
+                     reduction == RDB_REDUCE_MEAN ? stats + 3 * nq : nullptr,
+                     stats + 2 * nq,
+                     targets,
+                     ignore,
+                     reduction != RDB_REDUCE_NONE};
     if (dx) {
-        if (!equal) {
-            xent_wmax_kernel<<<1, 1024, 0, s>>>(grad, targets, ignore, nq, w.wmax);
+        const bool scan = nq <= 2048;
+        if (!scan) {
+            xent_wmax_kernel<<<1, 1024, 0, s>>>(wt, nq, w.wmax);
             RDB_LAUNCH_CHECK();
         }
-        xent_weighted_kernel<T><<<elementwise_blocks(nq * d8 / 8), NT, 0, s>>>(
-            static_cast<const T*>(q), nq, ldq, d, targets, ignore, equal ? nullptr : grad, w.wmax, w.qw, d8);
+        const int64_t items = nq * d8 / 8;
+        xent_weighted_kernel<T><<<scan ? (unsigned)std::min<int64_t>((items + NT - 1) / NT, num_sms())
+                                       : elementwise_blocks(items),
+                                  NT, 0, s>>>(static_cast<const T*>(q), nq, ldq, d, wt, scan, w.wmax, w.qw, d8);
         RDB_LAUNCH_CHECK();
     }
     Planes qo;
@@ -1100,7 +1143,7 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     ga.lddx = lddx;
     ga.dx_tma = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (lddx * (int64_t)sizeof(T)) % 16 == 0;
     ga.scale = scale;
-    ga.w = equal ? wt : Weight{w.wmax, nullptr};
+    ga.wmax = w.wmax;
     const Planes go{w.g, p.rows, nq * p.rows, p.planes};
     CUtensorMap mpart = mq, mdx = mq;  // (any valid map where there is nothing to store)
     if (dq)
@@ -1164,8 +1207,7 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         RDB_LAUNCH_CHECK();
     }
     if (dq) {
-        xent_dq_kernel<T><<<elementwise_blocks(nq * p.dp / 4), NT, 0, s>>>(w.part, p.q_split, nq, d, p.dp, targets,
-                                                                           ignore, wt, equal, scale,
+        xent_dq_kernel<T><<<elementwise_blocks(nq * p.dp / 4), NT, 0, s>>>(w.part, p.q_split, nq, d, p.dp, wt, scale,
                                                                            static_cast<T*>(dq), lddq);
         RDB_LAUNCH_CHECK();
     }
@@ -1221,7 +1263,6 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
         a.parts = p.slots * p.groups;
         a.part = w.part;
         a.ticket = w.ticket;
-        a.tdot = w.tdot;
         for (int i = 0; i < p.pieces; ++i) {
             const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
             a.n = rows;
@@ -1243,9 +1284,20 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
             }
             RDB_LAUNCH_CHECK();
         }
-        xent_join_kernel<<<(unsigned)std::min<int64_t>((nq + NT / 32 - 1) / (NT / 32), 16LL * num_sms()), NT, 0, s>>>(
-            w.part, p.slots * p.groups, w.tdot, targets, ignore_index, n, c, nq, stats, loss, reduction, loss,
-            w.ticket);
+        const unsigned blocks = (unsigned)std::min<int64_t>((nq + NT / 32 - 1) / (NT / 32), 16LL * num_sms());
+        const int parts = p.slots * p.groups;
+        if (dtype == RDB_F32)
+            xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const float*>(q), ldq,
+                                                   static_cast<const float*>(x), ldx, d, targets, ignore_index, n, c, nq,
+                                                   stats, loss, reduction, loss, w.ticket);
+        else if (dtype == RDB_F16)
+            xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const __half*>(q), ldq,
+                                                   static_cast<const __half*>(x), ldx, d, targets, ignore_index, n, c, nq,
+                                                   stats, loss, reduction, loss, w.ticket);
+        else
+            xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const __nv_bfloat16*>(q), ldq,
+                                                   static_cast<const __nv_bfloat16*>(x), ldx, d, targets, ignore_index, n,
+                                                   c, nq, stats, loss, reduction, loss, w.ticket);
         RDB_LAUNCH_CHECK();
     } else if (reduction != RDB_REDUCE_NONE) {
         xent_reduce_kernel<<<1, NT, 0, s>>>(targets, ignore_index, nq, reduction, stats, loss);

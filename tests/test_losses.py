@@ -13,15 +13,16 @@ of the storage type (bf16 2^-8, fp16 2^-11, fp32 2^-24):
   values of the size of 1 + loss:
   dl = 2 ds + (n + 16 + 4 max|s|) u32 (1 + loss).
 * G = g scale (p - [n = t]) is off by |G| (2 ds + (n + 16 + 4 max|s|) u32)
-  relative to p, and to p_t - 1 = expm1(-loss); it is rounded to the storage
-  type once, and for dx the weighted query once more; a product over k terms
-  adds k u32 of the sum of absolute values:
+  relative to p, and to p_t - 1 = expm1(-loss); over 1 - p_t it is rounded to
+  the storage type once, and for dx the query, times its weight and 1 - p_t, once
+  more; a product over k terms adds k u32 of the sum of absolute values:
   dq: (u + dp + n u32) (|G| @ |x|) + u |dq|,
   dx: (2 u + dp + nq u32) (|G|^T @ |q|) + u |dx|.
 * what underflows fp32 is off by up to 2^-126 a term: at most 2^12 terms of
   weight up to 2^10 (scale times an element) here, so 2^-104 in all.
 * fp16 rounds below its normal range in steps of 2^-24: G is held as
-  2^14 (p - [n = t]), the weighted query relative to the largest weight.
+  2^14 (p - [n = t]) / (1 - p_t), the weighted query relative to the largest
+  w (1 - p_t).
 """
 import ctypes
 import os
@@ -84,14 +85,15 @@ class Ref:
         self.tol_loss = torch.where(keep, 2 * ds + rel * (1 + self.loss) + UNDERFLOW, torch.zeros_like(self.loss))
         # steps of 2^-24 below fp16's normal range
         sub = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
-        wmax = w.abs().max().item()
+        rest = -torch.expm1(-self.loss)  # 1 - p_t
+        u_b = w * rest
         subG = sub * 2.0 ** -14 * scale
         self.tol_dq = 1.01 * ((u + dp + n * U32) * (G.abs() @ xd.abs()) + u * self.dq.abs() +
-                              subG * w[:, None] * xd.abs().sum(0)[None, :]) + sub + UNDERFLOW
-        pg = p.abs() * scale
+                              subG * u_b[:, None] * xd.abs().sum(0)[None, :]) + sub + UNDERFLOW
+        pg = torch.where(rest[:, None] > 0, p.abs() / rest[:, None], torch.zeros_like(p)) * scale * keep[:, None]
         self.tol_dx = 1.01 * ((2 * u + dp + nq * U32) * (G.abs().T @ qd.abs()) + u * self.dx.abs() +
-                              subG * (w[:, None] * qd.abs()).sum(0)[None, :] +
-                              sub * wmax * pg.sum(0)[:, None]) + sub + UNDERFLOW
+                              subG * (u_b[:, None] * qd.abs()).sum(0)[None, :] +
+                              sub * u_b.abs().max().item() * pg.sum(0)[:, None]) + sub + UNDERFLOW
 
 
 def within(got, want, tol, what):
