@@ -263,8 +263,13 @@ __device__ void reduce_losses(float* stats, const int64_t* targets, int64_t igno
                               float* total, float* ss, int* sc) {
     float s = 0.f;
     int cnt = 0;
-    for (int64_t i = threadIdx.x; i < nq; i += NT)
-        if (targets[i] != ignore) s += __ldcg(stats + 2 * nq + i), ++cnt;
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < nq; i += NT) {
+        const float l = __ldcg(stats + 2 * nq + i);
+        const bool counts = targets[i] != ignore;
+        s += counts ? l : 0.f;
+        cnt += counts;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     cnt = __reduce_add_sync(0xffffffffu, cnt);
@@ -277,14 +282,42 @@ __device__ void reduce_losses(float* stats, const int64_t* targets, int64_t igno
     }
 }
 
-// <q, x> of two rows by one warp: fp32 fma chains of d / 32 elements, joined
+// 8 elements of a row from column t on as floats; what lies behind d is neither
+// read nor kept
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int t, int d, float (&v)[8]) {
+    if (t + 8 <= d) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(row + t), b = *reinterpret_cast<const float4*>(row + t + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(row + t);
+            const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = t + i < d ? to_f(row[t + i]) : 0.f;
+    }
+}
+
+// <q, x> of two rows by one warp: 8 fp32 fma chains a lane, joined
 template <typename T>
 __device__ __forceinline__ float warp_dot(const T* q, const T* x, int d, int lane) {
-    float s = 0.f;
-    for (int t = lane; t < d; t += 32) s = fmaf(to_f(q[t]), to_f(x[t]), s);
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int t = lane * 8; t < d; t += 256) {
+        float a[8], b[8];
+        load8(q, t, d, a);
+        load8(x, t, d, b);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
+        for (int i = 0; i < 8; ++i) s[i] = fmaf(a[i], b[i], s[i]);
+    }
+    float v = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 // Joins the parts of each query, one warp per query; stats and loss of each.  The
@@ -306,6 +339,9 @@ __global__ void __launch_bounds__(NT)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int64_t b = static_cast<int64_t>(blockIdx.x) * (NT / 32) + warp; b < nq;
          b += static_cast<int64_t>(gridDim.x) * (NT / 32)) {
+        const int64_t t = targets[b];
+        const bool ignored = t == ignore, has = t >= 0 && t < n;
+        const float td = has ? warp_dot(q + b * ldq, x + t * ldx, d, lane) : -INFINITY;
         float M = -INFINITY, Z = 0.f;
 #pragma unroll 4
         for (int s = lane; s < parts; s += 32) {
@@ -320,9 +356,6 @@ __global__ void __launch_bounds__(NT)
             join(lo_m, lo_z, lane & o ? M : m, lane & o ? Z : z, c);
             M = lo_m, Z = lo_z;
         }
-        const int64_t t = targets[b];
-        const bool ignored = t == ignore, has = t >= 0 && t < n;
-        const float td = has ? warp_dot(q + b * ldq, x + t * ldx, d, lane) : -INFINITY;
         if (lane == 0) {
             const float nan = __int_as_float(0x7fc00000);
             // Z sums 2^(c v - c M); u: the target's exponent relative to that
@@ -391,6 +424,7 @@ struct Weights {
 // products NaN
 __device__ float largest_weight(const Weights& w, int64_t nq, float* sm) {
     float mx = 0.f;
+#pragma unroll 4
     for (int64_t i = threadIdx.x; i < nq; i += blockDim.x) mx = fmaxf(mx, fabsf(w.u(i)));
     mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mx;
@@ -404,26 +438,6 @@ __global__ void __launch_bounds__(1024) xent_wmax_kernel(const Weights w, int64_
     __shared__ float sm[32];
     const float mx = largest_weight(w, nq, sm);
     if (threadIdx.x == 0) *wmax = mx;
-}
-
-// 8 elements of a row from column t on as floats; what lies behind d is neither
-// read nor kept
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int t, int d, float (&v)[8]) {
-    if (t + 8 <= d) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(row + t), b = *reinterpret_cast<const float4*>(row + t + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(row + t);
-            const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = t + i < d ? to_f(row[t + i]) : 0.f;
-    }
 }
 
 // the three bf16 planes of 8 floats, plane stride in elements
