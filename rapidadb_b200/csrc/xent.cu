@@ -320,34 +320,39 @@ __device__ __forceinline__ float warp_dot(const T* q, const T* x, int d, int lan
     return v;
 }
 
-// Joins the parts of each query, one warp per query; stats and loss of each.  The
-// target's logit is computed here, in rounded fp32: the tensor cores cut their
-// sums towards zero, which shifts the largest logits of a query alike, and only
-// the target's shift would remain in the loss (7e-6 of it at d = 768).  An
-// ignored query has loss 0; one whose target is no row is NaN throughout.  For a
-// reduced loss the last block to finish sums the losses (in index order, whoever
-// it is) and leaves the number of queries that count behind the stats; `ticket`
-// was cleared by the scan.
+// Joins the parts of each query, by one warp, or by a whole block where there are
+// no more queries than SMs (wide); stats and loss of each.
+// The target's logit is computed here, in rounded fp32: the tensor cores cut
+// their sums towards zero, which shifts the largest logits of a query alike, and
+// only the target's shift would remain in the loss (7e-6 of it at d = 768).
+// An ignored query has loss 0; one whose target is no row is NaN throughout.
+// For a reduced loss the last block to finish sums the losses (in index order,
+// whoever it is) and leaves the number of queries that count behind the stats;
+// `ticket` was cleared by the scan.
 template <typename T>
 __global__ void __launch_bounds__(NT)
     xent_join_kernel(const float2* part, int parts, const T* q, int64_t ldq, const T* x, int64_t ldx, int d,
-                     const int64_t* targets, int64_t ignore, int64_t n, float c, int64_t nq, float* stats, float* loss, int reduction, float* total,
-                     unsigned* ticket) {
+                     const int64_t* targets, int64_t ignore, int64_t n, float c, int64_t nq, bool wide, float* stats,
+                     float* loss, int reduction, float* total, unsigned* ticket) {
+    __shared__ float2 sj[NT / 32];
     __shared__ float ss[NT / 32];
     __shared__ int sc[NT / 32];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t b = static_cast<int64_t>(blockIdx.x) * (NT / 32) + warp; b < nq;
-         b += static_cast<int64_t>(gridDim.x) * (NT / 32)) {
-        const int64_t t = targets[b];
+    const int per = wide ? 1 : NT / 32;  // queries per block and step
+    for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * per; b0 < nq; b0 += static_cast<int64_t>(gridDim.x) * per) {
+        const int64_t b = wide ? b0 : b0 + warp;
+        const bool mine = b < nq && (!wide || warp == 0);  // the warp that finishes the query
+        const int64_t t = b < nq ? targets[b] : -1;
         const bool ignored = t == ignore, has = t >= 0 && t < n;
-        const float td = has ? warp_dot(q + b * ldq, x + t * ldx, d, lane) : -INFINITY;
+        const float td = mine && has ? warp_dot(q + b * ldq, x + t * ldx, d, lane) : -INFINITY;
         float M = -INFINITY, Z = 0.f;
+        if (b < nq)
 #pragma unroll 4
-        for (int s = lane; s < parts; s += 32) {
-            const float2 v = part[b * parts + s];
-            join(M, Z, v.x, v.y, c);
-        }
+            for (int s = wide ? threadIdx.x : lane; s < parts; s += wide ? NT : 32) {
+                const float2 v = part[b * parts + s];
+                join(M, Z, v.x, v.y, c);
+            }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const float m = __shfl_xor_sync(0xffffffffu, M, o), z = __shfl_xor_sync(0xffffffffu, Z, o);
@@ -356,7 +361,14 @@ __global__ void __launch_bounds__(NT)
             join(lo_m, lo_z, lane & o ? M : m, lane & o ? Z : z, c);
             M = lo_m, Z = lo_z;
         }
-        if (lane == 0) {
+        if (wide) {
+            if (lane == 0) sj[warp] = make_float2(M, Z);
+            __syncthreads();
+            for (int k = 1; k < NT / 32; ++k)
+                if (warp == 0) join(M, Z, sj[k].x, sj[k].y, c);
+            __syncthreads();
+        }
+        if (lane == 0 && mine) {
             const float nan = __int_as_float(0x7fc00000);
             // Z sums 2^(c v - c M); u: the target's exponent relative to that
             const float Mc = M > -INFINITY ? M * c : 0.f;
@@ -1298,20 +1310,21 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
             }
             RDB_LAUNCH_CHECK();
         }
-        const unsigned blocks = (unsigned)std::min<int64_t>((nq + NT / 32 - 1) / (NT / 32), 16LL * num_sms());
+        const bool wide = nq <= num_sms();
+        const unsigned blocks = (unsigned)std::min<int64_t>(wide ? nq : (nq + NT / 32 - 1) / (NT / 32), 16LL * num_sms());
         const int parts = p.slots * p.groups;
         if (dtype == RDB_F32)
             xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const float*>(q), ldq,
-                                                   static_cast<const float*>(x), ldx, d, targets, ignore_index, n, c, nq,
+                                                   static_cast<const float*>(x), ldx, d, targets, ignore_index, n, c, nq, wide,
                                                    stats, loss, reduction, loss, w.ticket);
         else if (dtype == RDB_F16)
             xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const __half*>(q), ldq,
-                                                   static_cast<const __half*>(x), ldx, d, targets, ignore_index, n, c, nq,
+                                                   static_cast<const __half*>(x), ldx, d, targets, ignore_index, n, c, nq, wide,
                                                    stats, loss, reduction, loss, w.ticket);
         else
             xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const __nv_bfloat16*>(q), ldq,
                                                    static_cast<const __nv_bfloat16*>(x), ldx, d, targets, ignore_index, n,
-                                                   c, nq, stats, loss, reduction, loss, w.ticket);
+                                                   c, nq, wide, stats, loss, reduction, loss, w.ticket);
         RDB_LAUNCH_CHECK();
     } else if (reduction != RDB_REDUCE_NONE) {
         xent_reduce_kernel<<<1, NT, 0, s>>>(targets, ignore_index, nq, reduction, stats, loss);
