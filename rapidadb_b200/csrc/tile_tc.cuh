@@ -4,17 +4,17 @@
 // A CTA pair (cluster of 2, cta_group::2) computes one 256 x nn tile after the
 // other, nn <= 256, D = sum_k A[m, k] B[n, k]:
 //   warp 0      TMA producer: per K block of 128 bytes each CTA loads its 128
-//               rows of A and its nn / 2 rows of B into a ring of 5 or more
-//               stages.
+//               rows of A and its nn / 2 rows of B into a ring of 5 to 7 stages
+//               (4 to 6 measure the same where the MMAs bound the tile).
 //   warp 1      TMEM (two 256-column accumulators); the leader's lane 0 issues
 //               the MMAs and commits stage releases and finished accumulators.
 //   warps 2..17 epilogue, four per TMEM lane quadrant: a thread owns one row of
 //               its CTA's 128 and every fourth 32-column chunk of the tile (at
 //               most two).  It takes both into registers and releases the
 //               accumulator before it works on them, so the MMAs run up to two
-//               tiles ahead.  (Eight warps with one chunk in flight left the
-//               MMAs waiting: 4,096 x 131,072 x 128 forward 306 us, 137 us
-//               with no epilogue at all.)
+//               tiles ahead.  (4,096 x 131,072 x 128 forward: 219 us, 306 with
+//               eight warps and one chunk in flight, 137 with no epilogue at
+//               all; at d = 768 586, 613 and 556 us.)
 // An operand lies either K-major in memory (a row's K elements contiguous: one
 // box of 128 bytes x 128 rows per stage) or MN-major (the rows' index
 // contiguous: boxes of 64 elements x 64 K rows).  Both use the 128-byte

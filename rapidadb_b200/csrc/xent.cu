@@ -2,26 +2,31 @@
 //
 //   s_bn   = scale <q_b, x_n>                  (the [nq, n] matrix is never kept)
 //   loss_b = log sum_n exp(s_bn) - s_b,t(b)    (0 where t(b) == ignore_index)
-//   G_bn   = g_b scale (exp(s_bn) / sum_n exp(s_bn) - [n = t(b)])
+//   G_bn   = w_b scale (p_bn - [n = t(b)]),    p_bn = exp(s_bn) / sum_n exp(s_bn)
 //   dq = G x,  dx = G^T q
 //
-// Every product runs on the tcgen05 tile loop of tile_tc.cuh.
+// Every product runs on the tcgen05 tile loops of tile_tc.cuh and tile_f32.cuh.
 //
 // Forward: one pass over the rows.  The sum is taken in base 2 around a running
-// maximum in the epilogue of each 256 x 256 tile, c = scale log2 e,
+// maximum in the epilogue of each tile, c = scale log2 e,
 //   m = max_n c <q, x_n>,   z = sum_n 2^(c <q, x_n> - m),
 // held in fp32, one (m, z) per query, row split and epilogue group, joined by
 // xent_join_kernel.  The target's own term stays out of the running sum: with
 // r = the sum of the other terms relative to the target's, loss = log1p(r), so
-// a query that finds its row keeps a loss near 0, and its p - 1 = expm1(-loss),
+// a query that finds its row keeps a loss near 0, and its 1 - p = -expm1(-loss),
 // to full precision.
 //
-// Backward: the rows in pieces of C.  Per piece one launch recomputes the
-// logits and writes G / (g_b scale) = p - [n = t] as a [nq, C] workspace in the
-// operands' type (at most 512 MB), one launch multiplies
-// it both ways: dx rows directly (K = nq), dq into fp32 partial sums (K = C,
-// split over several tiles when there are few queries), joined at the end.
-// No atomics: every sum has a fixed order.
+// Backward: the rows in pieces.  Per piece one launch recomputes the logits and
+// writes a [nq, rows] workspace of G in the operands' type, every row of it over
+// its 1 - p_t (at most 512 MB), one launch multiplies it both ways: dx rows
+// directly (K = nq), dq into fp32 partial sums (K = rows, split over several
+// tiles when there are few queries), joined at the end.  No atomics on values:
+// every sum has a fixed order.
+//
+// Bound: the products, 2 nq n d FLOP each, one forward and three backward.  4,096
+// queries, 131,072 rows, d = 768, bf16: forward 578 us (1.43 PFLOP/s, the rate
+// cuBLAS holds for seconds is 1.40), probabilities 620, gradients 1,218.  Few
+// queries: the rows' bytes, 1 x 1M x 768 bf16 230 us (6.6 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

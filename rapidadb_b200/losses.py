@@ -39,8 +39,9 @@ def softmax_cross_entropy(queries: torch.Tensor, database: torch.Tensor, targets
     The loss is float32; gradients have their tensor's dtype.  Gradients are
     computed only for the inputs that require them, in a fixed order of sums
     (the same call gives the same bits), and once: a backward pass with
-    ``create_graph=True`` raises.  To capture a step into a CUDA graph, take the
-    gradients with ``torch.autograd.grad`` of leaves made inside the capture.
+    ``create_graph=True`` raises.  To capture a step into a CUDA graph, run it
+    once before, and take the gradients with ``torch.autograd.grad`` of leaves
+    made inside the capture.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
