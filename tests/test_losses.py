@@ -487,6 +487,87 @@ def test_captured_steps(device, dtype):
         want = step()
 
 
+def relative(got, want):
+    return ((got.double().cpu() - want).norm() / want.norm()).item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,n,d", [(40, 3000, 768), (100, 20000, 256), (300, 4000, 512)])
+@pytest.mark.parametrize("dtype", sorted(DT))
+def test_errors_in_norm(device, nq, n, d, dtype):
+    """Errors of whole results, much below the elementwise worst cases.  A loss
+    is the sum of n terms, each off by the cut of its logit (half a step of 2^-24
+    per instruction, d / 16 of them, on logits of about one tenth of the scale)
+    and a few roundings: 2^-20 covers them four times over.  fp32 gradients are
+    sums of such terms: 2^-18.  16-bit gradients round G and the query besides the
+    result, independently: sqrt(3) roundings, of 0.41 half steps in the mean."""
+    q, x, t, w = make(nq, n, d, DT[dtype], seed=3)
+    r = Ref(q, x, t, 20.0, w)
+    loss, dq, dx = run_all(q, x, t, w)
+    assert relative(loss, r.loss) < 2.0 ** -20
+    bound = 2.0 ** -18 if dtype == "fp32" else half_step(DT[dtype])
+    assert relative(dq, r.dq) < bound and relative(dx, r.dx) < bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [3, 150])
+def test_offsets_past_32_bits(device, nq):
+    """More than 2^31 elements of rows: losses, and the gradients of queries and
+    of rows at the end, in the middle and next to the 2^31st element."""
+    n, d = 2_900_000, 768
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(n, d, dtype=torch.bfloat16, device=device)
+    for part in x.split(500_000):
+        part.copy_(torch.randn(part.shape, generator=g, device=device) / d ** 0.5)
+    edge = 2 ** 31 // d
+    t = torch.randint(0, n, (nq,), generator=g, device=device)
+    t[0], t[1], t[2] = n - 1, edge, edge + 1
+    q = (x[t].float() + 0.05 * torch.randn(nq, d, generator=g, device=device)).to(torch.bfloat16)
+    qd, xd = q.clone().requires_grad_(), x.requires_grad_()
+    loss = loss_fn(qd, xd, t, scale=10.0, reduction="none")
+    dq, dx = torch.autograd.grad(loss, (qd, xd), torch.ones_like(loss))
+    x = x.detach()
+    lse = torch.full((nq,), -float("inf"), dtype=torch.float64, device=device)
+    for part in x.split(100_000):
+        lse = torch.logaddexp(lse, torch.logsumexp(10.0 * q.double() @ part.double().T, 1))
+    want = lse - 10.0 * (q.double() * x[t].double()).sum(1)
+    assert ((loss.double() - want).abs() <= 1e-4 * want).all()
+    ref = torch.zeros(nq, d, dtype=torch.float64, device=device)
+    for i, part in enumerate(x.split(100_000)):
+        p = torch.exp(10.0 * q.double() @ part.double().T - lse[:, None])
+        own = (t >= i * 100_000) & (t < i * 100_000 + len(part))
+        p[own.nonzero()[:, 0], t[own] - i * 100_000] -= 1.0
+        ref += 10.0 * p @ part.double()
+    assert relative(dq, ref.cpu()) < 2.0 ** -7
+    for lo, hi in ((0, 300), (edge - 150, edge + 150), (n - 300, n)):
+        p = torch.exp(10.0 * q.double() @ x[lo:hi].double().T - lse[:, None])
+        own = (t >= lo) & (t < hi)
+        p[own.nonzero()[:, 0], t[own] - lo] -= 1.0
+        assert relative(dx[lo:hi], (10.0 * p.T @ q.double()).cpu()) < 2.0 ** -7, (lo, hi)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DT))
+def test_two_threads_at_once(device, dtype):
+    from concurrent.futures import ThreadPoolExecutor
+
+    cases = [make(150, 900, 96, DT[dtype], seed=s) for s in (1, 2)]
+    want = [run_all(*c) for c in cases]
+    torch.cuda.synchronize()
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got = [run_all(*cases[i]) for _ in range(8)]
+        s.synchronize()
+        return got
+
+    with ThreadPoolExecutor(2) as ex:
+        for i, runs in enumerate(ex.map(work, (0, 1))):
+            for got in runs:
+                assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+
+
 @pytest.mark.gpu
 def test_train_quantise_score(device):
     """The operators together: a step of training queries and rows, the rows

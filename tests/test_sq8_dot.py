@@ -68,6 +68,23 @@ def test_abi_refusals_without_gpu():
     assert f(None, None, 0, 16, None, None, 4, 16, 16, 0, None, 4, None) == 0  # nothing to do
 
 
+def test_row_copy_refusals_without_gpu():
+    import ctypes
+    import os
+
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(__file__), "..", "rapidadb_b200", "librdb_kernels.so"))
+    lib.rdb_last_error.restype = ctypes.c_char_p
+    i64, vp = ctypes.c_int64, ctypes.c_void_p
+    f = lib.rdb_pad_rows
+    f.argtypes = [vp, i64, i64, i64, vp, i64, vp]
+    for a, msg in [((1 << 20, -1, 5, 5, 1 << 21, 16), b"shape"), ((1 << 20, 3, 0, 5, 1 << 21, 16), b"shape"),
+                   ((1 << 20, 3, 5, 5, 1 << 21, 24), b"multiples of 16"), ((1 << 20, 3, 17, 17, 1 << 21, 16), b"multiples"),
+                   ((1 << 20, 3, 5, 5, (1 << 21) + 8, 16), b"multiples"), ((None, 3, 5, 5, 1 << 21, 16), b"NULL"),
+                   ((1 << 20, 3, 5, 5, None, 16), b"NULL")]:
+        assert f(*a, None) == 1 and msg in lib.rdb_last_error(), (a, lib.rdb_last_error())
+    assert f(None, 0, 5, 5, None, 16, None) == 0
+
+
 @pytest.mark.gpu
 def test_refusals(device):
     C = _C()
@@ -253,6 +270,61 @@ def test_graph_stream_and_two_captures(device, nq):
     torch.cuda.synchronize()
     for o in outs:
         check(o, qc2, qs, xc, xs, torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 5])
+def test_codes_past_32_bits(device, nq):
+    n, d = 2_900_000, 768
+    g = torch.Generator(device="cuda").manual_seed(1)
+    xc = torch.empty(n, d, dtype=torch.int8, device=device)
+    for part in xc.split(500_000):
+        part.copy_(torch.randint(-127, 128, part.shape, generator=g, device=device, dtype=torch.int8))
+    qc = torch.randint(-127, 128, (nq, d), generator=g, device=device, dtype=torch.int8)
+    qs, xs = torch.rand(nq, generator=g, device=device) + 0.1, torch.rand(n, generator=g, device=device) + 0.1
+    out = _C().sq8_dot_product(qc, qs, xc, xs)
+    for i in range(0, n, 500_000):
+        acc = qc.double() @ xc[i:i + 500_000].double().T
+        ref = acc * (qs.double()[:, None] * xs[i:i + 500_000].double()[None, :])
+        assert ((out[:, i:i + 500_000].double() - ref).abs() <= 3.01 * U32 * ref.abs()).all(), i
+
+
+@pytest.mark.gpu
+def test_scores_past_32_bits(device):
+    """More than 2^31 scores."""
+    nq, n, d = 750, 2_900_000, 16
+    g = torch.Generator(device="cuda").manual_seed(2)
+    xc = torch.randint(-127, 128, (n, d), generator=g, device=device, dtype=torch.int8)
+    qc = torch.randint(-127, 128, (nq, d), generator=g, device=device, dtype=torch.int8)
+    qs, xs = torch.rand(nq, generator=g, device=device) + 0.1, torch.rand(n, generator=g, device=device) + 0.1
+    out = _C().sq8_dot_product(qc, qs, xc, xs, torch.bfloat16)
+    for b in (0, 3, 739, 740, 741, 749):
+        ref = (qc[b].double() @ xc.double().T) * (qs[b].double() * xs.double())
+        assert ((out[b].double() - ref).abs() <= (3.01 * U32 + 2.0 ** -8) * ref.abs()).all(), b
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once(device):
+    from concurrent.futures import ThreadPoolExecutor
+
+    rng = np.random.default_rng(8)
+    cases = []
+    for nq in (2, 300):
+        qc, qs = codes_of(rng, nq, 200)
+        xc, xs = codes_of(rng, 1500, 200)
+        cases.append([t.to(device) for t in (qc, qs, xc, xs)])
+    want = [_C().sq8_dot_product(*c) for c in cases]
+    torch.cuda.synchronize()
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got = [_C().sq8_dot_product(*cases[i]) for _ in range(20)]
+        s.synchronize()
+        return all(torch.equal(g, want[i]) for g in got)
+
+    with ThreadPoolExecutor(2) as ex:
+        assert all(ex.map(work, (0, 1)))
 
 
 @pytest.mark.gpu
