@@ -32,7 +32,7 @@ Rows aligned_rows(const at::Tensor& src) {
     check_status(rdb_pad_rows(s.data_ptr(), rows, cols * e, (rows <= 1 ? cols : s.stride(0)) * e, out.data_ptr(),
                               ldp * e, stream_ptr()),
                  "row copy");
-    return {out, ldp};
+    return {out.narrow(1, 0, cols), ldp};
 }
 
 void check_matrix(const at::Tensor& t, const char* name) {
@@ -81,6 +81,11 @@ void check_operands(const at::Tensor& queries, const at::Tensor& database, const
     check_matrix(database, "database");
     check_same_device(queries, database, "database");
     check_same_device(queries, targets, "targets");
+}
+
+void check_stats(const at::Tensor& stats, int64_t nq) {
+    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.dim() == 1 && stats.size(0) == 3 * nq + 1,
+                "stats must be float32 [3 * batch + 1]");
 }
 
 at::Tensor scratch(size_t bytes, const at::Tensor& like) {
@@ -166,7 +171,9 @@ Result run_backward(const XentArgs& a, const at::Tensor& grad, const at::Tensor&
 }
 
 // The autograd node.  It keeps the operands as the kernels read them (the
-// inputs themselves, or their padded copies) and the forward's statistics.
+// inputs themselves, or their padded copies) and the forward's statistics.  What
+// comes back may lie elsewhere and in other strides (saved-tensor hooks: offloaded
+// to the host, packed), so the backward pass looks at it afresh.
 struct XentLoss : torch::autograd::Function<XentLoss> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& queries,
                               const at::Tensor& database, const at::Tensor& targets, double scale,
@@ -174,7 +181,7 @@ struct XentLoss : torch::autograd::Function<XentLoss> {
         const XentArgs a = xent_args(queries, database, targets);
         Result r = run_forward(a, queries.options(), scale, ignore_index, static_cast<int>(reduction));
         ctx->save_for_backward({a.q.t, a.x.t, a.t, std::get<1>(r)});
-        ctx->saved_data["call"] = std::vector<int64_t>{a.d, a.q.ld, a.x.ld, ignore_index, reduction};
+        ctx->saved_data["call"] = std::vector<int64_t>{ignore_index, reduction};
         ctx->saved_data["scale"] = scale;
         return std::get<0>(r);
     }
@@ -184,18 +191,13 @@ struct XentLoss : torch::autograd::Function<XentLoss> {
         TORCH_CHECK(!at::GradMode::is_enabled(), "softmax_cross_entropy has no second derivative (create_graph=True)");
         const auto saved = ctx->get_saved_variables();
         const auto call = ctx->saved_data["call"].toIntVector();
-        XentArgs a;
-        a.q = {saved[0], call[1]};
-        a.x = {saved[1], call[2]};
-        a.t = saved[2];
-        a.nq = saved[0].size(0);
-        a.n = saved[1].size(0);
-        a.d = call[0];
-        a.dtype = dtype_code(saved[0].scalar_type());
+        check_operands(saved[0], saved[1], saved[2]);
+        check_same_device(saved[0], saved[3], "stats");
         c10::cuda::CUDAGuard guard(saved[0].device());
-        check_pending_status();
-        const Result r = run_backward(a, grads[0], saved[3], ctx->saved_data["scale"].toDouble(), call[3],
-                                      static_cast<int>(call[4]), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+        const XentArgs a = xent_args(saved[0], saved[1], saved[2]);
+        check_stats(saved[3], a.nq);
+        const Result r = run_backward(a, grads[0], saved[3].contiguous(), ctx->saved_data["scale"].toDouble(), call[0],
+                                      static_cast<int>(call[1]), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
         return {std::get<0>(r), std::get<1>(r), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     }
 };
@@ -226,8 +228,7 @@ Result softmax_cross_entropy_backward(const at::Tensor& grad, const at::Tensor& 
     c10::cuda::CUDAGuard guard(queries.device());
     at::NoGradGuard no_grad;
     const XentArgs a = xent_args(queries, database, targets);
-    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.dim() == 1 && stats.size(0) == 3 * a.nq + 1,
-                "stats must be float32 [3 * batch + 1]");
+    check_stats(stats, a.nq);
     TORCH_CHECK(reduction == RDB_REDUCE_NONE ? grad.dim() == 1 && grad.size(0) == a.nq : grad.numel() == 1,
                 "grad must have the shape of the loss");
     return run_backward(a, grad, stats.contiguous(), scale, ignore_index, reduction, need_queries, need_database);

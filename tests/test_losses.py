@@ -417,6 +417,49 @@ def test_strides_and_bases(device, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("d", [64, 37])
+def test_saved_tensors_that_come_back_elsewhere(device, d, dtype):
+    """Hooks on the saved tensors return them in other memory and other
+    strides (offloaded to the host and back, transposed, at odd bases): the
+    gradients stay the same."""
+    g = torch.Generator().manual_seed(4)
+    qw = torch.randn(40, 96, generator=g).to(DT[dtype]).to(device)
+    xw = torch.randn(300, 96, generator=g).to(DT[dtype]).to(device)
+    q, x = qw[:, :d], xw[::2, 8:8 + d]
+    t, w = torch.randint(0, 150, (40,), generator=g).to(device), torch.rand(40, generator=g).to(device)
+    want = run_all(q.detach(), x.detach(), t, w)
+
+    def transposed(v):
+        return v.t().contiguous().t() if v.dim() == 2 else v.repeat_interleave(2)[::2]
+
+    def odd_base(v):
+        out = torch.empty(v.numel() + 1, dtype=v.dtype, device=v.device)[1:].view(v.shape)
+        return out.copy_(v)
+
+    hooks = [torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True),
+             torch.autograd.graph.saved_tensors_hooks(lambda v: v, transposed),
+             torch.autograd.graph.saved_tensors_hooks(lambda v: v, odd_base)]
+    for h in hooks:
+        with h:
+            got = run_all(q.detach(), x.detach(), t, w)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_that_come_back_wrong_are_refused(device):
+    q, x, t, w = make(6, 40, 32, torch.float32)
+    for unpack, message in [(lambda v: v.cpu(), "CUDA"), (lambda v: v.half() if v.is_floating_point() else v, "stats"),
+                            (lambda v: v[:-1] if v.dim() == 1 else v, "targets")]:
+        qd, xd = q.to(device).requires_grad_(), x.to(device).requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, unpack):
+            loss = loss_fn(qd, xd, t.to(device))
+            with pytest.raises(RuntimeError, match=message):
+                torch.autograd.grad(loss, (qd, xd))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DT))
 def test_no_queries(device, dtype):
     q, x, t, w = make(1, 30, 16, DT[dtype])
     loss, dq, dx = run_all(q[:0], x, t[:0], w[:0])
