@@ -47,6 +47,11 @@ void check_same_device(const at::Tensor& a, const at::Tensor& b, const char* nam
 
 bool float_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
 
+// before anything of their size is made
+void check_rows(int64_t rows, const char* name) {
+    TORCH_CHECK(rows < (1LL << 31), name, " must have fewer than 2^31 rows");
+}
+
 struct XentArgs {
     Rows q, x;
     at::Tensor t;
@@ -67,7 +72,9 @@ XentArgs xent_args(const at::Tensor& queries, const at::Tensor& database, const 
     a.nq = queries.size(0);
     a.n = database.size(0);
     a.d = queries.size(1);
-    TORCH_CHECK(a.d < (1LL << 31) - 256, "dim must be < 2^31");
+    check_rows(a.nq, "queries");
+    check_rows(a.n, "database");
+    TORCH_CHECK(a.d < (1LL << 31) - 256, "dim must be < 2^31 - 256");
     a.dtype = dtype_code(queries.scalar_type());
     check_pending_status();
     a.q = aligned_rows(queries);
@@ -97,6 +104,7 @@ at::Tensor scratch(size_t bytes, const at::Tensor& like) {
 Result sq8_encode(const at::Tensor& vectors) {
     check_matrix(vectors, "vectors");
     TORCH_CHECK(float_type(vectors.scalar_type()), "vectors must be float32, float16 or bfloat16");
+    TORCH_CHECK(vectors.size(1) < (1LL << 31) - 256, "dim must be < 2^31 - 256");
     c10::cuda::CUDAGuard guard(vectors.device());
     at::Tensor codes = at::empty({vectors.size(0), vectors.size(1)}, vectors.options().dtype(at::kChar));
     at::Tensor scales = at::empty({vectors.size(0)}, vectors.options().dtype(at::kFloat));
@@ -120,6 +128,8 @@ at::Tensor sq8_dot_product(const at::Tensor& query_codes, const at::Tensor& quer
     TORCH_CHECK(scales.dim() == 1 && scales.size(0) == codes.size(0), "scales must be 1D [n]");
     TORCH_CHECK(float_type(dtype), "dtype must be float32, float16 or bfloat16");
     const int64_t nq = query_codes.size(0), n = codes.size(0), d = codes.size(1);
+    check_rows(nq, "query_codes");
+    check_rows(n, "codes");
     c10::cuda::CUDAGuard guard(codes.device());
     at::Tensor out = at::empty({nq, n}, codes.options().dtype(dtype));
     if (nq == 0 || n == 0) return out;

@@ -31,6 +31,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "tile_f32.cuh"
@@ -866,12 +867,21 @@ __global__ void __launch_bounds__(NT)
 
 // -------------------------------------------------------------- host side --
 
+constexpr int64_t kMaxRows = (1LL << 31) - 1;
+constexpr int kMaxDim = INT_MAX - 256;  // K blocks are counted in int
+
+// sizes for which there is a plan
+bool plannable(int dtype, int64_t nq, int64_t n, int d) {
+    return elem_size(dtype) != 0 && nq >= 0 && nq <= kMaxRows && n >= 1 && n <= kMaxRows && d >= 1 && d <= kMaxDim;
+}
+
 int check_common(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
                  const int64_t* targets, float scale, int reduction) {
     const int64_t e = (int64_t)elem_size(dtype);
     RDB_CHECK_ARG(e != 0, "unknown dtype %d", dtype);
     RDB_CHECK_ARG(nq >= 0 && n >= 1 && d >= 1 && ldq >= d && ldx >= d, "bad shape");
-    RDB_CHECK_ARG(nq < (1LL << 31) && n < (1LL << 31), "nq and n must be < 2^31");
+    RDB_CHECK_ARG(nq <= kMaxRows && n <= kMaxRows, "nq and n must be < 2^31");
+    RDB_CHECK_ARG(d <= kMaxDim, "d must be < 2^31 - 256");
     RDB_CHECK_ARG(scale > 0.f && scale <= 2.0e38f, "scale must be positive and finite");
     RDB_CHECK_ARG(reduction >= RDB_REDUCE_NONE && reduction <= RDB_REDUCE_SUM, "unknown reduction %d", reduction);
     RDB_CHECK_ARG(x && (nq == 0 || (q && targets)), "NULL pointer");
@@ -1254,7 +1264,7 @@ extern "C" {
 
 size_t rdb_softmax_xent_workspace(int dtype, int64_t nq, int64_t n, int d, int reduction) {
     (void)reduction;
-    if (elem_size(dtype) == 0 || nq < 0 || n < 1 || d < 1) return 0;
+    if (!plannable(dtype, nq, n, d)) return 0;
     const FwdPlan p = fwd_plan(dtype, nq, n, d);
     return fwd_ws(nullptr, p, dtype, nq, d).bytes;
 }
@@ -1339,7 +1349,7 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
 }
 
 size_t rdb_softmax_xent_backward_workspace(int dtype, int64_t nq, int64_t n, int d, int need_dq, int need_dx) {
-    if (elem_size(dtype) == 0 || nq < 0 || n < 1 || d < 1) return 0;
+    if (!plannable(dtype, nq, n, d)) return 0;
     const BwdPlan p = bwd_plan(dtype, nq, n, d, need_dq != 0, need_dx != 0);
     return bwd_ws(nullptr, p, dtype, nq, d, need_dq != 0, need_dx != 0).bytes;
 }

@@ -157,12 +157,17 @@ def test_abi_refusals_without_gpu():
             assert lib.rdb_softmax_xent_workspace(dt, nq, n, d, 0) > 0
             for flags in ((0, 0), (1, 0), (0, 1), (1, 1)):
                 assert lib.rdb_softmax_xent_backward_workspace(dt, nq, n, d, *flags) > 0
+    for nq, n, d in ((1 << 31, 5, 8), (1 << 40, 5, 8), (5, 1 << 31, 8), (5, 1 << 44, 8), (5, 5, (1 << 31) - 1),
+                     (-1, 5, 8), (5, 0, 8), (5, 5, 0)):  # and none where the calls refuse
+        assert lib.rdb_softmax_xent_workspace(2, nq, n, d, 0) == 0
+        assert lib.rdb_softmax_xent_backward_workspace(2, nq, n, d, 1, 1) == 0
     ok = dict(dt=2, q=1 << 20, nq=2, ldq=16, x=1 << 21, n=4, ldx=16, d=16, t=1 << 22, s=1.0, ign=-100, red=1)
     bad = [(dict(dt=5), b"dtype"), (dict(n=0), b"shape"), (dict(d=0), b"shape"), (dict(ldq=8), b"shape"),
            (dict(s=0.0), b"scale"), (dict(s=-1.0), b"scale"), (dict(s=float("inf")), b"scale"),
            (dict(s=float("nan")), b"scale"), (dict(red=3), b"reduction"), (dict(q=None), b"NULL"),
            (dict(t=None), b"NULL"), (dict(ldx=20), b"multiples of 16"), (dict(x=(1 << 21) + 2), b"aligned"),
-           (dict(n=1 << 31), b"2^31")]
+           (dict(n=1 << 31), b"2^31"), (dict(nq=1 << 31), b"2^31"),
+           (dict(d=(1 << 31) - 1, ldq=1 << 31, ldx=1 << 31), b"2^31 - 256")]
     for kw, msg in bad:
         a = list({**ok, **kw}.values())
         assert f(*a, 1 << 23, 1 << 24, 1 << 25, 1 << 40, None) == 1 and msg in lib.rdb_last_error(), kw
@@ -190,6 +195,11 @@ def test_refusals(device):
     for s in (0.0, -1.0, float("inf"), float("nan"), 1e39):
         with pytest.raises(RuntimeError, match="scale must be positive"):
             loss_fn(q, x, t, scale=s)
+    many = torch.zeros(1, 8, device=device).expand(1 << 31, 8)
+    with pytest.raises(RuntimeError, match="database must have fewer than 2\\^31 rows"):
+        loss_fn(q, many, t)
+    with pytest.raises(RuntimeError, match="queries must have fewer than 2\\^31 rows"):
+        loss_fn(many, x, t[:1].expand(1 << 31))
     loss, stats = _C().softmax_cross_entropy(q, x, t, 1.0, IGN, 0)
     with pytest.raises(RuntimeError, match="stats must be"):
         _C().softmax_cross_entropy_backward(loss, q, x, t, stats[:5], 1.0, IGN, 0)

@@ -96,6 +96,13 @@ def test_refusals(device):
                       ((c, s, c, s, torch.float64), "dtype must be"), ((c[:, :0], s, c[:, :0], s), "at least one")]:
         with pytest.raises(RuntimeError, match=msg):
             C.sq8_dot_product(*args)
+    many, ms = c[:1].expand(1 << 31, 16), s[:1].expand(1 << 31)
+    for args, msg in [((many, ms, c, s), "query_codes must have"), ((c, s, many, ms), "codes must have")]:
+        with pytest.raises(RuntimeError, match=msg + " fewer than 2\\^31 rows"):
+            C.sq8_dot_product(*args)
+    for d in ((1 << 31) - 256, (1 << 32) + 8):  # the latter is 8 in 32 bits
+        with pytest.raises(RuntimeError, match="dim must be <"):
+            C.sq8_encode(s[:1].reshape(1, 1).expand(1, d))
     with pytest.raises(RuntimeError, match="must be 2D"):
         C.sq8_encode(s)
     with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
