@@ -1,0 +1,47 @@
+// Launches whose start overlaps the end of what runs before them in the stream
+// (programmatic dependent launch): such a kernel is placed and set up (barriers,
+// tensor memory) while its predecessor drains, and waits before it touches global
+// memory.  A captured training step of 256 x 256 x 768 bf16 takes 33.2 us instead
+// of 37.0, the scores of one query and 100,000 int8 rows 16.1 instead of 18.4, a
+// loss over them 42 instead of 45.
+//
+// Every thread of a kernel launched this way calls chain_wait() before any access
+// to global memory: a kernel then finishes only after all before it, and what
+// follows it in the stream, launched in whichever way, sees all of them finished.
+#pragma once
+
+#include <utility>
+
+#include "common.cuh"
+
+namespace rdb {
+namespace {
+
+// What is before has finished and is visible; the next kernel may be placed.  (In
+// the other order a chain of short kernels is placed at once, each holding its
+// threads while it waits for all before it: 34.7 us, and slower than no overlap
+// for steps of small fp32 kernels.)
+__device__ __forceinline__ void chain_wait() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <class... K, class... A>
+int launch_chained(void (*kernel)(K...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t s, A&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    RDB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+    note_launch();
+    return RDB_OK;
+}
+
+}  // namespace
+}  // namespace rdb

@@ -2,6 +2,7 @@
 // layout TMA and 16-byte loads need, for operands that do not have it.
 #include <algorithm>
 
+#include "chain.cuh"
 #include "common.cuh"
 
 namespace rdb {
@@ -12,6 +13,7 @@ template <typename W>
 __global__ void __launch_bounds__(256)
     pad_rows_kernel(const uint8_t* __restrict__ src, int64_t rows, int64_t row_bytes, int64_t src_stride,
                     uint4* __restrict__ dst, int64_t units) {
+    chain_wait();
     const int64_t total = rows * units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * 256) {
@@ -48,14 +50,9 @@ extern "C" int rdb_pad_rows(const void* src, int64_t rows, int64_t row_bytes, in
     uint4* o = static_cast<uint4*>(dst);
     // the widest access that base, stride and row length allow
     const uint64_t align = reinterpret_cast<uintptr_t>(src) | (uint64_t)src_stride | (uint64_t)row_bytes;
-    if (align % 8 == 0)
-        pad_rows_kernel<uint2><<<blocks, 256, 0, s>>>(p, rows, row_bytes, src_stride, o, units);
-    else if (align % 4 == 0)
-        pad_rows_kernel<uint32_t><<<blocks, 256, 0, s>>>(p, rows, row_bytes, src_stride, o, units);
-    else if (align % 2 == 0)
-        pad_rows_kernel<uint16_t><<<blocks, 256, 0, s>>>(p, rows, row_bytes, src_stride, o, units);
-    else
-        pad_rows_kernel<uint8_t><<<blocks, 256, 0, s>>>(p, rows, row_bytes, src_stride, o, units);
-    RDB_LAUNCH_CHECK();
-    return RDB_OK;
+    const auto kernel = align % 8 == 0   ? pad_rows_kernel<uint2>
+                        : align % 4 == 0 ? pad_rows_kernel<uint32_t>
+                        : align % 2 == 0 ? pad_rows_kernel<uint16_t>
+                                         : pad_rows_kernel<uint8_t>;
+    return launch_chained(kernel, blocks, 256, 0, s, p, rows, row_bytes, src_stride, o, units);
 }

@@ -13,6 +13,7 @@
 
 #include <type_traits>
 
+#include "chain.cuh"
 #include "common.cuh"
 
 namespace rdb {
@@ -103,6 +104,7 @@ __global__ void __launch_bounds__(256)
     sq8_encode_rows_kernel(const T* __restrict__ x, int64_t n, int64_t ldx, int units, int8_t* __restrict__ codes,
                            int64_t ldc, float* __restrict__ scales) {
     constexpr int E = 16 / sizeof(T);  // elements of a unit
+    chain_wait();
     const int lane = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= n) return;
@@ -135,29 +137,25 @@ __global__ void __launch_bounds__(256)
     if (lane == 0) scales[row] = scale;
 }
 
+// rows that the kernel above takes
+bool whole_units(int elem, const void* x, int64_t ldx, int d, const int8_t* codes, int64_t ldc) {
+    const int e = 16 / elem;
+    return d % e == 0 && ldx % e == 0 && ldc % e == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
+           (reinterpret_cast<uintptr_t>(codes) & (e - 1)) == 0 && d / e <= 256;
+}
+
 template <typename T>
-bool encode_rows(const void* x, int64_t n, int64_t ldx, int d, int8_t* codes, int64_t ldc, float* scales,
-                 cudaStream_t s) {
-    constexpr int E = 16 / (int)sizeof(T);
-    const int units = d / E;
-    if (d % E != 0 || ldx % E != 0 || ldc % E != 0 || (reinterpret_cast<uintptr_t>(x) & 15) != 0 ||
-        (reinterpret_cast<uintptr_t>(codes) & (E - 1)) != 0 || units > 256)
-        return false;
-    const unsigned blocks = (unsigned)((n + 7) / 8);
-    const T* p = static_cast<const T*>(x);
-    if (units <= 32)
-        sq8_encode_rows_kernel<T, 1><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
-    else if (units <= 64)
-        sq8_encode_rows_kernel<T, 2><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
-    else if (units <= 96)
-        sq8_encode_rows_kernel<T, 3><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
-    else if (units <= 128)
-        sq8_encode_rows_kernel<T, 4><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
-    else if (units <= 192)
-        sq8_encode_rows_kernel<T, 6><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
-    else
-        sq8_encode_rows_kernel<T, 8><<<blocks, 256, 0, s>>>(p, n, ldx, units, codes, ldc, scales);
-    return true;
+int encode_rows(const void* x, int64_t n, int64_t ldx, int d, int8_t* codes, int64_t ldc, float* scales,
+                cudaStream_t s) {
+    const int units = d / (16 / (int)sizeof(T));
+    const auto kernel = units <= 32    ? sq8_encode_rows_kernel<T, 1>
+                        : units <= 64  ? sq8_encode_rows_kernel<T, 2>
+                        : units <= 96  ? sq8_encode_rows_kernel<T, 3>
+                        : units <= 128 ? sq8_encode_rows_kernel<T, 4>
+                        : units <= 192 ? sq8_encode_rows_kernel<T, 6>
+                                       : sq8_encode_rows_kernel<T, 8>;
+    return launch_chained(kernel, (unsigned)((n + 7) / 8), 256, 0, s, static_cast<const T*>(x), n, ldx, units, codes, ldc,
+                          scales);
 }
 
 // per-row metric value of the dequantised row: |x^|^2 (L2), |x^| or
@@ -191,12 +189,13 @@ int rdb_sq8_encode(int dtype, const void* x, int64_t n, int64_t ldx, int d, int8
     RDB_CHECK_ARG(n >= 0 && d >= 1 && ldx >= d && ldc >= d, "bad shape");
     if (n == 0) return RDB_OK;
     RDB_CHECK_ARG(x && codes && scales, "NULL pointer");
-    const unsigned blocks = (unsigned)((n + 7) / 8);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool done = dtype == RDB_F32   ? encode_rows<float>(x, n, ldx, d, codes, ldc, scales, s)
-                      : dtype == RDB_F16 ? encode_rows<__half>(x, n, ldx, d, codes, ldc, scales, s)
-                                         : encode_rows<__nv_bfloat16>(x, n, ldx, d, codes, ldc, scales, s);
-    if (!done) sq8_encode_kernel<<<blocks, 256, 0, s>>>(dtype, x, n, ldx, d, codes, ldc, scales);
+    if (whole_units((int)elem_size(dtype), x, ldx, d, codes, ldc)) {
+        if (dtype == RDB_F32) return encode_rows<float>(x, n, ldx, d, codes, ldc, scales, s);
+        if (dtype == RDB_F16) return encode_rows<__half>(x, n, ldx, d, codes, ldc, scales, s);
+        return encode_rows<__nv_bfloat16>(x, n, ldx, d, codes, ldc, scales, s);
+    }
+    sq8_encode_kernel<<<(unsigned)((n + 7) / 8), 256, 0, s>>>(dtype, x, n, ldx, d, codes, ldc, scales);
     RDB_LAUNCH_CHECK();
     return RDB_OK;
 }

@@ -55,6 +55,7 @@ __global__ void __launch_bounds__(GV_THREADS)
                    const int8_t* __restrict__ xc, const float* __restrict__ xs, int64_t n, int64_t ldx, int d,
                    T* __restrict__ out, int64_t ldo) {
     extern __shared__ __align__(16) int8_t sq[];  // [NQ][dp], zero behind d and behind nq
+    chain_wait();
     const int dp = (d + 15) / 16 * 16, chunks = dp / 16;
     for (int i = threadIdx.x; i < NQ * dp; i += GV_THREADS) {
         const int b = i / dp, t = i - b * dp;
@@ -131,10 +132,8 @@ int launch_few(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const
     const int rows = GV_THREADS / GV_LANES;
     const int64_t blocks = std::min<int64_t>((n + rows - 1) / rows, 4LL * num_sms());
     const size_t smem = static_cast<size_t>(NQ) * ((d + 15) / 16 * 16);
-    sq8_few_kernel<T, NQ><<<(unsigned)blocks, GV_THREADS, smem, s>>>(qc, qs, (int)nq, ldq, xc, xs, n, ldx, d,
-                                                                     static_cast<T*>(out), ldo);
-    RDB_LAUNCH_CHECK();
-    return RDB_OK;
+    return launch_chained(sq8_few_kernel<T, NQ>, (unsigned)blocks, GV_THREADS, smem, s, qc, qs, (int)nq, ldq, xc, xs, n,
+                          ldx, d, static_cast<T*>(out), ldo);
 }
 
 // ----------------------------------------------------------- tensor cores --
@@ -257,10 +256,8 @@ int launch_tile(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, cons
     RDB_TRY(make_map_3d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, d, n, 1, ldx, 0, a.x_rows));
     RDB_TRY(make_map_3d(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, d, nq, 1, ldq, 0, a.q_rows));
     const int64_t tiles = (int64_t)a.nqt * a.nxt;
-    sq8_tile_kernel<T><<<2 * (unsigned)std::min<int64_t>(tile_pairs(), tiles), TT_THREADS, TT_SMEM, s>>>(
-        mx, mq, a, tile_status());
-    RDB_LAUNCH_CHECK();
-    return RDB_OK;
+    return launch_chained(sq8_tile_kernel<T>, 2 * (unsigned)std::min<int64_t>(tile_pairs(), tiles), TT_THREADS, TT_SMEM, s,
+                          mx, mq, a, tile_status());
 }
 
 template <typename T>

@@ -208,6 +208,7 @@ __device__ __forceinline__ void tile_loop_f32(uint8_t* smem_raw, const P& p, con
         tmem_alloc_t<false>(tmem_slot, 4 * TF_N);
         tmem_relinquish_t<false>();
     }
+    chain_wait();  // what is above touches no global memory
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -46,6 +46,7 @@
 // what it has in flight, and the CTA frees its TMEM and exits.
 #pragma once
 
+#include "chain.cuh"
 #include "tc_common.cuh"
 
 namespace rdb {
@@ -234,6 +235,7 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
         tmem_alloc_t<true>(tmem_slot, 512);
         tmem_relinquish_t<true>();
     }
+    chain_wait();  // what is above touches no global memory
     tc_fence_before();
     cluster_sync_all();  // both CTAs' barriers initialised before any remote use
     tc_fence_after();

@@ -248,9 +248,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     xent_scan_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mx,
                      const __grid_constant__ FwdArgs a, const bool bf16, const TileStatus st) {
     extern __shared__ uint8_t smem_raw[];
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
     const FwdPolicy p{&mq, &mx, a};
     tile_loop(smem_raw, p, bf16, st);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
 }
 
 // the same for at most 128 queries and fp32 rows as they are
@@ -258,9 +258,9 @@ __global__ void __launch_bounds__(TF_THREADS, 1)
     xent_scan_f32_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ F32Rows x,
                          const __grid_constant__ FwdArgs a, const TileStatus st) {
     extern __shared__ uint8_t smem_raw[];
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
     const FwdPolicy p{&mq, nullptr, a};
     tile_loop_f32(smem_raw, p, x, st);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
 }
 
 // mean or sum of the losses of the queries that count, and their number, by one
@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(NT)
     xent_join_kernel(const float2* part, int parts, const T* q, int64_t ldq, const T* x, int64_t ldx, int d,
                      const int64_t* targets, int64_t ignore, int64_t n, float c, int64_t nq, bool wide, float* stats,
                      float* loss, int reduction, float* total, unsigned* ticket) {
+    chain_wait();
     __shared__ float2 sj[NT / 32];
     __shared__ float ss[NT / 32];
     __shared__ int sc[NT / 32];
@@ -414,6 +415,7 @@ __global__ void __launch_bounds__(NT)
 // the reduced loss of no queries
 __global__ void __launch_bounds__(NT)
     xent_reduce_kernel(const int64_t* targets, int64_t ignore, int64_t nq, int reduction, float* stats, float* total) {
+    chain_wait();
     __shared__ float ss[NT / 32];
     __shared__ int sc[NT / 32];
     reduce_losses(stats, targets, ignore, nq, reduction, total, ss, sc);
@@ -453,6 +455,7 @@ __device__ float largest_weight(const Weights& w, int64_t nq, float* sm) {
 }
 
 __global__ void __launch_bounds__(1024) xent_wmax_kernel(const Weights w, int64_t nq, float* wmax) {
+    chain_wait();
     __shared__ float sm[32];
     const float mx = largest_weight(w, nq, sm);
     if (threadIdx.x == 0) *wmax = mx;
@@ -485,6 +488,7 @@ template <typename T>
 __global__ void __launch_bounds__(NT)
     xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const Weights w, bool scan, float* wmax, void* out,
                          int64_t ldo) {
+    chain_wait();
     __shared__ float sm[NT / 32];
     float mx;
     if (scan) {
@@ -519,6 +523,7 @@ __global__ void __launch_bounds__(NT)
 // fp32 rows -> three bf16 planes [3][n][ldo], ldo a multiple of 8
 __global__ void __launch_bounds__(NT)
     xent_split_kernel(const float* x, int64_t n, int64_t ldx, int d, __nv_bfloat16* out, int64_t ldo) {
+    chain_wait();
     const int64_t units = ldo / 8, total = n * units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * NT) {
@@ -845,6 +850,7 @@ template <typename T>
 __global__ void __launch_bounds__(NT)
     xent_dq_kernel(const float* part, int splits, int64_t nq, int d, int dp, const Weights w, float scale, T* dq,
                    int64_t lddq) {
+    chain_wait();
     const int64_t units = dp / 4, total = nq * units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * NT) {
@@ -1099,9 +1105,8 @@ int prob_width(int64_t rows, int nqb, int pairs) {
 }
 
 int split_rows(const void* x, int64_t n, int64_t ldx, int d, __nv_bfloat16* out, cudaStream_t s) {
-    xent_split_kernel<<<elementwise_blocks(n * up(d, 8) / 8), NT, 0, s>>>(static_cast<const float*>(x), n, ldx, d, out,
-                                                                          up(d, 8));
-    RDB_LAUNCH_CHECK();
+    RDB_TRY(launch_chained(xent_split_kernel, elementwise_blocks(n * up(d, 8) / 8), NT, 0, s,
+                           static_cast<const float*>(x), n, ldx, d, out, up(d, 8)));
     return RDB_OK;
 }
 
@@ -1145,14 +1150,12 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     if (dx) {
         const bool scan = nq <= 2048;
         if (!scan) {
-            xent_wmax_kernel<<<1, 1024, 0, s>>>(wt, nq, w.wmax);
-            RDB_LAUNCH_CHECK();
+            RDB_TRY(launch_chained(xent_wmax_kernel, 1, 1024, 0, s, wt, nq, w.wmax));
         }
         const int64_t items = nq * d8 / 8;
-        xent_weighted_kernel<T><<<scan ? (unsigned)std::min<int64_t>((items + NT - 1) / NT, num_sms())
-                                       : elementwise_blocks(items),
-                                  NT, 0, s>>>(static_cast<const T*>(q), nq, ldq, d, wt, scan, w.wmax, w.qw, d8);
-        RDB_LAUNCH_CHECK();
+        RDB_TRY(launch_chained(xent_weighted_kernel<T>,
+                               scan ? (unsigned)std::min<int64_t>((items + NT - 1) / NT, num_sms()) : elementwise_blocks(items),
+                               NT, 0, s, static_cast<const T*>(q), nq, ldq, d, wt, scan, w.wmax, w.qw, d8));
     }
     Planes qo;
     RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
@@ -1205,17 +1208,16 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         RDB_CHECK_ARG(tiles < (1LL << 31), "too many tiles for one launch");
         pa.njobs = (int)tiles;
         if (p.direct) {
-            xent_prob_f32_kernel<<<(unsigned)std::min<int64_t>(num_sms(), tiles), TF_THREADS, TF_SMEM, s>>>(mq, mg, xr,
-                                                                                                           pa, st);
+            RDB_TRY(launch_chained(xent_prob_f32_kernel, (unsigned)std::min<int64_t>(num_sms(), tiles), TF_THREADS,
+                                   TF_SMEM, s, mq, mg, xr, pa, st));
         } else {
             Planes xo;
             RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
             RDB_TRY(operand_map(&mx, dtype, xo, d, rows, pa.width / 2));
             RDB_TRY(operand_map(&mxmn, dtype, xo, d, rows, 0));
-            xent_prob_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS, TT_SMEM, s>>>(
-                mq, mx, mg, pa, bf16, st);
+            RDB_TRY(launch_chained(xent_prob_kernel<T>, 2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS,
+                                   TT_SMEM, s, mq, mx, mg, pa, bf16, st));
         }
-        RDB_LAUNCH_CHECK();
 
         ga.n = rows;
         ga.kc = (int)((rows + 63) / 64);
@@ -1234,23 +1236,20 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
             gq.x_blocks = 0;
             gq.q_first = true;
             const int64_t jobs = (int64_t)gq.nt * gq.q_split;
-            xent_grad_f32_kernel<<<(unsigned)std::min<int64_t>(num_sms(), jobs), TF_THREADS, TF_SMEM, s>>>(mgk, mpart, xr,
-                                                                                                          gq, st);
-            RDB_LAUNCH_CHECK();
+            RDB_TRY(launch_chained(xent_grad_f32_kernel, (unsigned)std::min<int64_t>(num_sms(), jobs), TF_THREADS,
+                                   TF_SMEM, s, mgk, mpart, xr, gq, st));
         }
         ga.q_blocks = dq && !p.direct ? p.nqb : 0;
         ga.x_blocks = dx ? (int)((rows + TT_M - 1) / TT_M) : 0;
         const int64_t jobs = (int64_t)ga.nt * ((int64_t)ga.q_blocks * ga.q_split + ga.x_blocks);
         if (jobs == 0) continue;
         RDB_CHECK_ARG(jobs < (1LL << 31), "too many tiles for one launch");
-        xent_grad_kernel<T><<<2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM, s>>>(
-            mgk, mgmn, mxmn, mqw, mpart, mdx, ga, bf16, st);
-        RDB_LAUNCH_CHECK();
+        RDB_TRY(launch_chained(xent_grad_kernel<T>, 2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM,
+                               s, mgk, mgmn, mxmn, mqw, mpart, mdx, ga, bf16, st));
     }
     if (dq) {
-        xent_dq_kernel<T><<<elementwise_blocks(nq * p.dp / 4), NT, 0, s>>>(w.part, p.q_split, nq, d, p.dp, wt, scale,
-                                                                           static_cast<T*>(dq), lddq);
-        RDB_LAUNCH_CHECK();
+        RDB_TRY(launch_chained(xent_dq_kernel<T>, elementwise_blocks(nq * p.dp / 4), NT, 0, s, w.part, p.q_split, nq,
+                               d, p.dp, wt, scale, static_cast<T*>(dq), lddq));
     }
     return RDB_OK;
 }
@@ -1316,34 +1315,33 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
             const unsigned workers = (unsigned)std::min<int64_t>(p.workers, units);
             if (p.direct) {
                 const F32Rows xr{static_cast<const float*>(x), ldx, n, d};
-                xent_scan_f32_kernel<<<workers, TF_THREADS, TF_SMEM, s>>>(mq, xr, a, st);
+                RDB_TRY(launch_chained(xent_scan_f32_kernel, workers, TF_THREADS, TF_SMEM, s, mq, xr, a, st));
             } else {
                 Planes xo;
                 RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
                 RDB_TRY(operand_map(&mx, dtype, xo, d, rows, p.width / 2));
-                xent_scan_kernel<<<2 * workers, TT_THREADS, TT_SMEM, s>>>(mq, mx, a, dtype != RDB_F16, st);
+                RDB_TRY(launch_chained(xent_scan_kernel, 2 * workers, TT_THREADS, TT_SMEM, s, mq, mx, a,
+                                       dtype != RDB_F16, st));
             }
-            RDB_LAUNCH_CHECK();
         }
         const bool wide = nq <= num_sms();
         const unsigned blocks = (unsigned)std::min<int64_t>(wide ? nq : (nq + NT / 32 - 1) / (NT / 32), 16LL * num_sms());
         const int parts = p.slots * p.groups;
         if (dtype == RDB_F32)
-            xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const float*>(q), ldq,
-                                                   static_cast<const float*>(x), ldx, d, targets, ignore_index, n, c, nq, wide,
-                                                   stats, loss, reduction, loss, w.ticket);
+            RDB_TRY(launch_chained(xent_join_kernel<float>, blocks, NT, 0, s, w.part, parts,
+                                   static_cast<const float*>(q), ldq, static_cast<const float*>(x), ldx, d, targets,
+                                   ignore_index, n, c, nq, wide, stats, loss, reduction, loss, w.ticket));
         else if (dtype == RDB_F16)
-            xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const __half*>(q), ldq,
-                                                   static_cast<const __half*>(x), ldx, d, targets, ignore_index, n, c, nq, wide,
-                                                   stats, loss, reduction, loss, w.ticket);
+            RDB_TRY(launch_chained(xent_join_kernel<__half>, blocks, NT, 0, s, w.part, parts,
+                                   static_cast<const __half*>(q), ldq, static_cast<const __half*>(x), ldx, d, targets,
+                                   ignore_index, n, c, nq, wide, stats, loss, reduction, loss, w.ticket));
         else
-            xent_join_kernel<<<blocks, NT, 0, s>>>(w.part, parts, static_cast<const __nv_bfloat16*>(q), ldq,
-                                                   static_cast<const __nv_bfloat16*>(x), ldx, d, targets, ignore_index, n,
-                                                   c, nq, wide, stats, loss, reduction, loss, w.ticket);
-        RDB_LAUNCH_CHECK();
+            RDB_TRY(launch_chained(xent_join_kernel<__nv_bfloat16>, blocks, NT, 0, s, w.part, parts,
+                                   static_cast<const __nv_bfloat16*>(q), ldq, static_cast<const __nv_bfloat16*>(x),
+                                   ldx, d, targets, ignore_index, n, c, nq, wide, stats, loss, reduction, loss,
+                                   w.ticket));
     } else if (reduction != RDB_REDUCE_NONE) {
-        xent_reduce_kernel<<<1, NT, 0, s>>>(targets, ignore_index, nq, reduction, stats, loss);
-        RDB_LAUNCH_CHECK();
+        RDB_TRY(launch_chained(xent_reduce_kernel, 1, NT, 0, s, targets, ignore_index, nq, reduction, stats, loss));
     }
     return RDB_OK;
 }

@@ -622,6 +622,46 @@ def test_two_threads_at_once(device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("d", [64, 50])
+def test_short_calls_in_a_row(device, d, dtype):
+    """Calls whose launches overlap (each starts while the one before it ends)
+    on inputs that change between them, next to other kernels, give the bits of
+    the same calls with a synchronisation after each."""
+    q0, x0, t, _ = make(48, 700, d, DT[dtype])
+    q0, x0, t = q0.to(device), x0.to(device), t.to(device)
+
+    def run(sync):
+        q, x, out = q0.clone(), x0.clone(), []
+        for i in range(30):
+            a, b = q.detach().requires_grad_(), x.detach().requires_grad_()
+            loss = loss_fn(a, b, t, scale=5.0)
+            sync()
+            dq, dx = torch.autograd.grad(loss, (a, b))
+            sync()
+            c, s = _C().sq8_encode(x)
+            sync()
+            qc, qs = _C().sq8_encode(q)
+            sync()
+            scores = _C().sq8_dot_product(qc, qs, c, s, DT[dtype])
+            sync()
+            one = _C().sq8_dot_product(qc[i:i + 1], qs[i:i + 1], c, s)
+            sync()
+            out += [loss.detach(), dq, dx, scores, one]
+            q -= dq * 4
+            x -= dx * 4  # overwrites what the calls before read
+            del a, b, c, s, qc, qs  # the allocator hands their memory on
+            sync()
+        return out
+
+    want = run(torch.cuda.synchronize)
+    got = run(lambda: None)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b) and not a.isnan().any()
+
+
+@pytest.mark.gpu
 def test_train_quantise_score(device):
     """The operators together: a step of training queries and rows, the rows
     quantised into an int8 base, queries quantised and scored, top-k taken."""
