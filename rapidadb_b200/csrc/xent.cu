@@ -26,7 +26,7 @@
 // Bound: the products, 2 nq n d FLOP each, one forward and three backward.  4,096
 // queries, 131,072 rows, d = 768, bf16: forward 578 us (1.43 PFLOP/s, the rate
 // cuBLAS holds for seconds is 1.40), probabilities 620, gradients 1,218.  Few
-// queries: the rows' bytes, 1 x 1M x 768 bf16 230 us (6.6 TB/s).
+// queries: the rows' bytes, 1 x 1M x 768 bf16 225 us (6.8 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -261,6 +261,166 @@ __global__ void __launch_bounds__(TF_THREADS, 1)
     const FwdPolicy p{&mq, nullptr, a};
     tile_loop_f32(smem_raw, p, x, st);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
+}
+
+// ---- the same for a few queries, without tensor cores
+
+constexpr int ST_MAX_DIM = 1024;  // 32 elements of every query a lane
+
+// one 16-byte unit of a row as pairs of floats
+template <typename T>
+__device__ __forceinline__ void pairs16(const uint4& u, uint64_t (&v)[8 / sizeof(T)]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(T) == 4) {
+        v[0] = pack2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        v[1] = pack2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T* e = reinterpret_cast<const T*>(&w[i]);
+            v[i] = pack2(to_f(e[0]), to_f(e[1]));
+        }
+    }
+}
+
+// rows a warp has in flight: about 12 loads a lane
+constexpr int stream_rows(int units) { return units == 1 ? 8 : units <= 3 ? 4 : 2; }
+
+// A lane holds every 32nd 16-byte unit of the queries in registers, U of them, as
+// fp32; the warps take R rows each in turn (shares of their own, rows far apart,
+// are up to 20 % slower).  The products are fp32 fma chains; the lanes' sums of
+// R x NQ products are joined so that each lane ends up with one of them, whose
+// (m, z) it keeps.  One part per query and block.  (Queries in shared memory cost
+// a load per use: 50 us instead of 32 for the case below.)
+template <typename T, int NQ, int U>
+__global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
+    xent_stream_kernel(const T* __restrict__ q, int nq, int64_t ldq, const T* __restrict__ x, int64_t n, int64_t ldx,
+                       int d, const int64_t* __restrict__ targets, float c, float2* part, unsigned* ticket) {
+    constexpr int E = 16 / sizeof(T), P = E / 2;  // elements and pairs of a unit
+    constexpr int R = stream_rows(U), V = R * NQ, kDup = 32 / V;
+    __shared__ float2 sj[NT / 32][NQ];
+    chain_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int full = d / E, units = (d + E - 1) / E;
+    // A row's last unit may reach behind d, but not behind the row's stride, which
+    // is whole units: it is read whole and cut when it is used.  Only the last row
+    // may end with its elements.
+    auto load = [&](const T* row, bool last, int u) -> uint4 {
+        if (u < (last ? full : units)) return __ldg(reinterpret_cast<const uint4*>(row) + u);
+        union {
+            uint4 v;
+            T e[E];
+        } o;
+        o.v = make_uint4(0u, 0u, 0u, 0u);
+        if (last) {
+#pragma unroll
+            for (int t = 0; t < E; ++t)
+                if (u * E + t < d) o.e[t] = row[u * E + t];
+        }
+        return o.v;
+    };
+    auto cut = [&](uint4& v, int u) {
+        if (d % E == 0 || u != full) return;
+        uint32_t* o = reinterpret_cast<uint32_t*>(&v);
+        const int bytes = (d - full * E) * (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int left = bytes - 4 * i;
+            o[i] = left >= 4 ? o[i] : left > 0 ? o[i] & 0xffffu : 0u;
+        }
+    };
+    uint64_t qv[NQ][U * P];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint64_t v[P];
+            pairs16<T>(b < nq ? load(q + b * ldq, true, u * 32 + lane) : make_uint4(0u, 0u, 0u, 0u), v);
+#pragma unroll
+            for (int i = 0; i < P; ++i) qv[b][u * P + i] = v[i];
+        }
+    const int row = lane / kDup / NQ, bq = lane / kDup % NQ;  // of the sum this lane ends up with
+    const int64_t tgt = bq < nq ? targets[bq] : -1;
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * (NT / 32) + warp;
+    const int64_t nw = static_cast<int64_t>(gridDim.x) * (NT / 32);
+    int64_t r0 = w * R;
+    float m = -INFINITY, mb = 0.f, z = 0.f;
+    uint4 v[R][U];
+    if (r0 < n) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t i = min(r0 + r, n - 1);
+                v[r][u] = load(x + i * ldx, i == n - 1, u * 32 + lane);
+            }
+    }
+    for (; r0 < n; r0 += R * nw) {
+        float s[V];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            uint64_t acc[NQ][2];
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) acc[b][0] = acc[b][1] = 0;
+            // its successor replaces a unit as soon as it is used
+            const int64_t next = min(r0 + R * nw + r, n - 1);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint64_t xv[P];
+                cut(v[r][u], u * 32 + lane);
+                pairs16<T>(v[r][u], xv);
+                v[r][u] = load(x + next * ldx, next == n - 1, u * 32 + lane);
+#pragma unroll
+                for (int b = 0; b < NQ; ++b)
+#pragma unroll
+                    for (int i = 0; i < P; ++i) acc[b][i & 1] = fma_f32x2(xv[i], qv[b][u * P + i], acc[b][i & 1]);
+            }
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) {
+                float a0, a1;
+                unpack2(add_f32x2(acc[b][0], acc[b][1]), a0, a1);
+                s[r * NQ + b] = a0 + a1;
+            }
+        }
+        // each half of the lanes goes on with half of the sums
+#pragma unroll
+        for (int o = 16, k = V; o > 0; o >>= 1) {
+            if (k > 1) {
+                k /= 2;
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i)
+                    if (i < k) {
+                        const float keep = lane & o ? s[i + k] : s[i], give = lane & o ? s[i] : s[i + k];
+                        s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    }
+            } else {
+                s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+            }
+        }
+        const int64_t r = r0 + row;
+        if (r < n && r != tgt) {
+            if (s[0] > m) {
+                z *= ex2((m - s[0]) * c);
+                m = s[0];
+                mb = m * c;
+            }
+            z += ex2(fmaf(s[0], c, -mb));
+        }
+    }
+    // the warp's R sets of a query, in the first lanes' order, then the block's
+#pragma unroll
+    for (int o = 16; o >= kDup * NQ; o >>= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, o), oz = __shfl_xor_sync(0xffffffffu, z, o);
+        join(m, z, om, oz, c);
+    }
+    if (row == 0 && lane % kDup == 0) sj[warp][bq] = make_float2(m, z);
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < nq) {
+        float2 a = sj[0][threadIdx.x];
+        for (int k = 1; k < NT / 32; ++k) join(a.x, a.y, sj[k][threadIdx.x].x, sj[k][threadIdx.x].y, c);
+        part[threadIdx.x * gridDim.x + blockIdx.x] = a;
+    }
 }
 
 // mean or sum of the losses of the queries that count, and their number, by one
@@ -934,7 +1094,7 @@ int64_t piece_rows(int64_t n, int64_t most) {
 
 struct FwdPlan {
     int64_t rows;  // rows per piece
-    bool direct;
+    bool stream, direct;
     int pieces, nqb, nkb, nseg, groups, workers, slots, width, nsplit[2];  // nsplit of a full and of the last piece
 };
 
@@ -958,9 +1118,27 @@ int fwd_splits(int nqb, int64_t rows, int pairs) {
 // reads them; more queries share planes written once per piece.
 bool f32_direct(int dtype, int64_t nq) { return dtype == RDB_F32 && nq <= 128; }
 
+// A pass of CUDA cores where their products hide behind the rows' bytes: one
+// query, or up to four of fp32, whose six products of planes are the tile loop's
+// limit.  Whole forward call, us, streaming / tile loop:
+//   1 query,  bf16, 100,000 x 768   32.2 / 42.8     1M x 768   254 / 268
+//                   200,000 x 384   49 / 49 (shorter rows: equal)
+//   2 queries                       52 / 50                    317 / 268
+//   1 query,  fp32, 100,000 x 768   74 / 150        1M x 768   473 / 1,155
+//   4 queries                       78 / 150                   551 / 1,155
+bool streamed(int dtype, int64_t nq, int d) {
+    return nq >= 1 && nq <= (dtype == RDB_F32 ? 4 : 1) && d <= ST_MAX_DIM;
+}
+
 FwdPlan fwd_plan(int dtype, int64_t nq, int64_t n, int d) {
-    FwdPlan p;
+    FwdPlan p{};
     const int64_t dp = up(d, 8);
+    p.stream = streamed(dtype, nq, d);
+    if (p.stream) {
+        p.pieces = p.groups = 1;
+        p.slots = (int)std::min<int64_t>((n + 31) / 32, (nq == 1 ? 2LL : 1LL) * num_sms());
+        return p;
+    }
     p.direct = f32_direct(dtype, nq);
     // fp32: 256 MB of planes at a time
     p.rows = dtype == RDB_F32 && !p.direct ? piece_rows(n, (256LL << 20) / (6 * dp)) : up(n, 256);
@@ -992,7 +1170,7 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
     const int64_t dp = up(d, 8);
     w.ticket = a.take<unsigned>(1);
     w.part = a.take<float2>((size_t)p.groups * p.slots * nq);
-    if (dtype == RDB_F32) {
+    if (dtype == RDB_F32 && !p.stream) {
         w.qp = a.take<__nv_bfloat16>(3 * nq * dp);
         if (!p.direct) w.xp = a.take<__nv_bfloat16>(3 * p.rows * dp);
     }
@@ -1254,6 +1432,78 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     return RDB_OK;
 }
 
+// (max, sum) of every query's parts
+int tile_pass(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
+              const int64_t* targets, float c, const FwdPlan& p, const FwdWs& w, cudaStream_t s) {
+    static bool attr[64] = {false}, attr_d[64] = {false};
+    if (p.direct)
+        RDB_TRY(tile_f32_smem_attr(xent_scan_f32_kernel, attr_d));
+    else
+        RDB_TRY(tile_smem_attr(xent_scan_kernel, attr));
+    const TileStatus st = tile_status();
+    Planes qo;
+    RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
+    CUtensorMap mq, mx;
+    RDB_TRY(operand_map(&mq, dtype, qo, d, nq, tile_box_rows(nq, 128)));
+    FwdArgs a{};
+    a.q_rows = tile_box_rows(nq, 128);
+    a.width = p.width;
+    a.nq = nq;
+    a.nqb = p.nqb;
+    a.nkb = p.nkb;
+    a.nseg = p.nseg;
+    a.c = c;
+    a.targets = targets;
+    a.groups = p.groups;
+    a.parts = p.slots * p.groups;
+    a.part = w.part;
+    a.ticket = w.ticket;
+    for (int i = 0; i < p.pieces; ++i) {
+        const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
+        a.n = rows;
+        a.row0 = r0;
+        a.n32 = (int)((rows + 31) / 32);
+        a.nsplit = p.nsplit[i == p.pieces - 1];
+        a.slot0 = i * p.nsplit[0];
+        const int64_t units = (int64_t)a.nsplit * p.nqb;
+        RDB_CHECK_ARG(units < (1LL << 31), "too many tiles for one launch");
+        const unsigned workers = (unsigned)std::min<int64_t>(p.workers, units);
+        if (p.direct) {
+            const F32Rows xr{static_cast<const float*>(x), ldx, n, d};
+            RDB_TRY(launch_chained(xent_scan_f32_kernel, workers, TF_THREADS, TF_SMEM, s, mq, xr, a, st));
+        } else {
+            Planes xo;
+            RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
+            RDB_TRY(operand_map(&mx, dtype, xo, d, rows, p.width / 2));
+            RDB_TRY(launch_chained(xent_scan_kernel, 2 * workers, TT_THREADS, TT_SMEM, s, mq, mx, a,
+                                   dtype != RDB_F16, st));
+        }
+    }
+    return RDB_OK;
+}
+
+template <typename T, int NQ>
+int launch_stream(const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
+                  const int64_t* targets, float c, const FwdPlan& p, const FwdWs& w, cudaStream_t s) {
+    constexpr int k = sizeof(T) == 4 ? 2 : 1;  // units of 8 elements
+    const auto kernel = d * (int)sizeof(T) <= 512 ? xent_stream_kernel<T, NQ, 1>
+                        : d <= 256                ? xent_stream_kernel<T, NQ, k>
+                        : d <= 512                ? xent_stream_kernel<T, NQ, 2 * k>
+                        : d <= 768                ? xent_stream_kernel<T, NQ, 3 * k>
+                                                  : xent_stream_kernel<T, NQ, 4 * k>;
+    return launch_chained(kernel, (unsigned)p.slots, NT, 0, s, static_cast<const T*>(q), (int)nq, ldq,
+                          static_cast<const T*>(x), n, ldx, d, targets, c, w.part, w.ticket);
+}
+
+int stream_pass(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
+                const int64_t* targets, float c, const FwdPlan& p, const FwdWs& w, cudaStream_t s) {
+    const auto launch = dtype == RDB_BF16  ? launch_stream<__nv_bfloat16, 1>
+                        : dtype == RDB_F16 ? launch_stream<__half, 1>
+                        : nq == 1          ? launch_stream<float, 1>
+                                           : launch_stream<float, 4>;
+    return launch(q, nq, ldq, x, n, ldx, d, targets, c, p, w, s);
+}
+
 }  // namespace
 }  // namespace rdb
 
@@ -1280,50 +1530,10 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const float c = (float)(scale * kLog2e);
     if (nq > 0) {
-        static bool attr[64] = {false}, attr_d[64] = {false};
-        if (p.direct)
-            RDB_TRY(tile_f32_smem_attr(xent_scan_f32_kernel, attr_d));
+        if (p.stream)
+            RDB_TRY(stream_pass(dtype, q, nq, ldq, x, n, ldx, d, targets, c, p, w, s));
         else
-            RDB_TRY(tile_smem_attr(xent_scan_kernel, attr));
-        const TileStatus st = tile_status();
-        Planes qo;
-        RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
-        CUtensorMap mq, mx;
-        RDB_TRY(operand_map(&mq, dtype, qo, d, nq, tile_box_rows(nq, 128)));
-        FwdArgs a{};
-        a.q_rows = tile_box_rows(nq, 128);
-        a.width = p.width;
-        a.nq = nq;
-        a.nqb = p.nqb;
-        a.nkb = p.nkb;
-        a.nseg = p.nseg;
-        a.c = c;
-        a.targets = targets;
-        a.groups = p.groups;
-        a.parts = p.slots * p.groups;
-        a.part = w.part;
-        a.ticket = w.ticket;
-        for (int i = 0; i < p.pieces; ++i) {
-            const int64_t r0 = i * p.rows, rows = std::min(p.rows, n - r0);
-            a.n = rows;
-            a.row0 = r0;
-            a.n32 = (int)((rows + 31) / 32);
-            a.nsplit = p.nsplit[i == p.pieces - 1];
-            a.slot0 = i * p.nsplit[0];
-            const int64_t units = (int64_t)a.nsplit * p.nqb;
-            RDB_CHECK_ARG(units < (1LL << 31), "too many tiles for one launch");
-            const unsigned workers = (unsigned)std::min<int64_t>(p.workers, units);
-            if (p.direct) {
-                const F32Rows xr{static_cast<const float*>(x), ldx, n, d};
-                RDB_TRY(launch_chained(xent_scan_f32_kernel, workers, TF_THREADS, TF_SMEM, s, mq, xr, a, st));
-            } else {
-                Planes xo;
-                RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
-                RDB_TRY(operand_map(&mx, dtype, xo, d, rows, p.width / 2));
-                RDB_TRY(launch_chained(xent_scan_kernel, 2 * workers, TT_THREADS, TT_SMEM, s, mq, mx, a,
-                                       dtype != RDB_F16, st));
-            }
-        }
+            RDB_TRY(tile_pass(dtype, q, nq, ldq, x, n, ldx, d, targets, c, p, w, s));
         const bool wide = nq <= num_sms();
         const unsigned blocks = (unsigned)std::min<int64_t>(wide ? nq : (nq + NT / 32 - 1) / (NT / 32), 16LL * num_sms());
         const int parts = p.slots * p.groups;
