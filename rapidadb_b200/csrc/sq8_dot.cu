@@ -8,7 +8,7 @@
 //
 // One or two queries: the codes of the rows are what has to be read, so a
 // CUDA-core kernel (dp4a) streams them once past query codes held in shared
-// memory (1M x 768: 124 us, 6.2 TB/s).
+// memory (1M x 768: 117 us, 6.6 TB/s).
 // Otherwise the tcgen05 tile loop (kind::i8) with the rows as the tile's M: few
 // queries then make a narrow tile, and as a thread of the epilogue owns one row,
 // a warp's store of one query's scores is 32 consecutive elements and needs no
@@ -45,15 +45,18 @@ __device__ __forceinline__ float score(float qs, float xs, int acc) {
 
 constexpr int GV_THREADS = 256;
 constexpr int GV_LANES = 8;               // lanes per row: 128 bytes of a row per load
-constexpr int GV_BATCH = 6;               // 16-byte loads a lane has in flight (768 codes: the whole row)
+constexpr int GV_BATCH = 6;               // 16-byte loads a lane has in flight
 constexpr int GV_SMEM = 48 * 1024;        // query codes
 
-// Four rows per warp.
-template <typename T, int NQ>
-__global__ void __launch_bounds__(GV_THREADS)
+// The warps take 4 R rows each in turn (shares of their own, rows far apart, cost
+// 5 to 9 %); a lane reads B 16-byte chunks of each of R rows at a time, the whole
+// of them where R > 1.
+template <typename T, int NQ, int B>
+__global__ void __launch_bounds__(GV_THREADS, GV_BATCH / B > 1 ? 3 : 4)
     sq8_few_kernel(const int8_t* __restrict__ qc, const float* __restrict__ qs, int nq, int64_t ldq,
                    const int8_t* __restrict__ xc, const float* __restrict__ xs, int64_t n, int64_t ldx, int d,
                    T* __restrict__ out, int64_t ldo) {
+    constexpr int R = GV_BATCH / B, kRows = 32 / GV_LANES;
     extern __shared__ __align__(16) int8_t sq[];  // [NQ][dp], zero behind d and behind nq
     chain_wait();
     const int dp = (d + 15) / 16 * 16, chunks = dp / 16;
@@ -64,17 +67,15 @@ __global__ void __launch_bounds__(GV_THREADS)
     __syncthreads();
     const int lane = threadIdx.x & 31, sub = lane & (GV_LANES - 1);
     const int full = d / 16;  // 16-byte chunks that lie inside the row
-    // every warp an equal, contiguous share of the rows, four at a time
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * (GV_THREADS / 32) + threadIdx.x / 32;
-    const int64_t nw = static_cast<int64_t>(gridDim.x) * (GV_THREADS / 32);
-    const int64_t end = (w + 1) * n / nw;
-    // chunk sub + GV_LANES k of GV_BATCH chunks from c0 on
+    // A row's last chunk may reach behind d, but not behind the row's stride, which
+    // is whole chunks: it is read whole, and the query is zero there.  Only the last
+    // row may end with its codes.
     auto load = [&](int64_t r, int c) -> int4 {
         const int8_t* x = xc + r * ldx;
-        if (c < full) return __ldg(reinterpret_cast<const int4*>(x) + c);
+        const bool last = r == n - 1;
+        if (c < (last ? full : chunks)) return __ldg(reinterpret_cast<const int4*>(x) + c);
         uint32_t b[4] = {0u, 0u, 0u, 0u};
-        if (c < chunks) {
-            // the row's last bytes: nothing behind them is read
+        if (last && c < chunks) {
 #pragma unroll
             for (int t = 0; t < 16; ++t)
                 if (c * 16 + t < d)
@@ -82,46 +83,61 @@ __global__ void __launch_bounds__(GV_THREADS)
         }
         return make_int4(b[0], b[1], b[2], b[3]);
     };
-    int64_t r0 = w * n / nw;
-    if (r0 >= end) return;
-    int4 v[GV_BATCH];
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (GV_THREADS / 32) * kRows * R;
+    int64_t r0 = (static_cast<int64_t>(blockIdx.x) * (GV_THREADS / 32) + threadIdx.x / 32) * kRows * R + lane / GV_LANES;
+    int4 v[R][B];
+    float sc[R];
 #pragma unroll
-    for (int k = 0; k < GV_BATCH; ++k) v[k] = load(min(r0 + lane / GV_LANES, end - 1), sub + k * GV_LANES);
-    for (; r0 < end; r0 += 32 / GV_LANES) {
-        const int64_t r = r0 + lane / GV_LANES;
-        int acc[NQ];
+    for (int i = 0; i < R; ++i) {
+        const int64_t r = min(r0 + i * kRows, n - 1);
+        sc[i] = xs[r];
 #pragma unroll
-        for (int b = 0; b < NQ; ++b) acc[b] = 0;
-        for (int c0 = sub; c0 < chunks; c0 += GV_LANES * GV_BATCH) {
-            // the next batch, of this row or of the one after it, replaces every
-            // chunk as soon as it is used: GV_BATCH loads a lane stay in flight
-            const bool more = c0 + GV_LANES * GV_BATCH < chunks;
-            const int64_t rn = min(more ? r : r + 32 / GV_LANES, end - 1);
-            const int cn = more ? c0 + GV_LANES * GV_BATCH : sub;
+        for (int k = 0; k < B; ++k) v[i][k] = load(r, sub + k * GV_LANES);
+    }
+    for (; r0 - lane / GV_LANES < n; r0 += step) {
+        int acc[R][NQ];
 #pragma unroll
-            for (int k = 0; k < GV_BATCH; ++k) {
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int b = 0; b < NQ; ++b) acc[i][b] = 0;
+        for (int c0 = sub; c0 < chunks; c0 += GV_LANES * B) {
+            // the next batch, of this row or of a row of the next step, replaces
+            // every chunk as soon as it is used: GV_BATCH loads a lane stay in flight
+            const bool more = R == 1 && c0 + GV_LANES * B < chunks;
+            const int cn = more ? c0 + GV_LANES * B : sub;
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
                 const int c = min(c0 + k * GV_LANES, chunks - 1);
-                const int4 x = v[k];
+                int4 q[NQ];
 #pragma unroll
-                for (int b = 0; b < NQ; ++b) {
-                    const int4 q = *reinterpret_cast<const int4*>(sq + b * dp + c * 16);
-                    acc[b] = __dp4a(x.x, q.x, acc[b]);
-                    acc[b] = __dp4a(x.y, q.y, acc[b]);
-                    acc[b] = __dp4a(x.z, q.z, acc[b]);
-                    acc[b] = __dp4a(x.w, q.w, acc[b]);
+                for (int b = 0; b < NQ; ++b) q[b] = *reinterpret_cast<const int4*>(sq + b * dp + c * 16);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int4 x = v[i][k];
+#pragma unroll
+                    for (int b = 0; b < NQ; ++b) {
+                        acc[i][b] = __dp4a(x.x, q[b].x, acc[i][b]);
+                        acc[i][b] = __dp4a(x.y, q[b].y, acc[i][b]);
+                        acc[i][b] = __dp4a(x.z, q[b].z, acc[i][b]);
+                        acc[i][b] = __dp4a(x.w, q[b].w, acc[i][b]);
+                    }
+                    v[i][k] = load(min(r0 + i * kRows + (more ? 0 : step), n - 1), cn + k * GV_LANES);
                 }
-                v[k] = load(rn, cn + k * GV_LANES);
             }
         }
 #pragma unroll
-        for (int b = 0; b < NQ; ++b)
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = r0 + i * kRows;
+            const float s = sc[i];
+            sc[i] = xs[min(r + step, n - 1)];
 #pragma unroll
-            for (int o = GV_LANES / 2; o > 0; o >>= 1) acc[b] += __shfl_xor_sync(0xffffffffu, acc[b], o);
-        if (r < end) {
-            const float s = xs[r];
+            for (int b = 0; b < NQ; ++b) {
+                int a = acc[i][b];
 #pragma unroll
-            for (int b = 0; b < NQ; ++b)
-                if (b < nq && (b & (GV_LANES - 1)) == sub) out[b * ldo + r] = from_f<T>(score(qs[b], s, acc[b]));
+                for (int o = GV_LANES / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+                if (((i * NQ + b) & (GV_LANES - 1)) == sub && r < n && b < nq)
+                    out[b * ldo + r] = from_f<T>(score(qs[b], s, a));
+            }
         }
     }
 }
@@ -129,11 +145,16 @@ __global__ void __launch_bounds__(GV_THREADS)
 template <typename T, int NQ>
 int launch_few(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
                int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
-    const int rows = GV_THREADS / GV_LANES;
-    const int64_t blocks = std::min<int64_t>((n + rows - 1) / rows, 4LL * num_sms());
-    const size_t smem = static_cast<size_t>(NQ) * ((d + 15) / 16 * 16);
-    return launch_chained(sq8_few_kernel<T, NQ>, (unsigned)blocks, GV_THREADS, smem, s, qc, qs, (int)nq, ldq, xc, xs, n,
-                          ldx, d, static_cast<T*>(out), ldo);
+    // the whole row in as few loads as it takes, or GV_BATCH at a time: 4M x 128
+    // in 109 us, 2M x 384 in 121 (GV_BATCH for all: 200 and 129)
+    const auto kernel = d <= 128   ? sq8_few_kernel<T, NQ, 1>
+                        : d <= 256 ? sq8_few_kernel<T, NQ, 2>
+                        : d <= 512 ? sq8_few_kernel<T, NQ, 4>
+                                   : sq8_few_kernel<T, NQ, GV_BATCH>;
+    const int64_t rows = GV_THREADS / GV_LANES * (d <= 128 ? 6 : d <= 256 ? 3 : 1);
+    const int64_t blocks = std::min<int64_t>((n + rows - 1) / rows, (d <= 256 ? 3LL : 4LL) * num_sms());
+    return launch_chained(kernel, (unsigned)blocks, GV_THREADS, static_cast<size_t>(NQ) * ((d + 15) / 16 * 16), s, qc, qs,
+                          (int)nq, ldq, xc, xs, n, ldx, d, static_cast<T*>(out), ldo);
 }
 
 // ----------------------------------------------------------- tensor cores --
@@ -263,9 +284,10 @@ int launch_tile(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, cons
 template <typename T>
 int launch_dot(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
                int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
-    // One or two queries: 100,000 x 768 in 9.7 / 12.7 us against 18.6 of the tile
-    // loop (1,000 rows: 3.2 / 5.9).  From four on dp4a costs more than the codes'
-    // bytes: 19.5 us at four, 41 at eight, the tile loop 18.7.
+    // One or two queries: 100,000 x 768 in 8.8 / 11.7 us against 17.8 of the tile
+    // loop (1,000 rows: 2.8 / 5.2; 4M x 128: 109 / 129 us against 287).  From four
+    // on dp4a costs more than the codes' bytes: 150 us for 1M x 768 (4M x 128: 385),
+    // the tile loop 134 (287).
     const int64_t dp = (d + 15) / 16 * 16;
     if (nq == 1 && dp <= GV_SMEM) return launch_few<T, 1>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
     if (nq == 2 && 2 * dp <= GV_SMEM) return launch_few<T, 2>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);

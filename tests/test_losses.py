@@ -224,6 +224,40 @@ def test_loss_and_gradients(device, nq, n, d, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("nq,n,d", [(1, 9000, 100), (1, 700, 250), (4, 5001, 130), (3, 333, 511), (1, 2049, 768),
+                                    (4, 999, 769), (1, 130, 1024), (2, 40, 1025), (1, 1, 999), (2, 31, 1), (1, 7, 129)])
+def test_few_queries(device, nq, n, d, dtype):
+    check_all(*make(nq, n, d, DT[dtype], seed=n + d), scale=6.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("nq", [1, 3])
+@pytest.mark.parametrize("d", [5, 100, 258, 771])
+def test_few_queries_beside_other_values(device, nq, d, dtype):
+    """What lies between the rows does not count, and the last row ends with
+    the memory; ignored queries and targets that are no row as ever."""
+    g = torch.Generator().manual_seed(d)
+    n, ld = 77, (d + 7) // 8 * 8 + 8
+    buf = torch.full(((n - 1) * ld + d,), float("nan"), dtype=DT[dtype], device=device)
+    x = buf.as_strided((n, d), (ld, 1))
+    x.copy_(torch.randn(n, d, generator=g))
+    qbuf = torch.full(((nq - 1) * ld + d,), float("inf"), dtype=DT[dtype], device=device)
+    q = qbuf.as_strided((nq, d), (ld, 1))
+    q.copy_(torch.randn(nq, d, generator=g) / d ** 0.5)
+    t, w = torch.tensor([76, IGN, 0][:nq]), torch.rand(nq, generator=g)
+    got = run_all(q.detach(), x.detach(), t, w, 2.0)
+    r = Ref(q, x, t, 2.0, w)
+    within(got[0], r.loss, r.tol_loss, "loss")
+    within(got[1], r.dq, r.tol_dq, "dq")
+    within(got[2], r.dx, r.tol_dx, "dx")
+    t[0] = n
+    loss = loss_fn(q, x, t.to(device), reduction="none")
+    assert loss[0].isnan() and not loss[1:].isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DT))
 @pytest.mark.parametrize("reduction", ["mean", "sum"])
 def test_reductions(device, dtype, reduction):
     q, x, t, w = make(200, 333, 96, DT[dtype], ignored=31)

@@ -184,6 +184,26 @@ def test_dot_product(device, nq, n, d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nq", [1, 2])
+@pytest.mark.parametrize("n,d", [(1, 5), (9001, 100), (20000, 128), (6001, 129), (501, 256), (4097, 300), (1000, 512),
+                                 (333, 513), (77, 1600), (3, 12289)])
+def test_few_queries(device, nq, n, d, dtype):
+    """Also with other codes between the rows, where the last one ends with the memory."""
+    rng = np.random.default_rng(n + d)
+    qc, qs = codes_of(rng, nq, d)
+    xc, xs = codes_of(rng, n, d)
+    dev = [t.to(device) for t in (qc, qs, xc, xs)]
+    out = _C().sq8_dot_product(*dev, dtype)
+    check(out, qc, qs, xc, xs, dtype)
+    ld = (d + 15) // 16 * 16 + 16
+    buf = torch.full(((n - 1) * ld + d,), 77, dtype=torch.int8, device=device)
+    rows = buf.as_strided((n, d), (ld, 1))
+    rows.copy_(dev[2])
+    assert torch.equal(_C().sq8_dot_product(dev[0], dev[1], rows, dev[3], dtype), out)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("nq", [1, 5, 40, 300])
 def test_extreme_codes_and_long_rows(device, nq):
     """All codes at -128 / 127 and the largest allowed dimension: the integer
