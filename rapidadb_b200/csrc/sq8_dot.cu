@@ -168,9 +168,11 @@ struct DotArgs {
     int x_rows, q_rows;  // box rows
 };
 
-template <typename T>
+// COLS >= nq, or 256
+template <typename T, int COLS>
 struct DotPolicy {
     static constexpr bool kInt8 = true;
+    static constexpr int kAccCols = COLS;
     static constexpr int kStages = 6, kStgBytes = 256;
     // rows are walked in groups of 8 tiles: the tiles in flight form a block of
     // both operands that L2 holds
@@ -211,9 +213,10 @@ struct DotPolicy {
     };
 
     __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx& c) const {
+        if (COLS < TT_N && c.col0 >= j.nn) return;
         const int64_t r = static_cast<int64_t>(j.m0) + c.row;
         e.xs = r < a.n ? a.xs[r] : 0.f;
-        // the query scales of the warp's 64 columns
+        // the query scales of the warp's columns
         float* qs = reinterpret_cast<float*>(c.stg);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -257,27 +260,27 @@ struct DotPolicy {
     __device__ __forceinline__ void finish(const TileCtx&) const {}
 };
 
-template <typename T>
+template <typename T, int COLS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TT_THREADS, 1)
     sq8_tile_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mq,
                     const __grid_constant__ DotArgs a, const TileStatus st) {
     extern __shared__ uint8_t smem_raw[];
-    const DotPolicy<T> p{&mx, &mq, a};
+    const DotPolicy<T, COLS> p{&mx, &mq, a};
     tile_loop(smem_raw, p, false, st);
 }
 
-template <typename T>
+template <typename T, int COLS>
 int launch_tile(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
                 int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
     static bool attr[64] = {false};
-    RDB_TRY(tile_smem_attr(sq8_tile_kernel<T>, attr));
+    RDB_TRY(tile_smem_attr(sq8_tile_kernel<T, COLS>, attr));
     DotArgs a{qs, xs, nq, n, ldo, (int)((nq + TT_N - 1) / TT_N), (int)((n + TT_M - 1) / TT_M), (d + 127) / 128, out,
               tile_box_rows(n, 128), tile_box_rows((nq + 31) / 32 * 16, 128)};
     CUtensorMap mx, mq;
     RDB_TRY(make_map_3d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xc, d, n, 1, ldx, 0, a.x_rows));
     RDB_TRY(make_map_3d(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, qc, d, nq, 1, ldq, 0, a.q_rows));
     const int64_t tiles = (int64_t)a.nqt * a.nxt;
-    return launch_chained(sq8_tile_kernel<T>, 2 * (unsigned)std::min<int64_t>(tile_pairs(), tiles), TT_THREADS, TT_SMEM, s,
+    return launch_chained(sq8_tile_kernel<T, COLS>, 2 * (unsigned)std::min<int64_t>(tile_pairs(), tiles), TT_THREADS, TT_SMEM, s,
                           mx, mq, a, tile_status());
 }
 
@@ -285,13 +288,15 @@ template <typename T>
 int launch_dot(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
                int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
     // One or two queries: 100,000 x 768 in 8.8 / 11.7 us against 17.8 of the tile
-    // loop (1,000 rows: 2.8 / 5.2; 4M x 128: 109 / 129 us against 287).  From four
+    // loop (1,000 rows: 2.8 / 5.2; 4M x 128: 109 / 129 us against 198).  From four
     // on dp4a costs more than the codes' bytes: 150 us for 1M x 768 (4M x 128: 385),
-    // the tile loop 134 (287).
+    // the tile loop 134 (198).
     const int64_t dp = (d + 15) / 16 * 16;
     if (nq == 1 && dp <= GV_SMEM) return launch_few<T, 1>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
     if (nq == 2 && 2 * dp <= GV_SMEM) return launch_few<T, 2>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
-    return launch_tile<T>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
+    // (128 columns: four accumulators measure the same as two of 256)
+    if (nq <= 64) return launch_tile<T, 64>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
+    return launch_tile<T, TT_N>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
 }
 
 }  // namespace

@@ -28,6 +28,12 @@
 // A policy P supplies the tiles and what becomes of them:
 //   P::kInt8                       int8 operands, int32 accumulators
 //   P::kStages, P::kStgBytes       ring stages, staging bytes per epilogue warp
+//   P::kAccCols                    columns of an accumulator: the widest tile.  256: two
+//                                  of them; 64 or 128: eight or four, and the epilogue's
+//                                  warps take turns.  A tile of few columns and K blocks
+//                                  is shorter than the way from its MMAs through the
+//                                  epilogue back to a free accumulator (1M x 128 int8
+//                                  rows, 32 queries: 82 us with two, 56 with eight).
 //   P::Job                         TileJob and what the epilogue needs with it
 //   P::Iter(p, pair, npairs)       the pair's tiles: bool next(job), the same
 //                                  sequence in every role
@@ -55,6 +61,7 @@ namespace {
 constexpr int TT_M = 256;         // rows of a pair's tile
 constexpr int TT_N = 256;         // largest columns of a tile
 constexpr int TT_MAX_STAGES = 7;
+constexpr int TT_MAX_ACCS = 8;    // accumulators of 64 columns in TMEM
 constexpr int TT_A_BYTES = 16384;  // 128 rows x 128 bytes
 constexpr int TT_STAGE_BYTES = 2 * TT_A_BYTES;
 constexpr int TT_BLOCK_BYTES = 8192;  // 64 elements x 64 K rows (MN-major)
@@ -204,11 +211,12 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
                       TT_STAGES * TT_STAGE_BYTES + TT_EPI_WARPS * P::kStgBytes <= TT_MAX_STAGES * TT_STAGE_BYTES,
                   "stages and staging over the block's shared memory");
     uint8_t* stg = smem + TT_STAGES * TT_STAGE_BYTES;
+    static_assert((2 * TT_STAGES + 2 * TT_MAX_ACCS + 1) * 8 + 8 <= TT_BAR_BYTES, "barriers over their bytes");
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + TT_MAX_STAGES * TT_STAGE_BYTES);
     uint64_t* empty = full + TT_STAGES;
     uint64_t* tfull = empty + TT_STAGES;
-    uint64_t* tempty = tfull + 2;
-    uint64_t* mma_done = tempty + 2;
+    uint64_t* tempty = tfull + TT_MAX_ACCS;
+    uint64_t* mma_done = tempty + TT_MAX_ACCS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -223,7 +231,7 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < TT_MAX_ACCS; ++c) {
             mbar_init(&tfull[c], 1);
             mbar_init(&tempty[c], 2 * TT_EPI_WARPS);
         }
@@ -241,6 +249,9 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     static_assert(TT_N / 32 <= 2 * TT_GROUPS, "at most two chunks per epilogue warp");
+    constexpr int kAccs = 512 / P::kAccCols;
+    constexpr bool kNarrow = P::kAccCols <= TT_GROUPS * 32;  // one chunk per epilogue warp at most
+    static_assert(P::kAccCols <= TT_N && kAccs <= TT_MAX_ACCS && (kAccs & (kAccs - 1)) == 0, "accumulators");
 
     if (warp == 0) {
         if (lane == 0) {
@@ -318,13 +329,13 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
             typename P::Job j;
             typename P::Iter it(p, pair, npairs);
             for (; ok && it.next(j); ++tile) {
-                const int acc = tile & 1;
-                if (!mbar_wait(&tempty[acc], ((tile >> 1) & 1) ^ 1, abort_flag)) {
+                const int acc = tile % kAccs;
+                if (!mbar_wait(&tempty[acc], ((tile / kAccs) & 1) ^ 1, abort_flag)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * TT_N);
+                const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * P::kAccCols);
                 const uint32_t idesc =
                     P::kInt8 ? tc_idesc_i8(TT_M, j.nn)
                              : tc_idesc(bf16, TT_M, j.nn) | (j.a_mn ? 1u << 15 : 0u) | (j.b_mn ? 1u << 16 : 0u);
@@ -384,28 +395,31 @@ __device__ __forceinline__ void tile_loop(uint8_t* smem_raw, const P& p, const b
         typename P::Iter it(p, pair, npairs);
         uint32_t tile = 0;
         for (; it.next(j); ++tile) {
-            const int acc = tile & 1;
+            const int acc = tile % kAccs;
+            // the warps of a quadrant take turns at the columns there are
+            if (kNarrow) ctx.col0 = (ctx.grp + static_cast<int>(tile)) % TT_GROUPS * 32;
             p.begin(epi, j, ctx);
-            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (tile >> 1) & 1, abort_flag))) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (tile / kAccs) & 1, abort_flag))) {
                 tt_give_up(abort_flag, st, DEV_TIMEOUT_EPILOGUE);
                 break;
             }
             tc_fence_after();
             const uint32_t tbase =
-                tmem_base + (static_cast<uint32_t>(ctx.quad * 32) << 16) + static_cast<uint32_t>(acc * TT_N);
+                tmem_base + (static_cast<uint32_t>(ctx.quad * 32) << 16) + static_cast<uint32_t>(acc * P::kAccCols);
             uint32_t ra[32], rb[32];
-            // (columns behind a narrow tile hold older values, which no policy uses)
-            tmem_ld32_async(tbase + static_cast<uint32_t>(ctx.col0), ra);
-            tmem_ld32_async(tbase + static_cast<uint32_t>(ctx.col1), rb);
+            // (columns behind a narrow tile hold older values, and columns that its
+            // accumulator does not have are read from its first: no policy uses them)
+            tmem_ld32_async(tbase + static_cast<uint32_t>(!kNarrow || ctx.col0 < P::kAccCols ? ctx.col0 : 0), ra);
+            if (!kNarrow) tmem_ld32_async(tbase + static_cast<uint32_t>(ctx.col1), rb);
             tmem_ld_wait(ra);
-            tmem_ld_wait(rb);
+            if (!kNarrow) tmem_ld_wait(rb);
             tc_fence_before();
             __syncwarp();
             if (lane == 0)
                 mbar_arrive_cluster_relaxed(tempty_lead + static_cast<uint32_t>(acc * sizeof(uint64_t)));
             if (ctx.col0 < j.nn) p.chunk(epi, j, ctx, ctx.col0, ra);
             __syncwarp();
-            if (ctx.col1 < j.nn) p.chunk(epi, j, ctx, ctx.col1, rb);
+            if (!kNarrow && ctx.col1 < j.nn) p.chunk(epi, j, ctx, ctx.col1, rb);
             __syncwarp();
             p.end(epi, j, ctx);
         }

@@ -122,6 +122,7 @@ struct FwdArgs {
 
 struct FwdPolicy {
     static constexpr bool kInt8 = false;
+    static constexpr int kAccCols = TT_N;
     static constexpr int kStages = 7, kStgBytes = 0;
     [[maybe_unused]] static constexpr bool kBMn = false;  // (tile_f32.cuh)
     const CUtensorMap *mq, *mx;
@@ -709,6 +710,7 @@ struct ProbArgs {
 template <typename T>
 struct ProbPolicy {
     static constexpr bool kInt8 = false;
+    static constexpr int kAccCols = TT_N;
     static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
     [[maybe_unused]] static constexpr bool kBMn = false;
     const CUtensorMap *mq, *mx, *mg;
@@ -849,6 +851,7 @@ struct GradArgs {
 template <typename T>
 struct GradPolicy {
     static constexpr bool kInt8 = false;
+    static constexpr int kAccCols = TT_N;
     static constexpr int kStages = 5, kStgBytes = TT_STG_BYTES;
     [[maybe_unused]] static constexpr bool kBMn = true;
     const CUtensorMap *gk, *gmn, *xmn, *qmn, *mpart, *mdx;

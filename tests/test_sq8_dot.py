@@ -204,6 +204,19 @@ def test_few_queries(device, nq, n, d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nq", [3, 31, 32, 33, 64, 65])
+@pytest.mark.parametrize("n,d", [(100_001, 128), (60_000, 1), (40_000, 200)])
+def test_many_short_tiles(device, nq, n, d):
+    """Many more tiles than accumulators, a K block or two each: sums exact in fp32."""
+    g = torch.Generator().manual_seed(nq)
+    qc = torch.randint(-128, 128, (nq, d), generator=g, dtype=torch.int8).to(device)
+    xc = torch.randint(-128, 128, (n, d), generator=g, dtype=torch.int8).to(device)
+    out = _C().sq8_dot_product(qc, torch.ones(nq, device=device), xc, torch.ones(n, device=device))
+    # |sums| < 2^24: products of integers in fp32 are exact in any order
+    assert torch.equal(out.double(), qc.double() @ xc.double().T)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("nq", [1, 5, 40, 300])
 def test_extreme_codes_and_long_rows(device, nq):
     """All codes at -128 / 127 and the largest allowed dimension: the integer
