@@ -12,8 +12,8 @@
 // Otherwise the tcgen05 tile loop (kind::i8) with the rows as the tile's M: few
 // queries then make a narrow tile, and as a thread of the epilogue owns one row,
 // a warp's store of one query's scores is 32 consecutive elements and needs no
-// staging (staged TMA stores measured the same).  32 x 100,000 x 768: 22 us, the
-// codes' bytes; 4,096 x 16,384 x 1,024 in bf16: 70 us, of which the products take
+// staging (staged TMA stores measured the same).  32 x 100,000 x 768: 20 us from
+// a cold L2, the codes' bytes; 4,096 x 16,384 x 1,024 in bf16: 77 us, of which the products take
 // 45 and the conversion and scaling of 67M sums the rest.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -6,7 +6,7 @@
 //   warp 0      TMA producer: per K block of 128 bytes each CTA loads its 128
 //               rows of A and its nn / 2 rows of B into a ring of 5 to 7 stages
 //               (4 to 6 measure the same where the MMAs bound the tile).
-//   warp 1      TMEM (two 256-column accumulators); the leader's lane 0 issues
+//   warp 1      TMEM (two to eight accumulators, P::kAccCols); the leader's lane 0 issues
 //               the MMAs and commits stage releases and finished accumulators.
 //   warps 2..17 epilogue, four per TMEM lane quadrant: a thread owns one row of
 //               its CTA's 128 and every fourth 32-column chunk of the tile (at

@@ -5,7 +5,8 @@
 //   G_bn   = w_b scale (p_bn - [n = t(b)]),    p_bn = exp(s_bn) / sum_n exp(s_bn)
 //   dq = G x,  dx = G^T q
 //
-// Every product runs on the tcgen05 tile loops of tile_tc.cuh and tile_f32.cuh.
+// The products run on the tcgen05 tile loops of tile_tc.cuh and tile_f32.cuh; only a
+// forward pass of one query (fp32: up to four) streams the rows past CUDA cores.
 //
 // Forward: one pass over the rows.  The sum is taken in base 2 around a running
 // maximum in the epilogue of each tile, c = scale log2 e,
