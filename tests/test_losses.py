@@ -634,6 +634,52 @@ def test_offsets_past_32_bits(device, nq):
 
 
 @pytest.mark.gpu
+def test_one_query_past_32_bits(device):
+    """One query, whose rows are streamed, over more than 2^31 elements."""
+    n, d = 2_900_000, 768
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.empty(n, d, dtype=torch.bfloat16, device=device)
+    for part in x.split(500_000):
+        part.copy_(torch.randn(part.shape, generator=g, device=device) / d ** 0.5)
+    edge = 2 ** 31 // d
+    for t in (0, edge, edge + 1, n - 1):
+        q = (x[t:t + 1].float() * 1.5).to(torch.bfloat16)
+        loss = loss_fn(q, x, torch.tensor([t], device=device), scale=10.0).item()
+        s = torch.cat([10.0 * (part.double() @ q[0].double()) for part in x.split(100_000)])
+        want = (torch.logsumexp(s, 0) - s[t]).item()
+        assert abs(loss - want) <= 1e-4 * want, (t, loss, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DT))
+def test_one_query_captured_on_two_streams(device, dtype):
+    """Two captured losses of one query, replayed at once on two streams with
+    inputs that change between the replays."""
+    x = make(5, 3000, 200, DT[dtype])[1].to(device)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    qs = [torch.zeros(1, 200, dtype=DT[dtype], device=device) for _ in side]
+    ts = [torch.zeros(1, dtype=torch.long, device=device) for _ in side]
+    loss_fn(qs[0], x, ts[0])
+    torch.cuda.synchronize()
+    graphs, out = [], []
+    for q, t in zip(qs, ts):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            out.append(loss_fn(q, x, t, scale=4.0))
+    for i in range(8):
+        for k in range(2):
+            qs[k].copy_(x[17 * i + k:17 * i + k + 1] * 2)
+            ts[k].fill_(17 * i + k if i % 3 else 2999 - i)
+        torch.cuda.synchronize()
+        for s, graph in zip(side, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for q, t, o in zip(qs, ts, out):
+            assert torch.equal(o, loss_fn(q, x, t, scale=4.0))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(DT))
 def test_two_threads_at_once(device, dtype):
     from concurrent.futures import ThreadPoolExecutor
