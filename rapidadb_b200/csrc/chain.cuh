@@ -8,6 +8,10 @@
 // Every thread of a kernel launched this way calls chain_wait() before any access
 // to global memory: a kernel then finishes only after all before it, and what
 // follows it in the stream, launched in whichever way, sees all of them finished.
+// Its inputs are loaded by ordinary loads: the kernel is resident while they are
+// still being written, so the read-only path (__ldg, const __restrict__
+// parameters), which takes them as constant for its whole life and is not held
+// back by the wait, is closed to it.
 #pragma once
 
 #include <utility>

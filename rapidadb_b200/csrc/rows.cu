@@ -11,8 +11,8 @@ namespace {
 // one thread per 16-byte unit of the copy, reading W bytes at a time
 template <typename W>
 __global__ void __launch_bounds__(256)
-    pad_rows_kernel(const uint8_t* __restrict__ src, int64_t rows, int64_t row_bytes, int64_t src_stride,
-                    uint4* __restrict__ dst, int64_t units) {
+    pad_rows_kernel(const uint8_t* src, int64_t rows, int64_t row_bytes, int64_t src_stride,
+                    uint4* dst, int64_t units) {
     chain_wait();
     const int64_t total = rows * units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;

@@ -80,7 +80,7 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float scale, float in
 
 template <typename T>
 __device__ __forceinline__ void load16(const void* p, float (&v)[16 / sizeof(T)]) {
-    const uint4 u = __ldg(static_cast<const uint4*>(p));
+    const uint4 u = *static_cast<const uint4*>(p);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -101,8 +101,7 @@ __device__ __forceinline__ void load16(const void* p, float (&v)[16 / sizeof(T)]
 // 768 bf16 in 400 us, 5.8 TB/s (508 us with a division and two conversions each).
 template <typename T, int U>
 __global__ void __launch_bounds__(256)
-    sq8_encode_rows_kernel(const T* __restrict__ x, int64_t n, int64_t ldx, int units, int8_t* __restrict__ codes,
-                           int64_t ldc, float* __restrict__ scales) {
+    sq8_encode_rows_kernel(const T* x, int64_t n, int64_t ldx, int units, int8_t* codes, int64_t ldc, float* scales) {
     constexpr int E = 16 / sizeof(T);  // elements of a unit
     chain_wait();
     const int lane = threadIdx.x & 31;

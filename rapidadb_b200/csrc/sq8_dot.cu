@@ -53,9 +53,8 @@ constexpr int GV_SMEM = 48 * 1024;        // query codes
 // of them where R > 1.
 template <typename T, int NQ, int B>
 __global__ void __launch_bounds__(GV_THREADS, GV_BATCH / B > 1 ? 3 : 4)
-    sq8_few_kernel(const int8_t* __restrict__ qc, const float* __restrict__ qs, int nq, int64_t ldq,
-                   const int8_t* __restrict__ xc, const float* __restrict__ xs, int64_t n, int64_t ldx, int d,
-                   T* __restrict__ out, int64_t ldo) {
+    sq8_few_kernel(const int8_t* qc, const float* qs, int nq, int64_t ldq, const int8_t* xc, const float* xs, int64_t n,
+                   int64_t ldx, int d, T* out, int64_t ldo) {
     constexpr int R = GV_BATCH / B, kRows = 32 / GV_LANES;
     extern __shared__ __align__(16) int8_t sq[];  // [NQ][dp], zero behind d and behind nq
     chain_wait();
@@ -73,7 +72,7 @@ __global__ void __launch_bounds__(GV_THREADS, GV_BATCH / B > 1 ? 3 : 4)
     auto load = [&](int64_t r, int c) -> int4 {
         const int8_t* x = xc + r * ldx;
         const bool last = r == n - 1;
-        if (c < (last ? full : chunks)) return __ldg(reinterpret_cast<const int4*>(x) + c);
+        if (c < (last ? full : chunks)) return reinterpret_cast<const int4*>(x)[c];
         uint32_t b[4] = {0u, 0u, 0u, 0u};
         if (last && c < chunks) {
 #pragma unroll
@@ -86,7 +85,9 @@ __global__ void __launch_bounds__(GV_THREADS, GV_BATCH / B > 1 ? 3 : 4)
     const int64_t step = static_cast<int64_t>(gridDim.x) * (GV_THREADS / 32) * kRows * R;
     int64_t r0 = (static_cast<int64_t>(blockIdx.x) * (GV_THREADS / 32) + threadIdx.x / 32) * kRows * R + lane / GV_LANES;
     int4 v[R][B];
-    float sc[R];
+    float sc[R], sq_b[NQ];
+#pragma unroll
+    for (int b = 0; b < NQ; ++b) sq_b[b] = b < nq ? qs[b] : 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int64_t r = min(r0 + i * kRows, n - 1);
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(GV_THREADS, GV_BATCH / B > 1 ? 3 : 4)
 #pragma unroll
                 for (int o = GV_LANES / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
                 if (((i * NQ + b) & (GV_LANES - 1)) == sub && r < n && b < nq)
-                    out[b * ldo + r] = from_f<T>(score(qs[b], s, a));
+                    out[b * ldo + r] = from_f<T>(score(sq_b[b], s, a));
             }
         }
     }

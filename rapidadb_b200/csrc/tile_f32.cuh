@@ -100,7 +100,7 @@ __device__ __forceinline__ TfSource tf_source(const F32Rows& x, const TileJob& j
 __device__ __forceinline__ float4 tf_load(const TfSource& s, bool mn, int i) {
     const bool in = (mn ? i : 2 * i) < s.rows;
     const float* p = s.p + i * s.step;
-    if (in && s.cols >= 4) return __ldg(reinterpret_cast<const float4*>(p));
+    if (in && s.cols >= 4) return *reinterpret_cast<const float4*>(p);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (in && s.cols > 0) {
         // the row's last columns: nothing behind them is read

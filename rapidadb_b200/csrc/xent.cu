@@ -296,8 +296,8 @@ constexpr int stream_rows(int units) { return units == 1 ? 8 : units <= 3 ? 4 : 
 // a load per use: 50 us instead of 32 for the case below.)
 template <typename T, int NQ, int U>
 __global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
-    xent_stream_kernel(const T* __restrict__ q, int nq, int64_t ldq, const T* __restrict__ x, int64_t n, int64_t ldx,
-                       int d, const int64_t* __restrict__ targets, float c, float2* part, unsigned* ticket) {
+    xent_stream_kernel(const T* q, int nq, int64_t ldq, const T* x, int64_t n, int64_t ldx, int d, const int64_t* targets,
+                       float c, float2* part, unsigned* ticket) {
     constexpr int E = 16 / sizeof(T), P = E / 2;  // elements and pairs of a unit
     constexpr int R = stream_rows(U), V = R * NQ, kDup = 32 / V;
     __shared__ float2 sj[NT / 32][NQ];
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
     // is whole units: it is read whole and cut when it is used.  Only the last row
     // may end with its elements.
     auto load = [&](const T* row, bool last, int u) -> uint4 {
-        if (u < (last ? full : units)) return __ldg(reinterpret_cast<const uint4*>(row) + u);
+        if (u < (last ? full : units)) return reinterpret_cast<const uint4*>(row)[u];
         union {
             uint4 v;
             T e[E];
