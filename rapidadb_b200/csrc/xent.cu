@@ -34,6 +34,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "tile_f32.cuh"
 #include "tile_tc.cuh"
@@ -602,25 +603,67 @@ struct Weights {
     }
 };
 
-// largest |u_b|, by one block (every thread gets it); a NaN makes its own
-// products NaN
-__device__ float largest_weight(const Weights& w, int64_t nq, float* sm) {
-    float mx = 0.f;
+// Largest |u_b| (x) over the queries of one block out of `blocks`, and for fp16 the
+// largest |u_b| max_t |q_bt| (y).  Every thread gets them; a NaN makes its own
+// products NaN.
+template <typename T>
+__device__ float2 largest_weight(const Weights& w, const T* q, int64_t nq, int64_t ldq, int d, int block, int blocks,
+                                 float2* sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float mx = 0.f, my = 0.f;
+    if constexpr (std::is_same<T, __half>::value) {
+        for (int64_t b = block * (NT / 32) + warp; b < nq; b += blocks * (NT / 32)) {
+            const float u = fabsf(w.u(b));
+            if (!(u > 0.f)) continue;  // an ignored query may hold anything
+            float a = 0.f;
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < nq; i += blockDim.x) mx = fmaxf(mx, fabsf(w.u(i)));
+            for (int t = lane * 8; t < d; t += 256) {
+                float v[8];
+                load8(q + b * ldq, t, d, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) a = fmaxf(a, fabsf(v[k]));
+            }
+            mx = fmaxf(mx, u);
+            my = fmaxf(my, u * a);
+        }
+        my = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(my)));
+    } else {
+#pragma unroll 4
+        for (int64_t i = static_cast<int64_t>(block) * NT + threadIdx.x; i < nq; i += static_cast<int64_t>(blocks) * NT)
+            mx = fmaxf(mx, fabsf(w.u(i)));
+    }
     mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = mx;
+    if (lane == 0) sm[warp] = make_float2(mx, my);
     __syncthreads();
-    mx = sm[0];
-    for (int k = 1; k < static_cast<int>(blockDim.x / 32); ++k) mx = fmaxf(mx, sm[k]);
-    return mx;
+    float2 m = sm[0];
+#pragma unroll
+    for (int k = 1; k < NT / 32; ++k) m = make_float2(fmaxf(m.x, sm[k].x), fmaxf(m.y, sm[k].y));
+    return m;
 }
 
-__global__ void __launch_bounds__(1024) xent_wmax_kernel(const Weights w, int64_t nq, float* wmax) {
+constexpr int kWeightBlocks = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(NT)
+    xent_wmax_kernel(const T* q, int64_t nq, int64_t ldq, int d, const Weights w, float2* parts) {
     chain_wait();
-    __shared__ float sm[32];
-    const float mx = largest_weight(w, nq, sm);
-    if (threadIdx.x == 0) *wmax = mx;
+    __shared__ float2 sm[NT / 32];
+    const float2 m = largest_weight(w, q, nq, ldq, d, blockIdx.x, gridDim.x, sm);
+    if (threadIdx.x == 0) parts[blockIdx.x] = m;
+}
+
+// What the weighted queries are multiplied by besides 1 / max |u|.  bf16 (and the
+// planes of fp32) has fp32's exponents: 1.  fp16: the power of two that brings the
+// largest element between 2^14 and 2^15, so that elements keep their 11 bits down
+// to 2^-28 of it, as far as dx itself does.  (At 1 the largest of a unit query of
+// 768 elements is about 0.1, and a query of 1 / 500 of the largest weight is
+// subnormal: rows of dx that only such queries move lost up to all their digits.)
+template <typename T>
+__device__ __forceinline__ float weight_top(const float2& m) {
+    if constexpr (!std::is_same<T, __half>::value) return 1.f;
+    const float r = 32768.f * (m.x / m.y);  // (no less than 1/2: an element is at most 65,504)
+    if (!(m.y > 0.f) || isnan(r)) return 1.f;  // nothing to weigh, or infinite
+    return __uint_as_float(__float_as_uint(fminf(r, 0x1p100f)) & 0x7f800000u);
 }
 
 // the three bf16 planes of 8 floats, plane stride in elements
@@ -642,23 +685,32 @@ __device__ __forceinline__ void store_planes(const float (&v)[8], __nv_bfloat16*
     }
 }
 
-// Queries as an operand of dx = G^T (u q): out[b] = q[b] u_b / max |u|, so that
-// the type's range is used whatever the size of the gradients; zero rows for
-// ignored queries, whatever they hold.  fp32: three bf16 planes.  scan: every
-// block finds max |u| itself (few queries) and the first one leaves it in wmax.
+// Queries as an operand of dx = G^T (u q): out[b] = q[b] u_b / wmax, wmax = max |u|
+// over the above, so that the type's range is used whatever the size of the
+// gradients; zero rows for ignored queries, whatever they hold.  fp32: three bf16
+// planes.  nparts: sets of largest weights; 0: every block finds them itself (few
+// queries).  The first block leaves wmax behind.
 template <typename T>
 __global__ void __launch_bounds__(NT)
-    xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const Weights w, bool scan, float* wmax, void* out,
-                         int64_t ldo) {
+    xent_weighted_kernel(const T* q, int64_t nq, int64_t ldq, int d, const Weights w, const float2* parts, int nparts,
+                         float* wmax, void* out, int64_t ldo) {
     chain_wait();
-    __shared__ float sm[NT / 32];
-    float mx;
-    if (scan) {
-        mx = largest_weight(w, nq, sm);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *wmax = mx;
+    __shared__ float2 sm[NT / 32];
+    float2 m = make_float2(0.f, 0.f);
+    if (!std::is_same<T, __half>::value && nparts == 0) {
+        m = largest_weight(w, q, nq, ldq, d, 0, 1, sm);
     } else {
-        mx = *wmax;
+#pragma unroll
+        for (int k = 0; k < kWeightBlocks / 32; ++k) {
+            const int i = k * 32 + (threadIdx.x & 31);
+            const float2 v = i < nparts ? parts[i] : make_float2(0.f, 0.f);
+            m = make_float2(fmaxf(m.x, v.x), fmaxf(m.y, v.y));
+        }
+        m.x = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m.x)));
+        m.y = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m.y)));
     }
+    const float mx = m.x, top = weight_top<T>(m);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *wmax = mx / top;
     const int64_t units = ldo / 8, total = nq * units;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * NT) {
@@ -670,7 +722,7 @@ __global__ void __launch_bounds__(NT)
             for (int k = 0; k < 8; ++k) v[k] = 0.f;
         } else {
             load8(q + b * ldq, t, d, v);
-            const float u = w.u(b), f = u == 0.f ? 0.f : u / mx;
+            const float u = w.u(b), f = u == 0.f ? 0.f : u / mx * top;
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] *= f;
         }
@@ -1247,6 +1299,7 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
 
 struct BwdWs {
     float *wmax, *part;
+    float2* wparts;
     void *g, *qw;
     __nv_bfloat16 *qp, *xp;
     size_t bytes;
@@ -1257,6 +1310,7 @@ BwdWs bwd_ws(void* base, const BwdPlan& p, int dtype, int64_t nq, int d, bool ne
     Arena a{static_cast<char*>(base)};
     const int64_t d8 = up(d, 8);
     w.wmax = a.take<float>(1);
+    if (need_dx) w.wparts = a.take<float2>(kWeightBlocks);
     w.g = a.take<uint16_t>((size_t)p.planes * nq * p.rows);
     if (need_dq) w.part = a.take<float>((size_t)p.q_split * nq * p.dp);
     if (need_dx) w.qw = a.take<uint16_t>((size_t)p.planes * nq * d8);
@@ -1291,6 +1345,13 @@ int split_rows(const void* x, int64_t n, int64_t ldx, int d, __nv_bfloat16* out,
                            static_cast<const float*>(x), n, ldx, d, out, up(d, 8)));
     return RDB_OK;
 }
+
+// Whether every block of the weighted queries' launch finds the largest weight
+// itself, or a launch before it does.  Captured backward pass, us, itself / before:
+// 256 x 256 x 768 bf16 20.8 / 22.5, 1,024 x 1,024 x 256 24.6 / 24.8, 2,048 x 4,096 x
+// 128 34.7 / 32.8.  fp16, which reads the queries for it: always before (77 x 5,003
+// x 100 30.7 / 24.6).
+bool scan_weights(int dtype, int64_t nq) { return dtype != RDB_F16 && nq <= 1024; }
 
 // rows [r0, r0 + rows) as operand planes (fp32: split into xp first)
 int piece_operand(int dtype, const void* x, int64_t r0, int64_t rows, int64_t ldx, int d, __nv_bfloat16* xp, Planes* o,
@@ -1330,14 +1391,17 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
                      ignore,
                      reduction != RDB_REDUCE_NONE};
     if (dx) {
-        const bool scan = nq <= 2048;
+        const bool scan = scan_weights(dtype, nq);
+        const int per = dtype == RDB_F16 ? NT / 32 : NT;  // queries a block reads at a time
+        const int nparts = scan ? 0 : (int)std::min<int64_t>(kWeightBlocks, (nq + per - 1) / per);
         if (!scan) {
-            RDB_TRY(launch_chained(xent_wmax_kernel, 1, 1024, 0, s, wt, nq, w.wmax));
+            RDB_TRY(launch_chained(xent_wmax_kernel<T>, nparts, NT, 0, s, static_cast<const T*>(q), nq, ldq, d, wt,
+                                   w.wparts));
         }
         const int64_t items = nq * d8 / 8;
         RDB_TRY(launch_chained(xent_weighted_kernel<T>,
                                scan ? (unsigned)std::min<int64_t>((items + NT - 1) / NT, num_sms()) : elementwise_blocks(items),
-                               NT, 0, s, static_cast<const T*>(q), nq, ldq, d, wt, scan, w.wmax, w.qw, d8));
+                               NT, 0, s, static_cast<const T*>(q), nq, ldq, d, wt, w.wparts, nparts, w.wmax, w.qw, d8));
     }
     Planes qo;
     RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));

@@ -1,0 +1,121 @@
+"""Softmax cross entropy: digits of the gradients where weights differ by orders
+of magnitude.
+
+Tolerances as in test_losses.py; what is added to them is derived at each test.
+"""
+import pytest
+import torch
+from test_losses import Ref, U32, UNDERFLOW, half_step, make, run_all, within
+
+
+def fp16_row_tolerance(r, q, x, t, scale, w):
+    """Ref's tolerance of dx with the weighted queries of fp16 rounded in steps of
+    2^-25 below 2^-14, the largest of them between 2^14 and 2^15: those steps are
+    2^-39 of max_b |u_b| max_t |q_bt|, u_b = w_b (1 - p_t), and not 2^-25 of max |u_b|."""
+    u, sub = half_step(torch.float16), 2.0 ** -25
+    qd, xd = q.double(), x.double()
+    keep, (n, d) = t >= 0, x.shape
+    qd = torch.where(keep[:, None], qd, torch.zeros_like(qd))
+    s = scale * (qd @ xd.T)
+    p = torch.softmax(s, 1)
+    rest = -torch.expm1(-r.loss)
+    p[torch.arange(len(t)), t.clamp(min=0)] = -rest
+    u_b = torch.where(keep, w.double().abs(), torch.zeros(len(t), dtype=torch.float64)) * rest
+    smax = s.abs().max().item()
+    dp = 2 * scale * (d + 4) * U32 * (qd.abs() @ xd.abs().T).max().item() + (n + 16 + 4 * smax) * U32
+    pg = torch.where(rest[:, None] > 0, p.abs() / rest[:, None], torch.zeros_like(p)) * keep[:, None]  # |G| / u_b
+    return 1.01 * ((2 * u + dp + len(t) * U32) * scale * (pg.T @ (u_b[:, None] * qd.abs())) + u * r.dx.abs() +
+                   sub * 2.0 ** -14 * scale * (u_b[:, None] * qd.abs()).sum(0)[None, :] +
+                   sub * 2.0 ** -14 * scale * (u_b * qd.abs().amax(1)).max().item() * pg.sum(0)[:, None]) + sub + UNDERFLOW
+
+
+def steep(nq, lo, hi, seed):
+    """Weights spread evenly over the orders of two between 2^lo and 2^hi, of both signs."""
+    g = torch.Generator().manual_seed(seed)
+    return torch.exp2(lo + (hi - lo) * torch.rand(nq, generator=g)) * torch.where(torch.rand(nq, generator=g) < 0.5, -1.0, 1.0)
+
+
+# the largest element of dx, scale * w * max |q| (about 0.2), stays below 65504
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,n,d,scale,lo,hi", [(256, 4096, 768, 20.0, -4, 13), (256, 4096, 768, 40.0, -6, 12),
+                                                (60, 700, 100, 20.0, -4, 13), (2100, 3000, 64, 10.0, -4, 13),
+                                                (3, 500, 64, 10.0, -6, 13), (33, 90, 1030, 6.0, -3, 14)])
+def test_fp16_rows_gradient_under_unequal_weights(device, nq, n, d, scale, lo, hi):
+    """Every row of dx is as exact as its own digits allow, whatever the weights
+    of other queries are."""
+    q, x, t, _ = make(nq, n, d, torch.float16, seed=nq + n, ignored=nq // 9)
+    w = steep(nq, lo, hi, nq)
+    dx = run_all(q, x, t, w, scale)[2]
+    r = Ref(q, x, t, scale, w)
+    assert r.dx.abs().max().item() < 60000.0
+    within(dx, r.dx, fp16_row_tolerance(r, q, x, t, scale, w), "dx")
+
+
+def pairs(nq, d, seed, found):
+    """Query b lies between rows 2 b (its target) and 2 b + 1 alone, closer to the
+    target by found[b], and far from all others: their two rows of dx are its own."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.linalg.qr(torch.randn(d, 2 * nq, generator=g, dtype=torch.float64))[0].T.contiguous()
+    noise = torch.randn(nq, d, generator=g, dtype=torch.float64)
+    noise -= noise @ x.T @ x
+    q = (0.7 + found[:, None]) * x[::2] + 0.7 * x[1::2] + 0.3 * torch.nn.functional.normalize(noise, dim=1)
+    return q.half(), x.half(), 2 * torch.arange(nq)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,d", [(100, 768), (30, 100), (3, 64)])
+def test_fp16_rows_of_light_queries(device, nq, d):
+    """Rows that only a query of small weight moves, next to queries of up to 2^21
+    times its weight."""
+    q, x, t = pairs(nq, d, nq, torch.zeros(nq, dtype=torch.float64))
+    w = steep(nq, -8, 13, nq)
+    w[0], w[-1] = 2.0 ** 13, 2.0 ** -8
+    scale = 40.0
+    dx = run_all(q, x, t, w, scale)[2]
+    r = Ref(q, x, t, scale, w)
+    assert r.dx.abs().max().item() < 65000.0
+    within(dx, r.dx, fp16_row_tolerance(r, q, x, t, scale, w), "dx")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq,d", [(100, 768), (30, 100)])
+def test_fp16_rows_gradient_of_trained_queries(device, nq, d):
+    """Queries whose 1 - p_t goes from 1/2 down to 1e-7, under one loss scale: every
+    row of dx in norm.  Three independent roundings of 0.41 half steps in the mean,
+    sqrt(3) of that, and the cut of the logits (below 2^-13 of p) beside it."""
+    scale = 40.0
+    q, x, t = pairs(nq, d, 5, torch.linspace(0.0, 0.4, nq, dtype=torch.float64))
+    w = torch.full((nq,), 4096.0)
+    dx = run_all(q, x, t, w, scale)[2].cpu().double()
+    r = Ref(q, x, t, scale, w)
+    norm = r.dx.norm(dim=1)
+    assert norm.min().item() > 2.0 ** -14 * d ** 0.5  # elements of fp16's normal range
+    err = (dx - r.dx).norm(dim=1) / norm
+    assert err.max().item() < 1.25 * half_step(torch.float16), err.max().item()
+
+
+@pytest.mark.gpu
+def test_fp16_rows_gradient_of_odd_queries(device):
+    """Zero queries, tiny ones, ones next to the largest, with weights to match:
+    no overflow on the way, and nothing of the others is lost."""
+    n, d, scale = 64, 40, 2.0 ** -12
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(n, d, generator=g).half()
+    q = torch.randn(12, d, generator=g).half()
+    q[0] = 0
+    q[1] *= 2.0 ** -20
+    q[2] = (torch.randn(d, generator=g) * 8000).half()
+    t = torch.arange(12)
+    for w in (torch.ones(12), torch.tensor([1e30] + [1.0] * 11), torch.tensor([1.0, 1e12, 2.0 ** -10] + [1.0] * 9),
+              torch.tensor([1e-30] * 12), torch.zeros(12)):
+        dx = run_all(q, x, t, w, scale)[2]
+        r = Ref(q, x, t, scale, w)
+        inside = r.dx.abs() < 60000.0
+        tol = torch.where(inside, fp16_row_tolerance(r, q, x, t, scale, w), torch.full_like(r.dx, float("inf")))
+        got = dx.cpu().double()
+        assert not got.isnan().any()
+        assert ((got - r.dx).abs() <= tol)[inside].all(), w
+    for bad in (float("inf"), float("nan")):
+        w = torch.ones(12)
+        w[5] = bad
+        assert run_all(q, x, t, w, scale)[2].isnan().all()
