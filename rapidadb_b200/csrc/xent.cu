@@ -427,16 +427,17 @@ __global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
 }
 
 // mean or sum of the losses of the queries that count, and their number, by one
-// block in index order
+// block in index order; in 64 bits, since a thread's part of many queries is one
+// long chain (in fp32 the sum of 2^20 losses was off by 4e-5)
 __device__ void reduce_losses(float* stats, const int64_t* targets, int64_t ignore, int64_t nq, int reduction,
-                              float* total, float* ss, int* sc) {
-    float s = 0.f;
+                              float* total, double* ss, int* sc) {
+    double s = 0.;
     int cnt = 0;
 #pragma unroll 8
     for (int64_t i = threadIdx.x; i < nq; i += NT) {
         const float l = __ldcg(stats + 2 * nq + i);
         const bool counts = targets[i] != ignore;
-        s += counts ? l : 0.f;
+        s += counts ? static_cast<double>(l) : 0.;
         cnt += counts;
     }
 #pragma unroll
@@ -446,7 +447,7 @@ __device__ void reduce_losses(float* stats, const int64_t* targets, int64_t igno
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < NT / 32; ++w) ss[0] += ss[w], sc[0] += sc[w];
-        *total = reduction == RDB_REDUCE_MEAN ? ss[0] / static_cast<float>(sc[0]) : ss[0];
+        *total = static_cast<float>(reduction == RDB_REDUCE_MEAN ? ss[0] / sc[0] : ss[0]);
         stats[3 * nq] = static_cast<float>(sc[0]);
     }
 }
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(NT)
                      float* loss, int reduction, float* total, unsigned* ticket) {
     chain_wait();
     __shared__ float2 sj[NT / 32];
-    __shared__ float ss[NT / 32];
+    __shared__ double ss[NT / 32];
     __shared__ int sc[NT / 32];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -579,7 +580,7 @@ __global__ void __launch_bounds__(NT)
 __global__ void __launch_bounds__(NT)
     xent_reduce_kernel(const int64_t* targets, int64_t ignore, int64_t nq, int reduction, float* stats, float* total) {
     chain_wait();
-    __shared__ float ss[NT / 32];
+    __shared__ double ss[NT / 32];
     __shared__ int sc[NT / 32];
     reduce_losses(stats, targets, ignore, nq, reduction, total, ss, sc);
 }

@@ -1,11 +1,11 @@
 """Softmax cross entropy: digits of the gradients where weights differ by orders
-of magnitude.
+of magnitude, and of long sums.
 
 Tolerances as in test_losses.py; what is added to them is derived at each test.
 """
 import pytest
 import torch
-from test_losses import Ref, U32, UNDERFLOW, half_step, make, run_all, within
+from test_losses import IGN, Ref, U32, UNDERFLOW, half_step, loss_fn, make, run_all, within
 
 
 def fp16_row_tolerance(r, q, x, t, scale, w):
@@ -119,3 +119,21 @@ def test_fp16_rows_gradient_of_odd_queries(device):
         w = torch.ones(12)
         w[5] = bad
         assert run_all(q, x, t, w, scale)[2].isnan().all()
+
+
+# ------------------------------------------------------------------ long sums
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 777, 2 ** 20 + 3])
+def test_reduced_loss_is_the_sum_of_the_losses(device, nq):
+    """Mean and sum are rounded once from a 64-bit sum of the losses that
+    reduction="none" gives (2 u32 for the rounding and the mean's division)."""
+    g = torch.Generator(device="cuda").manual_seed(nq)
+    q = torch.rand(nq, 16, generator=g, device=device)
+    x = torch.rand(9, 16, generator=g, device=device)
+    t = torch.randint(0, 9, (nq,), generator=g, device=device)
+    t[1::7] = IGN
+    each = loss_fn(q, x, t, reduction="none").double()
+    count = (t != IGN).sum().item()
+    total = each.sum().item()
+    assert abs(loss_fn(q, x, t, reduction="sum").item() - total) <= 2 * U32 * total
+    assert abs(loss_fn(q, x, t).item() - total / count) <= 2 * U32 * total / count
