@@ -898,9 +898,21 @@ struct GradArgs {
     void* dx;              // rows of the piece, where dx_tma is false
     int64_t lddx;
     bool dx_tma;           // the rows of dx have 16-byte strides
+    bool dx_sums;          // dx in 16 bits goes to fp32 sums first, by mdx
     float scale;
     const float* wmax;     // what dx has to be multiplied with besides
 };
+
+// A tile's K axis is walked in runs of this many blocks of 64, added up in rounded
+// fp32 where the result lies, by the one CTA that owns the tile: the tensor cores
+// cut an accumulator towards zero at every instruction (four a block), by 1e-7 of
+// the final sum each where all terms have one sign (dq over 2^25 rows in one run a
+// split: 3.3e-3 too small).  fp32: 32 cuts of the large accumulator.  16 bits: 512,
+// 5e-5, where the result is rounded by up to 5e-4 (fp16); backward of 4,096 x
+// 131,072 x 768 bf16 1,876 us, 1,853 in one run, 1,919 in runs of 64 blocks.  dx in
+// 16 bits is stored after one run, and only more than 8,192 queries need fp32 sums
+// beside it.
+constexpr int kRun32 = 8, kRun16 = 128;
 
 template <typename T>
 struct GradPolicy {
@@ -915,10 +927,7 @@ struct GradPolicy {
         bool is_dx, more;  // more: adds to what this CTA stored before
         int split;
     };
-    // Of fp32 operands a tile's K axis is walked in runs of 8 blocks (32 cuts of
-    // the large accumulator), added up in rounded fp32 where the result lies, by
-    // the one CTA that owns the tile.
-    static constexpr int kRun = sizeof(T) == 4 ? 8 : 1 << 30;
+    static constexpr int kRun = sizeof(T) == 4 ? kRun32 : kRun16;
     struct Iter {
         const GradPolicy& p;
         int i, step, left;  // K blocks of the last tile still to do
@@ -996,7 +1005,7 @@ struct GradPolicy {
             if (x + c.lane < a.d)
                 for (int i = 0; i < rows; ++i, o += a.lddx) {
                     float v = t[i * 32 + ((c.lane + i) & 31)];
-                    if (kRun < 1 << 30 && j.more) v += to_f(*o);
+                    if (sizeof(T) == 4 && j.more) v += to_f(*o);
                     *o = from_f<T>(v);
                 }
             __syncwarp();
@@ -1008,7 +1017,7 @@ struct GradPolicy {
             stg_wait_read(c.lane);
         bool wide = true;
         if constexpr (sizeof(T) == 2) {
-            if (j.is_dx) {
+            if (j.is_dx && !a.dx_sums) {
                 wide = false;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -1085,6 +1094,24 @@ __global__ void __launch_bounds__(NT)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (t + k < d) dq[b * lddq + t + k] = from_f<T>(skip ? 0.f : o[k]);
+    }
+}
+
+// dx in 16 bits from its sums in fp32
+template <typename T>
+__global__ void __launch_bounds__(NT)
+    xent_dx_kernel(const float* sums, int64_t n, int d, int dp, T* dx, int64_t lddx) {
+    chain_wait();
+    const int64_t units = dp / 4, total = n * units;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * NT) {
+        const int64_t r = i / units;
+        const int t = static_cast<int>(i - r * units) * 4;
+        const float4 v = *reinterpret_cast<const float4*>(sums + r * dp + t);
+        const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (t + k < d) dx[r * lddx + t + k] = from_f<T>(o[k]);
     }
 }
 
@@ -1238,6 +1265,7 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
 struct BwdPlan {
     int64_t rows;  // rows per piece
     bool direct;   // fp32 rows split on the way (dq, probabilities)
+    bool dx_sums;  // dx of a piece in fp32 first
     int pieces, planes, nqb, nt, nkb, nseg, kq, dp;
     int q_nt, q_width, q_split, q_per;  // dq: column tiles, K splits, K blocks per split
     bool q_first;
@@ -1267,6 +1295,7 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
     p.nkb = (d + 63) / 64;
     p.kq = (int)((nq + 63) / 64);
     p.dp = (int)up(d, 32);
+    p.dx_sums = need_dx && dtype != RDB_F32 && p.kq > kRun16;
     p.q_width = p.direct ? TF_N : TT_N;
     p.q_nt = (d + p.q_width - 1) / p.q_width;
     // K splits of dq: the split that ends first, tiles dealt out in turn; a
@@ -1299,7 +1328,7 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
 }
 
 struct BwdWs {
-    float *wmax, *part;
+    float *wmax, *part, *dx;
     float2* wparts;
     void *g, *qw;
     __nv_bfloat16 *qp, *xp;
@@ -1315,6 +1344,7 @@ BwdWs bwd_ws(void* base, const BwdPlan& p, int dtype, int64_t nq, int d, bool ne
     w.g = a.take<uint16_t>((size_t)p.planes * nq * p.rows);
     if (need_dq) w.part = a.take<float>((size_t)p.q_split * nq * p.dp);
     if (need_dx) w.qw = a.take<uint16_t>((size_t)p.planes * nq * d8);
+    if (p.dx_sums) w.dx = a.take<float>((size_t)p.rows * p.dp);
     if (dtype == RDB_F32) {
         w.qp = a.take<__nv_bfloat16>(3 * nq * d8);
         if (!p.direct) w.xp = a.take<__nv_bfloat16>(3 * p.rows * d8);
@@ -1432,7 +1462,8 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
     ga.kq = p.kq;
     ga.q_first = p.q_first;
     ga.lddx = lddx;
-    ga.dx_tma = dx && (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (lddx * (int64_t)sizeof(T)) % 16 == 0;
+    ga.dx_sums = p.dx_sums;
+    ga.dx_tma = p.dx_sums || (dx && (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (lddx * (int64_t)sizeof(T)) % 16 == 0);
     ga.scale = scale;
     ga.wmax = w.wmax;
     const Planes go{w.g, p.rows, nq * p.rows, p.planes};
@@ -1472,7 +1503,9 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         ga.q_split = (ga.kc + p.q_per - 1) / p.q_per;
         ga.add = i > 0;
         ga.dx = dx ? static_cast<T*>(dx) + r0 * lddx : nullptr;
-        if (ga.dx_tma)
+        if (p.dx_sums)
+            RDB_TRY(make_store_map(&mdx, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, w.dx, p.dp, rows, 1, 4LL * p.dp, 0));
+        else if (ga.dx_tma)
             RDB_TRY(make_store_map(&mdx, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : map_type(dtype),
                                    (int)sizeof(T), ga.dx, d, rows, 1, lddx * (int64_t)sizeof(T), 0));
         if (p.direct && dq) {
@@ -1493,6 +1526,11 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         RDB_CHECK_ARG(jobs < (1LL << 31), "too many tiles for one launch");
         RDB_TRY(launch_chained(xent_grad_kernel<T>, 2 * (unsigned)std::min<int64_t>(pairs, jobs), TT_THREADS, TT_SMEM,
                                s, mgk, mgmn, mxmn, mqw, mpart, mdx, ga, bf16, st));
+        if constexpr (sizeof(T) == 2) {
+            if (p.dx_sums)
+                RDB_TRY(launch_chained(xent_dx_kernel<T>, elementwise_blocks(rows * p.dp / 4), NT, 0, s, w.dx, rows, d,
+                                       p.dp, static_cast<T*>(ga.dx), lddx));
+        }
     }
     if (dq) {
         RDB_TRY(launch_chained(xent_dq_kernel<T>, elementwise_blocks(nq * p.dp / 4), NT, 0, s, w.part, p.q_split, nq,

@@ -5,7 +5,7 @@ Tolerances as in test_losses.py; what is added to them is derived at each test.
 """
 import pytest
 import torch
-from test_losses import IGN, Ref, U32, UNDERFLOW, half_step, loss_fn, make, run_all, within
+from test_losses import DT, IGN, Ref, U32, UNDERFLOW, half_step, loss_fn, make, run_all, within
 
 
 def fp16_row_tolerance(r, q, x, t, scale, w):
@@ -137,3 +137,53 @@ def test_reduced_loss_is_the_sum_of_the_losses(device, nq):
     total = each.sum().item()
     assert abs(loss_fn(q, x, t, reduction="sum").item() - total) <= 2 * U32 * total
     assert abs(loss_fn(q, x, t).item() - total / count) <= 2 * U32 * total / count
+
+
+# An accumulator of the tensor cores is cut towards zero at every instruction (16
+# products), by 2^-23 of itself in the mean and less than 2^-22.  A run of up to 8,192
+# products is 512 instructions, over which the sum grows: it loses at most
+# 512 * 2^-22 / 2 = 2^-14 of itself, and half of that in the mean.  The joins of the
+# runs are rounded to either side: 2^7 of them a split here, 2^-18 in the worst case.
+LONG = 2.0 ** -14
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("nq", [1, 3])
+def test_query_gradient_over_many_rows(device, nq, dtype):
+    """2^25 rows of equal logits (zero queries): dq is their mean, G the exact
+    2^-11, so that only the sum and the last rounding are off."""
+    n, d = 2 ** 25 + 1, 16
+    g = torch.Generator(device="cuda").manual_seed(nq)
+    x = torch.empty(n, d, dtype=DT[dtype], device=device)
+    for part in x.split(2 ** 22):
+        part.copy_(torch.rand(part.shape, generator=g, device=device) * 0.5 + torch.linspace(0.5, 1.0, d, device=device))
+    x[-1] = 0
+    q = torch.zeros(nq, d, dtype=DT[dtype], device=device, requires_grad=True)
+    t = torch.full((nq,), n - 1, device=device)
+    dq, = torch.autograd.grad(loss_fn(q, x, t, scale=1.0, reduction="sum"), q)
+    want = sum(part.double().sum(0) for part in x.split(2 ** 22)) / n
+    tol = (half_step(DT[dtype]) + LONG) * want
+    assert ((dq.double() - want).abs() <= tol).all(), ((dq.double() - want).abs() / want).max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim", [16, 19])
+def test_row_gradient_of_many_queries(device, dim, dtype):
+    """2^20 queries against zero rows: p = 1/65, G the exact 256, every row that is
+    no target has dx = scale / 65 of the queries' sum.  The weighted queries are
+    rounded besides, independently: half a step over sqrt(2^20), 2^-19 at 2^-8."""
+    nq, n, scale = 2 ** 20, 65, 2.0 ** -8
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    q = (torch.rand(nq, dim, generator=g, device=device) * 0.5 + torch.linspace(0.5, 1.0, dim, device=device)).to(DT[dtype])
+    x = torch.zeros(n, dim, dtype=DT[dtype], device=device, requires_grad=True)
+    t = torch.zeros(nq, dtype=torch.long, device=device)
+    loss = loss_fn(q, x, t, scale=scale, reduction="sum")
+    want = scale * q.double().sum(0) / n
+    assert abs(loss.item() / nq - torch.log(torch.tensor(65.0)).item()) < 1e-4
+    dx, = torch.autograd.grad(loss, x)
+    tol = (half_step(DT[dtype]) + LONG + 2.0 ** -16) * want
+    assert ((dx[1:].double() - want).abs() <= tol).all(), ((dx[1:].double() - want).abs() / want).max().item()
+    # the target's row: (p - 1) of every query
+    assert ((dx[0].double() + (n - 1) * want).abs() <= (n - 1) * tol).all()
