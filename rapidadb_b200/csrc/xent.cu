@@ -5,8 +5,10 @@
 //   G_bn   = w_b scale (p_bn - [n = t(b)]),    p_bn = exp(s_bn) / sum_n exp(s_bn)
 //   dq = G x,  dx = G^T q
 //
-// The products run on the tcgen05 tile loops of tile_tc.cuh and tile_f32.cuh; only a
-// forward pass of one query (fp32: up to four) streams the rows past CUDA cores.
+// The products run on the tcgen05 tile loops of tile_tc.cuh and tile_f32.cuh; only
+// the logits of one query (fp32: up to four) come from rows streamed past CUDA
+// cores, in the forward and in the backward pass: G then divides terms by a sum of
+// the very same ones.
 //
 // Forward: one pass over the rows.  The sum is taken in base 2 around a running
 // maximum in the epilogue of each tile, c = scale log2 e,
@@ -266,6 +268,26 @@ __global__ void __launch_bounds__(TF_THREADS, 1)
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0u;
 }
 
+// What turns a query's logits into its row of G, 2^14 (p - [n = t]) / (1 - p_t): the
+// terms 2^(c <q, x> - m - lz), -2^14 at the target, or nothing.  Two roundings, of
+// the exponent relative to the largest logit and of the one relative to their sum:
+// both small for the terms that count.
+struct GTerm {
+    float m, lz;
+    int64_t tgt;  // target as a row of the piece (any value: not there)
+    bool zero;    // an ignored query, one whose target is certain, or none
+    __device__ __forceinline__ GTerm() : m(0.f), lz(0.f), tgt(-1), zero(true) {}
+    __device__ __forceinline__ GTerm(const float* stats, const int64_t* targets, int64_t b, int64_t nq, int64_t ignore,
+                                     int64_t row0) {
+        const int64_t t = targets[b];
+        const float rest = -expm1f(-stats[2 * nq + b]);  // 1 - p_t
+        zero = t == ignore || rest == 0.f;
+        tgt = zero ? -1 : t - row0;
+        m = stats[b];
+        lz = stats[nq + b] + log2f(rest) - kGLog2;
+    }
+};
+
 // ---- the same for a few queries, without tensor cores
 
 constexpr int ST_MAX_DIM = 1024;  // 32 elements of every query a lane
@@ -294,16 +316,29 @@ constexpr int stream_rows(int units) { return units == 1 ? 8 : units <= 3 ? 4 : 
 // are up to 20 % slower).  The products are fp32 fma chains; the lanes' sums of
 // R x NQ products are joined so that each lane ends up with one of them, whose
 // (m, z) it keeps.  One part per query and block.  (Queries in shared memory cost
-// a load per use: 50 us instead of 32 for the case below.)
-template <typename T, int NQ, int U>
+// a load per use: 50 us instead of 32 for 100,000 x 768 bf16.)
+// PROB: the backward pass, which writes G of a piece of the rows instead.  (From
+// the tile loop's logits, whose sums are cut where these are rounded, fp32
+// gradients were off by up to 4e-5; and 1M x 768 in fp32 takes 0.5 ms here, 1.2
+// there.)
+struct StreamOut {
+    float2* part;      // forward
+    unsigned* ticket;
+    void* g;           // PROB: G of the piece in T, fp32 as three bf16 planes
+    int64_t ldg, plane, row0;
+    const float* stats;
+    int64_t ignore;
+};
+
+template <typename T, int NQ, int U, bool PROB>
 __global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
     xent_stream_kernel(const T* q, int nq, int64_t ldq, const T* x, int64_t n, int64_t ldx, int d, const int64_t* targets,
-                       float c, float2* part, unsigned* ticket) {
+                       float c, const __grid_constant__ StreamOut out) {
     constexpr int E = 16 / sizeof(T), P = E / 2;  // elements and pairs of a unit
     constexpr int R = stream_rows(U), V = R * NQ, kDup = 32 / V;
     __shared__ float2 sj[NT / 32][NQ];
     chain_wait();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0u;
+    if (!PROB && blockIdx.x == 0 && threadIdx.x == 0) *out.ticket = 0u;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int full = d / E, units = (d + E - 1) / E;
     // A row's last unit may reach behind d, but not behind the row's stride, which
@@ -344,7 +379,8 @@ __global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
             for (int i = 0; i < P; ++i) qv[b][u * P + i] = v[i];
         }
     const int row = lane / kDup / NQ, bq = lane / kDup % NQ;  // of the sum this lane ends up with
-    const int64_t tgt = bq < nq ? targets[bq] : -1;
+    const GTerm term = PROB && bq < nq ? GTerm(out.stats, targets, bq, nq, out.ignore, out.row0) : GTerm();
+    const int64_t tgt = PROB || bq >= nq ? -1 : targets[bq];
     const int64_t w = static_cast<int64_t>(blockIdx.x) * (NT / 32) + warp;
     const int64_t nw = static_cast<int64_t>(gridDim.x) * (NT / 32);
     int64_t r0 = w * R;
@@ -402,7 +438,22 @@ __global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
             }
         }
         const int64_t r = r0 + row;
-        if (r < n && r != tgt) {
+        if constexpr (PROB) {
+            if (r < n && bq < nq && lane % kDup == 0) {
+                float v = term.zero ? 0.f : r == term.tgt ? -kGScale : ex2(fmaf(s[0], c, -term.m) - term.lz);
+                const int64_t at = bq * out.ldg + r;
+                if constexpr (sizeof(T) == 2) {
+                    static_cast<T*>(out.g)[at] = from_f<T>(v);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        const __nv_bfloat16 h = __float2bfloat16_rn(v);
+                        static_cast<__nv_bfloat16*>(out.g)[k * out.plane + at] = h;
+                        v -= __bfloat162float(h);  // exact
+                    }
+                }
+            }
+        } else if (r < n && r != tgt) {
             if (s[0] > m) {
                 z *= ex2((m - s[0]) * c);
                 m = s[0];
@@ -411,18 +462,20 @@ __global__ void __launch_bounds__(NT, NQ == 1 ? 2 : 1)
             z += ex2(fmaf(s[0], c, -mb));
         }
     }
-    // the warp's R sets of a query, in the first lanes' order, then the block's
+    if constexpr (!PROB) {
+        // the warp's R sets of a query, in the first lanes' order, then the block's
 #pragma unroll
-    for (int o = 16; o >= kDup * NQ; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o), oz = __shfl_xor_sync(0xffffffffu, z, o);
-        join(m, z, om, oz, c);
-    }
-    if (row == 0 && lane % kDup == 0) sj[warp][bq] = make_float2(m, z);
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) < nq) {
-        float2 a = sj[0][threadIdx.x];
-        for (int k = 1; k < NT / 32; ++k) join(a.x, a.y, sj[k][threadIdx.x].x, sj[k][threadIdx.x].y, c);
-        part[threadIdx.x * gridDim.x + blockIdx.x] = a;
+        for (int o = 16; o >= kDup * NQ; o >>= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m, o), oz = __shfl_xor_sync(0xffffffffu, z, o);
+            join(m, z, om, oz, c);
+        }
+        if (row == 0 && lane % kDup == 0) sj[warp][bq] = make_float2(m, z);
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < nq) {
+            float2 a = sj[0][threadIdx.x];
+            for (int k = 1; k < NT / 32; ++k) join(a.x, a.y, sj[k][threadIdx.x].x, sj[k][threadIdx.x].y, c);
+            out.part[threadIdx.x * gridDim.x + blockIdx.x] = a;
+        }
     }
 }
 
@@ -793,24 +846,11 @@ struct ProbPolicy {
             return true;
         }
     };
-    struct Epi {
-        float m, lz;
-        int64_t tgt;
-        bool zero;  // an ignored query, one whose target is certain, or none
-    };
+    using Epi = GTerm;
 
     __device__ __forceinline__ void begin(Epi& e, const Job& j, const TileCtx& c) const {
         const int64_t b = j.m0 + c.row;
-        e.zero = true;
-        e.tgt = -1;
-        e.m = e.lz = 0.f;
-        if (b >= a.nq) return;
-        const int64_t t = a.targets[b];
-        const float rest = -expm1f(-a.stats[2 * a.nq + b]);  // 1 - p_t
-        e.zero = t == a.ignore || rest == 0.f;
-        if (!e.zero) e.tgt = t - a.row0;
-        e.m = a.stats[b];
-        e.lz = a.stats[a.nq + b] + log2f(rest) - kGLog2;
+        e = b < a.nq ? GTerm(a.stats, a.targets, b, a.nq, a.ignore, a.row0) : GTerm();
     }
 
     __device__ __forceinline__ void chunk(Epi& e, const Job& j, const TileCtx& c, int col,
@@ -818,8 +858,6 @@ struct ProbPolicy {
         const int y = j.m0 + c.row - c.lane, x = j.n0 + col;
         if (y >= a.nq || x >= a.n) return;
         float v[32];
-        // two roundings, of the exponent relative to the largest logit and of
-        // the one relative to their sum: both small for the terms that count
         const uint64_t c2 = pack2(a.c, a.c), m2 = pack2(-e.m, -e.m), z2 = pack2(-e.lz, -e.lz);
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -1214,13 +1252,17 @@ bool streamed(int dtype, int64_t nq, int d) {
     return nq >= 1 && nq <= (dtype == RDB_F32 ? 4 : 1) && d <= ST_MAX_DIM;
 }
 
+int stream_blocks(int64_t nq, int64_t rows) {
+    return (int)std::min<int64_t>((rows + 31) / 32, (nq == 1 ? 2LL : 1LL) * num_sms());
+}
+
 FwdPlan fwd_plan(int dtype, int64_t nq, int64_t n, int d) {
     FwdPlan p{};
     const int64_t dp = up(d, 8);
     p.stream = streamed(dtype, nq, d);
     if (p.stream) {
         p.pieces = p.groups = 1;
-        p.slots = (int)std::min<int64_t>((n + 31) / 32, (nq == 1 ? 2LL : 1LL) * num_sms());
+        p.slots = stream_blocks(nq, n);
         return p;
     }
     p.direct = f32_direct(dtype, nq);
@@ -1264,6 +1306,7 @@ FwdWs fwd_ws(void* base, const FwdPlan& p, int dtype, int64_t nq, int d) {
 
 struct BwdPlan {
     int64_t rows;  // rows per piece
+    bool stream;   // rows past CUDA cores (probabilities)
     bool direct;   // fp32 rows split on the way (dq, probabilities)
     bool dx_sums;  // dx of a piece in fp32 first
     int pieces, planes, nqb, nt, nkb, nseg, kq, dp;
@@ -1276,6 +1319,7 @@ int64_t rounds(int64_t jobs, int64_t workers) { return (jobs + workers - 1) / wo
 
 BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool need_dx) {
     BwdPlan p;
+    p.stream = streamed(dtype, nq, d);
     p.direct = f32_direct(dtype, nq);
     p.planes = dtype == RDB_F32 ? 3 : 1;
     p.nseg = dtype == RDB_F32 ? 6 : 1;
@@ -1396,6 +1440,29 @@ int piece_operand(int dtype, const void* x, int64_t r0, int64_t rows, int64_t ld
     return split_rows(base, rows, ldx, d, xp, s);
 }
 
+template <typename T, int NQ, bool PROB>
+int launch_stream_t(const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
+                    const int64_t* targets, float c, const StreamOut& out, int blocks, cudaStream_t s) {
+    constexpr int k = sizeof(T) == 4 ? 2 : 1;  // units of 8 elements
+    const auto kernel = d * (int)sizeof(T) <= 512 ? xent_stream_kernel<T, NQ, 1, PROB>
+                        : d <= 256                ? xent_stream_kernel<T, NQ, k, PROB>
+                        : d <= 512                ? xent_stream_kernel<T, NQ, 2 * k, PROB>
+                        : d <= 768                ? xent_stream_kernel<T, NQ, 3 * k, PROB>
+                                                  : xent_stream_kernel<T, NQ, 4 * k, PROB>;
+    return launch_chained(kernel, (unsigned)blocks, NT, 0, s, static_cast<const T*>(q), (int)nq, ldq,
+                          static_cast<const T*>(x), n, ldx, d, targets, c, out);
+}
+
+template <bool PROB>
+int launch_stream(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
+                  const int64_t* targets, float c, const StreamOut& out, int blocks, cudaStream_t s) {
+    const auto launch = dtype == RDB_BF16  ? launch_stream_t<__nv_bfloat16, 1, PROB>
+                        : dtype == RDB_F16 ? launch_stream_t<__half, 1, PROB>
+                        : nq == 1          ? launch_stream_t<float, 1, PROB>
+                                           : launch_stream_t<float, 4, PROB>;
+    return launch(q, nq, ldq, x, n, ldx, d, targets, c, out, blocks, s);
+}
+
 template <typename T>
 int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
                const int64_t* targets, float scale, int64_t ignore, int reduction, const float* grad,
@@ -1434,9 +1501,9 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
                                scan ? (unsigned)std::min<int64_t>((items + NT - 1) / NT, num_sms()) : elementwise_blocks(items),
                                NT, 0, s, static_cast<const T*>(q), nq, ldq, d, wt, w.wparts, nparts, w.wmax, w.qw, d8));
     }
-    Planes qo;
-    RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
-    CUtensorMap mq, mqw;
+    Planes qo{w.qp, d8, nq * d8, 3};
+    if (!p.stream || dtype != RDB_F32) RDB_TRY(piece_operand(dtype, q, 0, nq, ldq, d, w.qp, &qo, s));
+    CUtensorMap mq, mqw;  // (mq of streamed queries is read by nobody)
     RDB_TRY(operand_map(&mq, dtype, qo, d, nq, tile_box_rows(nq, 128)));
     mqw = mq;
     if (dx) RDB_TRY(operand_map(&mqw, dtype, Planes{w.qw, d8, nq * d8, p.planes}, d, nq, 0));
@@ -1485,15 +1552,20 @@ int backward_t(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x,
         const int64_t tiles = (rows + pa.width - 1) / pa.width * p.nqb;
         RDB_CHECK_ARG(tiles < (1LL << 31), "too many tiles for one launch");
         pa.njobs = (int)tiles;
-        if (p.direct) {
+        if (p.stream)
+            RDB_TRY(launch_stream<true>(dtype, q, nq, ldq, static_cast<const T*>(x) + r0 * ldx, rows, ldx, d, targets,
+                                        pa.c, StreamOut{nullptr, nullptr, w.g, p.rows, nq * p.rows, r0, stats, ignore},
+                                        stream_blocks(nq, rows), s));
+        else if (p.direct)
             RDB_TRY(launch_chained(xent_prob_f32_kernel, (unsigned)std::min<int64_t>(num_sms(), tiles), TF_THREADS,
                                    TF_SMEM, s, mq, mg, xr, pa, st));
-        } else {
+        if (!p.direct) {
             Planes xo;
             RDB_TRY(piece_operand(dtype, x, r0, rows, ldx, d, w.xp, &xo, s));
             RDB_TRY(operand_map(&mx, dtype, xo, d, rows, pa.width / 2));
             RDB_TRY(operand_map(&mxmn, dtype, xo, d, rows, 0));
-            RDB_TRY(launch_chained(xent_prob_kernel<T>, 2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS,
+            if (!p.stream)
+                RDB_TRY(launch_chained(xent_prob_kernel<T>, 2 * (unsigned)std::min<int64_t>(pairs, tiles), TT_THREADS,
                                    TT_SMEM, s, mq, mx, mg, pa, bf16, st));
         }
 
@@ -1589,28 +1661,6 @@ int tile_pass(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, 
     return RDB_OK;
 }
 
-template <typename T, int NQ>
-int launch_stream(const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
-                  const int64_t* targets, float c, const FwdPlan& p, const FwdWs& w, cudaStream_t s) {
-    constexpr int k = sizeof(T) == 4 ? 2 : 1;  // units of 8 elements
-    const auto kernel = d * (int)sizeof(T) <= 512 ? xent_stream_kernel<T, NQ, 1>
-                        : d <= 256                ? xent_stream_kernel<T, NQ, k>
-                        : d <= 512                ? xent_stream_kernel<T, NQ, 2 * k>
-                        : d <= 768                ? xent_stream_kernel<T, NQ, 3 * k>
-                                                  : xent_stream_kernel<T, NQ, 4 * k>;
-    return launch_chained(kernel, (unsigned)p.slots, NT, 0, s, static_cast<const T*>(q), (int)nq, ldq,
-                          static_cast<const T*>(x), n, ldx, d, targets, c, w.part, w.ticket);
-}
-
-int stream_pass(int dtype, const void* q, int64_t nq, int64_t ldq, const void* x, int64_t n, int64_t ldx, int d,
-                const int64_t* targets, float c, const FwdPlan& p, const FwdWs& w, cudaStream_t s) {
-    const auto launch = dtype == RDB_BF16  ? launch_stream<__nv_bfloat16, 1>
-                        : dtype == RDB_F16 ? launch_stream<__half, 1>
-                        : nq == 1          ? launch_stream<float, 1>
-                                           : launch_stream<float, 4>;
-    return launch(q, nq, ldq, x, n, ldx, d, targets, c, p, w, s);
-}
-
 }  // namespace
 }  // namespace rdb
 
@@ -1638,7 +1688,8 @@ int rdb_softmax_xent(int dtype, const void* q, int64_t nq, int64_t ldq, const vo
     const float c = (float)(scale * kLog2e);
     if (nq > 0) {
         if (p.stream)
-            RDB_TRY(stream_pass(dtype, q, nq, ldq, x, n, ldx, d, targets, c, p, w, s));
+            RDB_TRY(launch_stream<false>(dtype, q, nq, ldq, x, n, ldx, d, targets, c,
+                                         StreamOut{w.part, w.ticket, nullptr, 0, 0, 0, nullptr, 0}, p.slots, s));
         else
             RDB_TRY(tile_pass(dtype, q, nq, ldq, x, n, ldx, d, targets, c, p, w, s));
         const bool wide = nq <= num_sms();

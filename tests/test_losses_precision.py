@@ -1,11 +1,11 @@
 """Softmax cross entropy: digits of the gradients where weights differ by orders
-of magnitude, and of long sums.
+of magnitude, of long sums, and of the few queries that are streamed.
 
 Tolerances as in test_losses.py; what is added to them is derived at each test.
 """
 import pytest
 import torch
-from test_losses import DT, IGN, Ref, U32, UNDERFLOW, half_step, loss_fn, make, run_all, within
+from test_losses import DT, IGN, Ref, U32, UNDERFLOW, half_step, loss_fn, make, relative, run_all, within
 
 
 def fp16_row_tolerance(r, q, x, t, scale, w):
@@ -187,3 +187,35 @@ def test_row_gradient_of_many_queries(device, dim, dtype):
     assert ((dx[1:].double() - want).abs() <= tol).all(), ((dx[1:].double() - want).abs() / want).max().item()
     # the target's row: (p - 1) of every query
     assert ((dx[0].double() + (n - 1) * want).abs() <= (n - 1) * tol).all()
+
+
+# ------------------------------------------------------- streamed few queries
+@pytest.mark.gpu
+@pytest.mark.parametrize("near", [0.0, 0.6, 0.9])
+@pytest.mark.parametrize("nq,n,d", [(1, 20000, 768), (4, 20000, 768), (2, 3000, 1024), (3, 5000, 200), (1, 900, 64)])
+@pytest.mark.parametrize("dtype", sorted(DT))
+def test_errors_in_norm_of_few_queries(device, nq, n, d, dtype, near):
+    """As test_errors_in_norm at sizes whose forward pass streams the rows (one
+    query, fp32 up to four), also where many rows that are not the target lie close
+    to the query and carry the weight: the statistics and G come from logits that
+    are rounded alike."""
+    q, x, t, w = make(nq, n, d, DT[dtype], seed=n + d)
+    if near:
+        g = torch.Generator().manual_seed(7)
+        x = x.double()
+        for b in range(nq):
+            k = torch.randperm(n, generator=g)[:20]
+            k = k[~torch.isin(k, t)]
+            noise = torch.nn.functional.normalize(torch.randn(len(k), d, generator=g, dtype=torch.float64), dim=1)
+            x[k] = torch.nn.functional.normalize(near * q[b].double() + (1 - near) * noise, dim=1)
+        x = x.to(DT[dtype])
+    r = Ref(q, x, t, 20.0, w)
+    loss, dq, dx = run_all(q, x, t, w)
+    # One loss is no mean of many, and logits come up to 20: the exponent of a part's
+    # sum and of its join are rounded by u32 of 20 log2 e, twice each, 80 u32.  Two and
+    # more 16-bit queries run on the tensor cores, which cut a logit by up to 2^-22 of
+    # itself at each of d / 16 instructions while it grows: 20 d / 16 * 2^-23.
+    cut = 20 * d / 16 * 2.0 ** -23 if nq > 1 and dtype != "fp32" else 0.0
+    assert ((loss.cpu().double() - r.loss).abs() <= 2.0 ** -20 * r.loss + 80 * U32 + cut).all()
+    bound = 2.0 ** -18 if dtype == "fp32" else half_step(DT[dtype])
+    assert relative(dq, r.dq) < bound and relative(dx, r.dx) < bound, (relative(dq, r.dq), relative(dx, r.dx))
