@@ -110,7 +110,17 @@ int rdb_row_sqnorms(int dtype, const void* x, int64_t n, int d, float* out, void
  *              relative to its 1 - p_t.  The backward call's reduction and
  *              targets must be the forward's.
  * fp32 operands are multiplied as three bf16 planes (24 bits); infinities in
- * them give NaN.  ws: 16-byte aligned; backward at most about 2 GB. */
+ * them, and values above 3.39e38 (the largest bf16), may give NaN.
+ * ws: 16-byte aligned, of at most (e: 2 bytes, fp32 6; d up to a multiple of 32)
+ *   forward   32 MB + 64 bytes a query; fp32: 6 d bytes a query, and for more than
+ *             128 queries 256 MB of rows' planes at a time, each with 10 MB of
+ *             parts or 32 bytes a query
+ *   backward  G of a piece of the rows, e nq bytes a row: 512 MB, or 2 GB where
+ *             4,096 rows take that much, and no fewer than 256 rows; dq: 64 MB,
+ *             or 4 d bytes a query; dx: e d bytes a query, and 512 MB where more
+ *             than 8,192 16-bit queries need fp32 sums of a piece; fp32: 6 d
+ *             bytes a query, and 256 MB of planes for more than 128 queries
+ *             (256 rows of planes or sums where the rows are longer than that). */
 #define RDB_REDUCE_NONE 0
 #define RDB_REDUCE_MEAN 1
 #define RDB_REDUCE_SUM 2

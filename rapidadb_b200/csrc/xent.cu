@@ -21,10 +21,9 @@
 //
 // Backward: the rows in pieces.  Per piece one launch recomputes the logits and
 // writes a [nq, rows] workspace of G in the operands' type, every row of it over
-// its 1 - p_t (at most 512 MB), one launch multiplies it both ways: dx rows
-// directly (K = nq), dq into fp32 partial sums (K = rows, split over several
-// tiles when there are few queries), joined at the end.  No atomics on values:
-// every sum has a fixed order.
+// its 1 - p_t, one launch multiplies it both ways: dx rows directly (K = nq), dq
+// into fp32 partial sums (K = rows, split over several tiles when there are few
+// queries), joined at the end.  No atomics on values: every sum has a fixed order.
 //
 // Bound: the products, 2 nq n d FLOP each, one forward and three backward.  4,096
 // queries, 131,072 rows, d = 768, bf16: forward 578 us (1.43 PFLOP/s, the rate
@@ -1323,23 +1322,25 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
     p.direct = f32_direct(dtype, nq);
     p.planes = dtype == RDB_F32 ? 3 : 1;
     p.nseg = dtype == RDB_F32 ? 6 : 1;
+    p.kq = (int)((nq + 63) / 64);
+    p.dp = (int)up(d, 32);
+    p.dx_sums = need_dx && dtype != RDB_F32 && p.kq > kRun16;
     const int64_t col = std::max<int64_t>(1, nq * 2 * p.planes);  // bytes of G per row
     // G of a piece: 512 MB.  Pieces that stay in L2 (64 MB) have fewer tiles to
     // deal out and more launches, and the products are bound by the tensor
     // cores, not by reading G: 4,096 x 131,072 x 768 both gradients 2,013 us at
     // 64 MB, 1,971 at 128, 1,924 at 256, 1,865 at 512.  At least 4,096 rows
-    // within 2 GB: the partial sums of dq are read and written once a piece.
+    // within 2 GB: the partial sums of dq are read and written once a piece.  Never
+    // less than a tile's 256 rows.
     int64_t most = (512LL << 20) / col;
     if (most < 4096) most = std::max(most, std::min<int64_t>(4096, (2LL << 30) / col));
     if (dtype == RDB_F32 && !p.direct) most = std::min<int64_t>(most, (256LL << 20) / (6 * up(d, 8)));
+    if (p.dx_sums) most = std::min<int64_t>(most, (512LL << 20) / (4LL * p.dp));  // (counts from d = 4,096 on)
     p.rows = piece_rows(n, most);
     p.pieces = (int)((n + p.rows - 1) / p.rows);
     p.nqb = (int)std::max<int64_t>(1, (nq + TT_M - 1) / TT_M);
     p.nt = (d + TT_N - 1) / TT_N;
     p.nkb = (d + 63) / 64;
-    p.kq = (int)((nq + 63) / 64);
-    p.dp = (int)up(d, 32);
-    p.dx_sums = need_dx && dtype != RDB_F32 && p.kq > kRun16;
     p.q_width = p.direct ? TF_N : TT_N;
     p.q_nt = (d + p.q_width - 1) / p.q_width;
     // K splits of dq: the split that ends first, tiles dealt out in turn; a
