@@ -219,3 +219,61 @@ def test_errors_in_norm_of_few_queries(device, nq, n, d, dtype, near):
     assert ((loss.cpu().double() - r.loss).abs() <= 2.0 ** -20 * r.loss + 80 * U32 + cut).all()
     bound = 2.0 ** -18 if dtype == "fp32" else half_step(DT[dtype])
     assert relative(dq, r.dq) < bound and relative(dx, r.dx) < bound, (relative(dq, r.dq), relative(dx, r.dx))
+
+
+# --------------------------------------------------- close rows on the tile loops
+@pytest.mark.gpu
+@pytest.mark.parametrize("near", [0.6, 0.9])
+@pytest.mark.parametrize("nq,n,d", [(5, 9000, 768), (128, 4000, 256), (129, 4000, 256), (300, 8000, 512)])
+@pytest.mark.parametrize("dtype", sorted(DT))
+def test_errors_in_norm_beside_close_rows(device, nq, n, d, dtype, near):
+    """Twenty rows beside each query that are not its target carry the weight.  Their
+    logits, up to 20, come from the tensor cores, which cut a sum of d products at
+    d / 16 instructions (fp32: of the largest planes) by up to 2^-22 of itself while
+    it grows: the loss moves by 20 d / 16 * 2^-23 at most; G, over a sum of the same
+    terms, by their differences alone."""
+    q, x, t, w = make(nq, n, d, DT[dtype], seed=n + d)
+    g = torch.Generator().manual_seed(7)
+    x = x.double()
+    free = torch.randperm(n, generator=g)
+    free = free[~torch.isin(free, t)]
+    for b in range(nq):
+        k = free[20 * b:20 * b + 20]
+        noise = torch.nn.functional.normalize(torch.randn(len(k), d, generator=g, dtype=torch.float64), dim=1)
+        x[k] = torch.nn.functional.normalize(near * q[b].double() + (1 - near) * noise, dim=1)
+    x = x.to(DT[dtype])
+    r = Ref(q, x, t, 20.0, w)
+    loss, dq, dx = run_all(q, x, t, w)
+    cut = 20 * d / 16 * 2.0 ** -23
+    assert ((loss.cpu().double() - r.loss).abs() <= 2.0 ** -20 * r.loss + 80 * U32 + cut).all()
+    bound = 2.0 ** -18 if dtype == "fp32" else half_step(DT[dtype])
+    assert relative(dq, r.dq) < bound and relative(dx, r.dx) < bound, (relative(dq, r.dq), relative(dx, r.dx))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("nq,n,d", [(8192, 3000, 40), (8193, 3000, 40), (9000, 45000, 71), (16500, 700, 256)])
+def test_row_gradient_past_one_run(device, nq, n, d, dtype):
+    """At and past the queries whose products fit one run, over one piece of the rows
+    and two: errors in norm, three independent roundings."""
+    g = torch.Generator(device="cuda").manual_seed(nq)
+    unit = torch.nn.functional.normalize
+    x = unit(torch.randn(n, d, generator=g, device=device), dim=1).to(DT[dtype])
+    t = torch.randint(0, n, (nq,), generator=g, device=device)
+    q = unit(x[t].float() + unit(torch.randn(nq, d, generator=g, device=device), dim=1), dim=1).to(DT[dtype])
+    t[3::50] = IGN
+    w = torch.rand(nq, generator=g, device=device) + 0.1
+    a, b = q.clone().requires_grad_(), x.clone().requires_grad_()
+    dq, dx = torch.autograd.grad(loss_fn(a, b, t, scale=8.0, reduction="none"), (a, b), w)
+    xd = x.double()
+    want_q, want_x = torch.zeros(nq, d, dtype=torch.float64, device=device), torch.zeros_like(xd)
+    for part in torch.arange(nq, device=device).split(1000):
+        part = part[t[part] != IGN]
+        p = torch.softmax(8.0 * q[part].double() @ xd.T, 1)
+        p[torch.arange(len(part), device=device), t[part]] -= 1.0
+        p *= 8.0 * w[part].double()[:, None]
+        want_q[part] = p @ xd
+        want_x += p.T @ q[part].double()
+    u = half_step(DT[dtype])
+    assert relative(dq, want_q.cpu()) < u and relative(dx, want_x.cpu()) < u
+    assert (dq[3::50] == 0).all()
