@@ -107,11 +107,17 @@ int rdb_row_sqnorms(int dtype, const void* x, int64_t n, int d, float* out, void
  *   dq / dx    gradients in `dtype` (NULL: not wanted); sums over queries and
  *              rows run in fp32 in a fixed order.  16-bit operands: the matrix G
  *              is rounded to their type once on the way, every query's row
- *              relative to its 1 - p_t.  The backward call's reduction and
- *              targets must be the forward's.
+ *              relative to its 1 - p_t, and for dx the query, times its weight
+ *              and 1 - p_t, once more: in norm 1.1 (dq) and 1.4 times (dx) the
+ *              error of the result's own rounding.  The backward call's reduction and targets must be
+ *              the forward's.
+ * Logits are summed in fp32 by the tensor cores, which cut towards zero, but for
+ * the target's (rounded): a loss is off by about 4e-7 of itself, and where rows
+ * that are no target lie beside the query by up to 3e-5 (d = 768) or 1e-4 (2,048)
+ * of a unit in fp32, three times that in 16 bits.
  * fp32 operands are multiplied as three bf16 planes (24 bits); infinities in
  * them, and values above 3.39e38 (the largest bf16), may give NaN.
- * ws: 16-byte aligned, of at most (e: 2 bytes, fp32 6; d up to a multiple of 32)
+ * ws (the same for every reduction): 16-byte aligned, of at most (e: 2 bytes, fp32 6; d up to a multiple of 32)
  *   forward   32 MB + 64 bytes a query; fp32: 6 d bytes a query, and for more than
  *             128 queries 256 MB of rows' planes at a time, each with 10 MB of
  *             parts or 32 bytes a query
@@ -181,7 +187,9 @@ int rdb_flat_search(int metric, int dtype, const void* q, int64_t nq, int64_t ld
  * python/rapidadb/config.py:21-26) without defining it; here a row x is
  * stored as scale = max_i |x_i| / 127 (fp32 division; 0 for a zero row) and
  * codes c_i = rint(x_i / scale) clamped to [-127, 127] (ties to even), and
- * stands for the dequantised row x^_i = fl(scale * c_i).
+ * stands for the dequantised row x^_i = fl(scale * c_i).  Rows are meant to be
+ * finite: the maximum passes over NaN, and a quotient that is NaN (a NaN element,
+ * an infinite one over the infinite scale) has the code -127.
  *   rdb_sq8_encode        x [n, d] (dtype, stride ldx) -> codes [n, ldc] int8
  *                         (columns d .. ldc - 1 zero), scales [n]
  *   rdb_sq8_row_values    per-row metric values of x^ (as rdb_vec_values)

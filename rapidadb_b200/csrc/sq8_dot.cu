@@ -12,8 +12,9 @@
 // Otherwise the tcgen05 tile loop (kind::i8) with the rows as the tile's M: few
 // queries then make a narrow tile, and as a thread of the epilogue owns one row,
 // a warp's store of one query's scores is 32 consecutive elements and needs no
-// staging (staged TMA stores measured the same).  32 x 100,000 x 768: 20 us from
-// a cold L2, the codes' bytes; 4,096 x 16,384 x 1,024 in bf16: 77 us, of which the products take
+// staging (staged TMA stores spilled registers and measured the same).  32 x
+// 100,000 x 768: 20 us from a cold L2, where the codes' bytes take 12 and the scores'
+// 2; 32 x 1M x 768 134, 1.1 times its bytes; 4,096 x 16,384 x 1,024 in bf16: 77 us, of which the products take
 // 45 and the conversion and scaling of 67M sums the rest.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -45,7 +46,10 @@ __device__ __forceinline__ float score(float qs, float xs, int acc) {
 
 constexpr int GV_THREADS = 256;
 constexpr int GV_LANES = 8;               // lanes per row: 128 bytes of a row per load
-constexpr int GV_BATCH = 6;               // 16-byte loads a lane has in flight
+// 16-byte loads a lane has in flight.  Rows of 768 codes take one batch, longer ones
+// end with a part of one, which costs nothing: 1M x 1,024 154 us (6.7 TB/s), 700,000
+// x 1,152 123 (6.6), 1M x 768 117 (6.6).
+constexpr int GV_BATCH = 6;
 constexpr int GV_SMEM = 48 * 1024;        // query codes
 
 // The warps take 4 R rows each in turn (shares of their own, rows far apart, cost
@@ -147,7 +151,7 @@ template <typename T, int NQ>
 int launch_few(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
                int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
     // the whole row in as few loads as it takes, or GV_BATCH at a time: 4M x 128
-    // in 109 us, 2M x 384 in 121 (GV_BATCH for all: 200 and 129)
+    // in 102 us, 2M x 384 in 121 (GV_BATCH for all: 200 and 129)
     const auto kernel = d <= 128   ? sq8_few_kernel<T, NQ, 1>
                         : d <= 256 ? sq8_few_kernel<T, NQ, 2>
                         : d <= 512 ? sq8_few_kernel<T, NQ, 4>
@@ -288,10 +292,12 @@ int launch_tile(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, cons
 template <typename T>
 int launch_dot(const int8_t* qc, const float* qs, int64_t nq, int64_t ldq, const int8_t* xc, const float* xs,
                int64_t n, int64_t ldx, int d, void* out, int64_t ldo, cudaStream_t s) {
-    // One or two queries: 100,000 x 768 in 8.8 / 11.7 us against 17.8 of the tile
-    // loop (1,000 rows: 2.8 / 5.2; 4M x 128: 109 / 129 us against 198).  From four
-    // on dp4a costs more than the codes' bytes: 150 us for 1M x 768 (4M x 128: 385),
-    // the tile loop 134 (198).
+    // One or two queries, calls in a row: 1M x 768 in 117 / 118 us against 130 of the
+    // tile loop, 1M x 1,024 154 against 163, 4M x 128 102 / 103 against 197, and from
+    // L2 100,000 x 768 9.1 / 12.0 against 18.0 and 1,000 x 768 4.4 against 7.2 (100,000
+    // x 768 with 256 MB written between the calls: 24.6 for both, against 26.7).  From
+    // four on dp4a costs more than the codes' bytes: 150 us for 1M x 768 (4M x 128:
+    // 385), the tile loop 134 (198).
     const int64_t dp = (d + 15) / 16 * 16;
     if (nq == 1 && dp <= GV_SMEM) return launch_few<T, 1>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);
     if (nq == 2 && 2 * dp <= GV_SMEM) return launch_few<T, 2>(qc, qs, nq, ldq, xc, xs, n, ldx, d, out, ldo, s);

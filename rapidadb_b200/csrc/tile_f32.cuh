@@ -19,11 +19,12 @@
 //                 way B lies (below)
 //   warps 10..17  epilogue, two per TMEM lane quadrant; policies as in
 //                 tile_tc.cuh
-// A stage is 96 KB (three planes of both operands): two of them.  What bounds it
-// is shared memory: per K block the MMAs read 192 KB of operands, 96 KB are
-// written, 32 KB pass through L1, 2,500 cycles at 128 bytes a cycle, where the
-// products alone take 1,536.  128 x 100,000 x 768 forward: 144 us (the rows' HBM
-// time is 47); with the planes written to memory first 430.
+// A stage is 96 KB (three planes of both operands): two of them.  Per K block the
+// MMAs read 192 KB of operands, 96 KB are written, 32 KB pass through L1: 2,500
+// cycles of shared memory at 128 bytes a cycle, where the products alone take
+// 1,536.  128 x 100,000 x 768 forward: 144 us, of which that explains 92 (the rows'
+// HBM time is 47); with two stages a late converter or commit holds up everything.
+// With 256 MB written before the call 159, by planes in memory 326.
 //
 // B is K-major (tile rows = matrix rows, K along the row) or MN-major (tile rows
 // = matrix columns, K = matrix rows).

@@ -11,8 +11,8 @@
 //   warps 2..17 epilogue, four per TMEM lane quadrant: a thread owns one row of
 //               its CTA's 128 and every fourth 32-column chunk of the tile (at
 //               most two).  It takes both into registers and releases the
-//               accumulator before it works on them, so the MMAs run up to two
-//               tiles ahead.  (4,096 x 131,072 x 128 forward: 219 us, 306 with
+//               accumulator before it works on them, so the MMAs run ahead by up
+//               to as many tiles as there are accumulators, 512 / P::kAccCols.  (4,096 x 131,072 x 128 forward: 219 us, 306 with
 //               eight warps and one chunk in flight, 137 with no epilogue at
 //               all; at d = 768 586, 613 and 556 us.)
 // An operand lies either K-major in memory (a row's K elements contiguous: one
@@ -44,8 +44,9 @@
 //                                  that wide)
 //   p.end(epi, job, ctx)           after the tile's chunks
 //   p.finish(ctx)                  once, after the last tile
-// The epilogue's warps never wait for one another: they drift apart by up to
-// two tiles, so that one's exponentials overlap another's maxima and stores.
+// The epilogue's warps never wait for one another: they drift apart by up to as
+// many tiles (two of 256 columns, eight of 64), so that one's exponentials overlap
+// another's maxima and stores.
 //
 // Every mbarrier wait is bounded: a role that gives up raises the CTA's abort
 // flag and the device status word (also in its host copy), waits (bounded) for

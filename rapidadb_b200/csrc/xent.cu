@@ -1221,7 +1221,8 @@ struct FwdPlan {
 
 // Row splits of one piece: as many as give every pair the same number of rows
 // (in groups of 32), for the number of rounds that costs least; a split costs
-// about a third of a tile (its fill and parts).
+// about a third of a tile (its fill and parts).  A tile counts as 256 columns; of
+// the direct plan's 128 two count as one.
 int fwd_splits(int nqb, int64_t rows, int pairs) {
     const int64_t n32 = (rows + 31) / 32;
     int64_t best = 1;
@@ -1236,7 +1237,12 @@ int fwd_splits(int nqb, int64_t rows, int pairs) {
 }
 
 // fp32 rows are split on the way (tile_f32.cuh) where one block of 128 queries
-// reads them; more queries share planes written once per piece.
+// reads them; more queries share planes written once per piece.  100,000 x 768, us,
+// forward / forward and dq, on the way / by planes (cold L2): 5 queries 153 / 309
+// and 429 / 773, 128 queries 159 / 326 and 457 / 872; by planes alone 129 queries 313
+// / 847, 256 336 / 906, 1,024 832 / 2,530.  A block holds no more than 128 queries:
+// beyond, the rows would be split once per block, and two forward passes of 159 take
+// as long as the planes of 129 to 256.
 bool f32_direct(int dtype, int64_t nq) { return dtype == RDB_F32 && nq <= 128; }
 
 // A pass of CUDA cores where their products hide behind the rows' bytes: one
@@ -1345,7 +1351,11 @@ BwdPlan bwd_plan(int dtype, int64_t nq, int64_t n, int d, bool need_dq, bool nee
     p.q_nt = (d + p.q_width - 1) / p.q_width;
     // K splits of dq: the split that ends first, tiles dealt out in turn; a
     // tile costs about six K blocks on top of its own (fill, drain, store).
-    // Direct dq tiles have a launch of their own.
+    // Direct dq tiles have a launch of their own.  Limits: 64 splits (4 x 200,000 x
+    // 768 bf16 backward 137 us with up to 16, 126 with 32 to 256; 32 queries 159, 141
+    // with 32 to 128, 135 with 256), of the direct plan about one per SM (8 and 128 x
+    // 100,000 x 768 fp32: the same within 3 % from 40 to 320), and 64 MB of parts
+    // (4,096 x 131,072 x 768 1,371 us at 16 MB, 1,255 at 64 and at 256).
     const int64_t workers = p.direct ? num_sms() : tile_pairs(), kc = std::min(p.rows, up(n, 64)) / 64;
     const int64_t nx = need_dx && !p.direct ? (p.rows + TT_M - 1) / TT_M * p.nt : 0, lx = (int64_t)p.kq * p.nseg + 6;
     p.q_split = 1;

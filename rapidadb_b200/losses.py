@@ -36,9 +36,18 @@ def softmax_cross_entropy(queries: torch.Tensor, database: torch.Tensor, targets
         reduction:    "mean" over the queries that are not ignored (NaN when
                       all are), "sum" or "none" ([batch] losses).
 
-    The loss is float32; gradients have their tensor's dtype.  Gradients are
-    computed only for the inputs that require them, in a fixed order of sums
-    (the same call gives the same bits), and once: a backward pass with
+    The loss is float32; gradients have their tensor's dtype.  Sums are held in
+    float32.  16-bit gradients are rounded twice before their final rounding, the
+    matrix of probabilities and (for the rows' gradient) the weighted queries, each
+    to the operands' type: in norm about 1.1 (queries) and 1.4 times (rows) as far
+    from the exact value as the final rounding alone.  float32 operands are
+    multiplied as three bfloat16 planes; gradients are within 4e-6 in norm, and
+    infinities in operands give NaN.  The backward pass keeps no logits; its
+    workspace is the probabilities of a piece of the rows (512 MB, up to 2 GB for
+    very many queries) and a few values per element of the queries.
+
+    Gradients are computed only for the inputs that require them, in a fixed order
+    of sums (the same call gives the same bits), and once: a backward pass with
     ``create_graph=True`` raises.  To capture a step into a CUDA graph, run it
     once before, and take the gradients with ``torch.autograd.grad`` of leaves
     made inside the capture.
