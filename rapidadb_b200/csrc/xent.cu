@@ -714,9 +714,10 @@ __global__ void __launch_bounds__(NT)
 template <typename T>
 __device__ __forceinline__ float weight_top(const float2& m) {
     if constexpr (!std::is_same<T, __half>::value) return 1.f;
-    const float r = 32768.f * (m.x / m.y);  // (no less than 1/2: an element is at most 65,504)
-    if (!(m.y > 0.f) || isnan(r)) return 1.f;  // nothing to weigh, or infinite
-    return __uint_as_float(__float_as_uint(fminf(r, 0x1p100f)) & 0x7f800000u);
+    const float r = 32768.f * (m.x / m.y);
+    if (!(m.y > 0.f) || isnan(r)) return 1.f;  // nothing to weigh, or an infinite weight
+    // an element is at most 65,504: below 1/2 the product m.y has overflown
+    return __uint_as_float(__float_as_uint(fminf(fmaxf(r, 0.5f), 0x1p100f)) & 0x7f800000u);
 }
 
 // the three bf16 planes of 8 floats, plane stride in elements

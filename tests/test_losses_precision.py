@@ -107,7 +107,7 @@ def test_fp16_rows_gradient_of_odd_queries(device):
     q[2] = (torch.randn(d, generator=g) * 8000).half()
     t = torch.arange(12)
     for w in (torch.ones(12), torch.tensor([1e30] + [1.0] * 11), torch.tensor([1.0, 1e12, 2.0 ** -10] + [1.0] * 9),
-              torch.tensor([1e-30] * 12), torch.zeros(12)):
+              torch.tensor([1e-30] * 12), torch.zeros(12), torch.tensor([1.0, 1.0, 1e36] + [1.0] * 9)):
         dx = run_all(q, x, t, w, scale)[2]
         r = Ref(q, x, t, scale, w)
         inside = r.dx.abs() < 60000.0
