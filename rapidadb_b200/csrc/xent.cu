@@ -27,7 +27,7 @@
 //
 // Bound: the products, 2 nq n d FLOP each, one forward and three backward.  4,096
 // queries, 131,072 rows, d = 768, bf16: forward 578 us (1.43 PFLOP/s, the rate
-// cuBLAS holds for seconds is 1.40), probabilities 620, gradients 1,218.  Few
+// cuBLAS holds for seconds is 1.40), probabilities 620, gradients 1,240.  Few
 // queries: the rows' bytes, 1 x 1M x 768 bf16 225 us (6.8 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
